@@ -70,6 +70,12 @@ SIGNATURES = {
     "dsa_concat_and_cache_ds_mla": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _p, _i, _p, _p, _i64, _i, _p]),
     "dsa_indexer_qk_store": (_i, [_p, _i, _p, _i, _p, _i, _i64, _p, _i64, _p, _i64, _i, _p, _p, ctypes.c_float, _p,
                                   _p, _i64, _i, ctypes.c_float, _p, _i, _i, _p]),
+    "dsa_tree_mla_decode_workspace_bytes": (_sz, [_i, _i, _i]),
+    "dsa_tree_mla_decode": (_i, [_p, _i, _p, _p, _i, _p, _i, _i64, _i, _p, _i64, _i, _p, _p, _p, _i64, _i, _i, _i, _d,
+                                 _p, _sz, _p]),
+    "dsa_commit_draft_rows": (_i, [_p, _i, _i64, _i, _i, _p, _i64, _i, _p, _p, _i, _p, _i64, _i, _i, _p]),
+    "dsa_gather_cache": (_i, [_p, _i, _i64, _i, _p, _i, _i64, _i, _i, _p, _i64, _i, _p, _p, _i, _p]),
+    "dsa_rotary_embedding": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _p]),
 }
 
 

@@ -60,6 +60,54 @@ def forward_mqa_sparse(q: torch.Tensor, kv_cache: torch.Tensor, topk_indices_buf
     return o, lse
 
 
+def draft_tree_masks(parents: torch.Tensor):
+    """Masks and depths of draft trees, for tree_mla_decode and the rotary
+    positions. parents int [B, T <= 64]: the draft that draft i extends, or -1
+    for the context's last token; parents[b, i] < i (values outside [-1, i) are
+    taken as -1). Returns (mask int64 [B, T], bit j of [b, i] set when j is i
+    or an ancestor of i; depth int64 [B, T], 0 at the roots): draft i stands at
+    rotary position pre + depth. Pointer doubling, static shapes: CUDA-graph
+    safe."""
+    B, T = parents.shape
+    if T > 64:
+        raise RuntimeError(f"at most 64 drafts a request (got {T})")
+    i = torch.arange(T, device=parents.device)
+    up = parents.to(torch.int64)
+    up = torch.where((up >= 0) & (up < i), up, -1)
+    mask = (torch.ones_like(i) << i).expand(B, T).clone()
+    depth = torch.zeros(B, T, dtype=torch.int64, device=parents.device)
+    depth = torch.where(up >= 0, depth + 1, depth)
+    for _ in range(max(T - 1, 0).bit_length()):
+        on = up >= 0
+        at = up.clamp(min=0)
+        mask = torch.where(on, mask | mask.gather(1, at), mask)
+        depth = torch.where(on, depth + depth.gather(1, at), depth)
+        up = torch.where(on, up.gather(1, at), up)
+    return mask, depth
+
+
+def forward_mqa_tree(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                     tree_mask: torch.Tensor, scale: float, draft_lens: torch.Tensor | None = None,
+                     kv_lora_rank: int = 512):
+    """Verification of a tree of drafts: every draft attends its request's
+    context and its own ancestors in one pass over the paged latent cache
+    (where expand_spec_rows turns a line of drafts into independent rows).
+
+    q [B, T, H, 576], or the step's tokens [B * T, H, 576] with tree_mask [B,
+    T]; seq_lens counts the drafts. Returns (o in q's dtype and leading shape,
+    [.., H, 512], lse f32 [.., H]).
+    """
+    B, T = tree_mask.shape
+    lead = q.shape[:-1]
+    q4 = q.reshape(B, T, q.shape[-2], q.shape[-1])
+    out_dtype = q.dtype if q.dtype in (torch.float16, torch.bfloat16) else torch.float16
+    qk = q4 if q4.dtype == out_dtype and q4.is_contiguous() else q4.to(out_dtype).contiguous()
+    o = torch.empty(*qk.shape[:3], kv_lora_rank, dtype=out_dtype, device=q.device)
+    lse = torch.empty(qk.shape[:3], dtype=torch.float32, device=q.device)
+    ops.tree_mla_decode(o, lse, qk, kv_cache, block_table, seq_lens, tree_mask, float(scale), draft_lens)
+    return o.view(*lead, kv_lora_rank), lse.view(lead)
+
+
 def per_token_metadata(chunks, nd0: int, q_len: int, query_start_loc: torch.Tensor, block_table: torch.Tensor):
     """Per-token causal lengths and block-table rows for sparse prefill
     (triton_mla.py:414-466): validates that the indexer's chunk entries

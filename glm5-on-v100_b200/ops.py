@@ -484,6 +484,140 @@ def _indexer_qk_store_impl(q_out, weights_out, kv_cache, q, kw, slot_mapping, ln
                float(weight_scale), _vp(slot_mapping.contiguous()), T, H, _stream(q.device))
 
 
+def _same_device(dev, **tensors):
+    for name, t in tensors.items():
+        _check(t is None or (t.is_cuda and t.device == dev), f"{name} must be on {dev}")
+
+
+def _paged(block_table, lens, name, B):
+    _int32(block_table, "block_table")
+    _int32(lens, name)
+    _rowmajor(block_table, "block_table")
+    _check(block_table.size(0) >= B, f"block_table has fewer than {B} rows")
+
+
+def _latent_format(kv_cache):
+    """(format, elements per row) of a latent cache tensor."""
+    if kv_cache.dtype == torch.uint8:
+        _check(kv_cache.dim() >= 2 and kv_cache.size(-1) == DSMLA_ROW_BYTES,
+               "fp8 kv_cache last dim must be 656 (fp8_ds_mla layout)")
+        return L.DSA_FP8_DS_MLA, DSMLA_ROW_BYTES
+    _check(kv_cache.dtype in (torch.float16, torch.bfloat16) and kv_cache.dim() >= 2 and kv_cache.size(-1) == 576,
+           "kv_cache must be fp16/bf16 [.., page, 576] or uint8 fp8_ds_mla [.., page, 656]")
+    return _DTYPE[kv_cache.dtype], 576
+
+
+def _tree_mla_decode_impl(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, draft_lens, scale):
+    _check(q.is_cuda, "q must be a CUDA tensor")
+    _same_device(q.device, o=o, lse=lse, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens,
+                 tree_mask=tree_mask, draft_lens=draft_lens)
+    _check(q.dtype in (torch.float16, torch.bfloat16), "q must be fp16 or bf16")
+    _check(o.dtype in (torch.float16, torch.bfloat16), "o must be fp16 or bf16")
+    _check(lse.dtype == torch.float32, "lse must be fp32")
+    fmt, row = _latent_format(kv_cache)
+    _check(q.dim() == 4 and q.size(3) == 576, "q must be [B, T, n_head, 576]")
+    B, T, H = q.size(0), q.size(1), q.size(2)
+    _check(tuple(o.shape) == (B, T, H, 512) and tuple(lse.shape) == (B, T, H), "o/lse shape mismatch with q")
+    _check(q.is_contiguous() and o.is_contiguous() and lse.is_contiguous() and kv_cache.is_contiguous(),
+           "q, o, lse and kv_cache must be contiguous")
+    _paged(block_table, seq_lens, "seq_lens", B)
+    _check(seq_lens.dim() == 1 and seq_lens.numel() >= B, "seq_lens must be [B]")
+    _check(tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.size(0) >= B and
+           tree_mask.size(1) == T and (T <= 1 or tree_mask.stride(1) == 1),
+           "tree_mask must be int64 [B, T] with unit inner stride")
+    if draft_lens is not None:
+        _int32(draft_lens, "draft_lens")
+        _check(draft_lens.dim() == 1 and draft_lens.numel() >= B, "draft_lens must be [B]")
+        draft_lens = draft_lens.contiguous()
+    page = kv_cache.size(-2)
+    _check(page > 0, "kv_cache has no rows in a page")
+    with torch.cuda.device(q.device):
+        ws_bytes = int(L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        L.call("dsa_tree_mla_decode", _vp(o), _DTYPE[o.dtype], _vp(lse), _vp(q), _DTYPE[q.dtype], _vp(kv_cache), fmt,
+               kv_cache.numel() // row, page, _vp(block_table), max(block_table.stride(0), block_table.size(1)),
+               block_table.size(1), _vp(seq_lens.contiguous()), _vp(draft_lens), _vp(tree_mask),
+               max(tree_mask.stride(0), T), B, T, H, float(scale), _vp(ws), ws_bytes, _stream(q.device))
+
+
+def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens):
+    if not caches:
+        return
+    c0 = caches[0]
+    _check(c0.is_cuda and c0.dim() >= 2, "caches must be CUDA tensors [.., page, row]")
+    _same_device(c0.device, block_table=block_table, seq_lens=seq_lens, accepted=accepted, draft_lens=draft_lens)
+    for i, c in enumerate(caches):
+        _check(c.device == c0.device and c.shape == c0.shape and c.dtype == c0.dtype and c.is_contiguous(),
+               f"cache {i} must be contiguous with the shape, dtype and device of the first")
+    _check(len({c.data_ptr() for c in caches}) == len(caches), "the same cache twice in the list")
+    _check(accepted.dim() == 2, "accepted must be [B, n_accept]")
+    _int32(accepted, "accepted")
+    B, A = accepted.shape
+    _check(A <= 1 or accepted.stride(1) == 1, "accepted must have unit inner stride")
+    _paged(block_table, seq_lens, "seq_lens", B)
+    _check(seq_lens.dim() == 1 and seq_lens.numel() >= B, "seq_lens must be [B]")
+    _int32(draft_lens, "draft_lens")
+    _check(draft_lens.dim() == 1 and draft_lens.numel() >= B, "draft_lens must be [B]")
+    page, row_bytes = c0.size(-2), c0.size(-1) * c0.element_size()
+    if c0.numel() == 0:
+        return
+    ptrs = (ctypes.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
+    with torch.cuda.device(c0.device):
+        L.call("dsa_commit_draft_rows", ptrs, len(caches), c0.numel() // c0.size(-1), page, row_bytes,
+               _vp(block_table), max(block_table.stride(0), block_table.size(1)), block_table.size(1),
+               _vp(seq_lens.contiguous()), _vp(draft_lens.contiguous()), 64, _vp(accepted),
+               max(accepted.stride(0), A), A, B, _stream(c0.device))
+
+
+def _gather_cache_impl(out, cache, block_table, cu_seq_lens, seq_starts):
+    _check(out.is_cuda, "out must be a CUDA tensor")
+    _same_device(out.device, cache=cache, block_table=block_table, cu_seq_lens=cu_seq_lens, seq_starts=seq_starts)
+    _check(out.dtype in (torch.float16, torch.bfloat16), "out must be fp16 or bf16")
+    _check(cache.dim() >= 2 and cache.is_contiguous(), "cache must be contiguous [.., page, row]")
+    if cache.dtype == torch.uint8:
+        _check(cache.size(-1) in (DSMLA_ROW_BYTES, IDXK_FP8_ROW_BYTES), "uint8 cache rows must be 656 or 132 bytes")
+        fmt, width = ((L.DSA_FP8_DS_MLA, 576) if cache.size(-1) == DSMLA_ROW_BYTES else (L.DSA_FP8_IDXK, 128))
+    else:
+        _check(cache.dtype in (torch.float16, torch.bfloat16), "cache must be fp16, bf16 or uint8 (fp8)")
+        fmt, width = _DTYPE[cache.dtype], cache.size(-1)
+    _check(out.dim() == 2 and out.size(1) == width and out.stride(1) == 1, f"out must be [N, {width}], unit inner stride")
+    _check(cu_seq_lens.dim() == 1 and cu_seq_lens.numel() >= 1, "cu_seq_lens must be [B + 1]")
+    B = cu_seq_lens.numel() - 1
+    _paged(block_table, cu_seq_lens, "cu_seq_lens", B)
+    if seq_starts is not None:
+        _int32(seq_starts, "seq_starts")
+        _check(seq_starts.dim() == 1 and seq_starts.numel() >= B, "seq_starts must be [B]")
+        seq_starts = seq_starts.contiguous()
+    _check(cache.size(-2) > 0, "cache has no rows in a page")
+    n = out.size(0)
+    if n == 0:
+        return
+    with torch.cuda.device(out.device):
+        L.call("dsa_gather_cache", _vp(out), _DTYPE[out.dtype], max(out.stride(0), width) if n == 1 else out.stride(0),
+               n, _vp(cache), fmt, cache.numel() // cache.size(-1), cache.size(-2), width, _vp(block_table),
+               max(block_table.stride(0), block_table.size(1)), block_table.size(1), _vp(cu_seq_lens.contiguous()),
+               _vp(seq_starts), B, _stream(out.device))
+
+
+def _rotary_embedding_impl(out, x, positions, cos_sin_cache, is_neox, rope_offset):
+    _check(x.is_cuda, "x must be a CUDA tensor")
+    _same_device(x.device, out=out, positions=positions, cos_sin_cache=cos_sin_cache)
+    _check(x.dtype in _DTYPE and out.dtype == x.dtype, "x and out must be fp16, bf16 or fp32, the same dtype")
+    _check(x.dim() == 3 and tuple(out.shape) == tuple(x.shape), "x and out must be [T, n_head, width]")
+    T, H, W = x.shape
+    _check(W <= 1 or (x.stride(2) == 1 and out.stride(2) == 1), "x and out must have unit inner stride")
+    _check(positions.dtype == torch.int64 and positions.dim() == 1 and positions.numel() == T and
+           positions.is_contiguous(), "positions must be contiguous int64 [T]")
+    _check(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.dim() == 2 and cos_sin_cache.is_contiguous() and
+           cos_sin_cache.size(0) > 0, "cos_sin_cache must be contiguous f32 [max_pos, rotary_dim]")
+    if x.numel() == 0:
+        return
+    with torch.cuda.device(x.device):
+        L.call("dsa_rotary_embedding", _vp(out), out.stride(0), out.stride(1), _vp(x), x.stride(0), x.stride(1),
+               _DTYPE[x.dtype], _vp(positions), _vp(cos_sin_cache), cos_sin_cache.size(0), cos_sin_cache.size(1),
+               int(rope_offset), int(bool(is_neox)), T, H, W, _stream(x.device))
+
+
 # ------------------------------------------------------ torch registration
 _lib_def = torch.library.Library(NAMESPACE, "DEF")
 _SCHEMAS = {
@@ -520,6 +654,15 @@ _SCHEMAS = {
                          "Tensor slot_mapping, Tensor? ln_weight, Tensor? ln_bias, float ln_eps, Tensor? positions, "
                          "Tensor? cos_sin_cache, bool is_neox, float weight_scale) -> ()",
                          _indexer_qk_store_impl, "CUDA"),
+    # verification of a tree of drafts, cache read-back (no reference op)
+    "tree_mla_decode": ("(Tensor! o, Tensor! lse, Tensor q, Tensor kv_cache, Tensor block_table, Tensor seq_lens, "
+                        "Tensor tree_mask, Tensor? draft_lens, float scale) -> ()", _tree_mla_decode_impl, "CUDA"),
+    "commit_draft_rows": ("(Tensor(a!)[] caches, Tensor block_table, Tensor seq_lens, Tensor accepted, "
+                          "Tensor draft_lens) -> ()", _commit_draft_rows_impl, "CUDA"),
+    "gather_cache": ("(Tensor! out, Tensor cache, Tensor block_table, Tensor cu_seq_lens, Tensor? seq_starts) -> ()",
+                     _gather_cache_impl, "CUDA"),
+    "rotary_embedding": ("(Tensor! out, Tensor x, Tensor positions, Tensor cos_sin_cache, bool is_neox, "
+                         "int rope_offset) -> ()", _rotary_embedding_impl, "CUDA"),
 }
 for _name, (_schema, _fn, _key) in _SCHEMAS.items():
     _lib_def.define(_name + _schema)
@@ -532,7 +675,8 @@ def _noop_fake(*args, **kwargs):
 
 for _name in ("sm70_sparse_mla_decode", "sm70_indexer_logits", "sm70_indexer_logits_packed", "sm70_decode_topk",
               "persistent_topk", "sm70_indexer_k_store", "sm70_indexer_shard_merge",
-              "sm70_indexer_shard_merge_p2p", "concat_and_cache_ds_mla", "indexer_qk_store"):
+              "sm70_indexer_shard_merge_p2p", "concat_and_cache_ds_mla", "indexer_qk_store", "tree_mla_decode",
+              "commit_draft_rows", "gather_cache", "rotary_embedding"):
     torch.library.register_fake(f"{NAMESPACE}::{_name}")(_noop_fake)
 
 
@@ -615,3 +759,38 @@ def indexer_qk_store(q_out, weights_out, kv_cache, q, kw, slot_mapping, ln_weigh
     weights_out = kw[:, 128:] * weight_scale."""
     _op("indexer_qk_store")(q_out, weights_out, kv_cache, q, kw, slot_mapping, ln_weight, ln_bias, float(ln_eps),
                             positions, cos_sin_cache, is_neox, float(weight_scale))
+
+
+def tree_mla_decode(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, scale: float, draft_lens=None) -> None:
+    """Attention of a tree of drafts over the whole latent cache: q [B, T, H,
+    576] -> o [B, T, H, 512], lse [B, T, H] f32. seq_lens counts the drafts
+    (the last draft_lens[b], default T, positions of a request); bit j of
+    tree_mask[b, i] (int64, T <= 64) lets draft i see draft j, the positions
+    before the drafts are seen by all. Rows that see nothing and rows past
+    draft_lens[b] become o = 0, lse = -inf."""
+    _op("tree_mla_decode")(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, draft_lens, float(scale))
+
+
+def commit_draft_rows(caches, block_table, seq_lens, accepted, draft_lens) -> None:
+    """After verification: in every cache of the list (latent or indexer-K, one
+    geometry and block table; one launch for up to 128 layers) the k-th
+    accepted draft's row moves from position pre + accepted[b, k] to pre + k,
+    pre = seq_lens[b] - draft_lens[b]. accepted int32 [B, n <= 64], -1 padded."""
+    _op("commit_draft_rows")(caches, block_table, seq_lens, accepted, draft_lens)
+
+
+def gather_cache(out, cache, block_table, cu_seq_lens, seq_starts=None) -> None:
+    """Cache rows read back and dequantised, request after request: out [N,
+    width] fp16/bf16 <- positions seq_starts[b] + (0 .. cu_seq_lens[b+1] -
+    cu_seq_lens[b]) of request b. Reads latent caches (656-byte rows -> 576
+    values), indexer-K caches (132 -> 128) and 16-bit caches. Rows of out past
+    cu_seq_lens[B] are left as they were."""
+    _op("gather_cache")(out, cache, block_table, cu_seq_lens, seq_starts)
+
+
+def rotary_embedding(out, x, positions, cos_sin_cache, is_neox: bool = False, rope_offset: int = 0) -> None:
+    """out = x [T, n_head, width] with elements [rope_offset, rope_offset +
+    cos_sin_cache.size(1)) of every head rotated; the rest is copied. out may
+    be x (in place) or a slice of another tensor, such as the rotary columns
+    of the attention's query rows. The table: rope.rope_cos_sin_cache."""
+    _op("rotary_embedding")(out, x, positions, cos_sin_cache, bool(is_neox), int(rope_offset))

@@ -395,6 +395,92 @@ int dsa_shard_exchange_merge(int32_t* out, int64_t out_stride,
                              int64_t timeout_ns, int32_t* err_flag,
                              void* stream);
 
+/* =====================================================================
+ * Verification of a tree of drafts. No reference counterpart: the reference
+ * verifies a line of drafts as extra decode rows (tmla.py:261-279).
+ *
+ * dsa_tree_mla_decode: attention of every draft of a request over the whole
+ * paged latent cache. Request b has seq_lens[b] positions; the last
+ * n = min(max(draft_lens[b], 0), T) of them (T when draft_lens is NULL) are
+ * its drafts, pre = seq_lens[b] - n positions precede them. Row (i, h) sees
+ * position p when p < pre, or when bit p - pre of tree_mask[b, i] is set:
+ *   o[b,i,h,:512] = sum_p softmax_p(scale * q[b,i,h,:] . kv_p[:576]) kv_p[:512]
+ *   lse[b,i,h]    = log-sum-exp of the scaled scores
+ * A row that sees nothing, and rows i >= n: o = 0, lse = -inf. Positions at or
+ * past seq_lens[b], and draft positions that no row of the request sees, are
+ * never read. A position that is seen resolves as in dsa_sparse_mla_decode; a
+ * cache row outside [0, n_kv_rows), or past the block table, reads as zeros.
+ * A position that some rows see must hold finite values: its NaN or infinity
+ * reaches the other rows of the request too.
+ *
+ * q      [B, T, n_head, 576] f16 or bf16, contiguous (bf16 with a bf16 cache)
+ * kv     f16/bf16 [.., page, 576] or u8 [.., page, 656] (DSA_FP8_DS_MLA)
+ * tree_mask int64 [B, T], row stride mask_stride; T <= 64
+ * o      [B, T, n_head, 512] f16 or bf16, contiguous; lse f32 [B, T, n_head]
+ * workspace: at least dsa_tree_mla_decode_workspace_bytes(B, T, n_head) bytes
+ *   of device memory, 16-byte aligned (may be NULL when that is 0); calls that
+ *   overlap on the GPU need their own.
+ * ===================================================================== */
+size_t dsa_tree_mla_decode_workspace_bytes(int B, int T, int n_head);
+
+int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void* q,
+                        int q_dtype, const void* kv_cache, int kv_format,
+                        int64_t n_kv_rows, int page_size,
+                        const int32_t* block_table, int64_t bt_stride,
+                        int max_blocks, const int32_t* seq_lens,
+                        const int32_t* draft_lens, const int64_t* tree_mask,
+                        int64_t mask_stride, int B, int T, int n_head,
+                        double scale, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* dsa_commit_draft_rows: the k-th accepted draft's row moves from position
+ * pre + accepted[b, k] to pre + k (pre as above), as raw bytes, in each of
+ * n_caches caches that share one geometry and block table (one per layer;
+ * caches is a HOST array of device pointers). All rows of a request are read
+ * before any is written. Entries below 0 or not below the request's draft
+ * count, and rows outside the block table or the cache, are skipped.
+ * row_bytes: a multiple of 16 up to 1152, or of 4 up to 132. n_drafts and
+ * n_accept <= 64. */
+int dsa_commit_draft_rows(void* const* caches, int n_caches, int64_t n_rows,
+                          int page_size, int row_bytes,
+                          const int32_t* block_table, int64_t bt_stride,
+                          int max_blocks, const int32_t* seq_lens,
+                          const int32_t* draft_lens, int n_drafts,
+                          const int32_t* accepted, int64_t acc_stride,
+                          int n_accept, int B, void* stream);
+
+/* dsa_gather_cache: cache rows read back as 16-bit values, request after
+ * request. Output row i with cu_seq_lens[b] <= i < cu_seq_lens[b+1] is
+ * position seq_starts[b] + i - cu_seq_lens[b] of request b (seq_starts may be
+ * NULL: 0), resolved through the block table; rows outside the table or the
+ * cache are zeros, output rows of no request are left as they were.
+ * cache_format DSA_FP8_DS_MLA (576 values: codes times their tile's scale, the
+ * f16 rotary tail), DSA_FP8_IDXK (128 values), or DSA_F16 / DSA_BF16 rows of
+ * `width` values (a multiple of 8). One rounding, to out's type.
+ * out [n_out, width] f16/bf16, row stride out_stride (elements, multiple of 8);
+ * cu_seq_lens int32 [B + 1] ascending. */
+int dsa_gather_cache(void* out, int out_dtype, int64_t out_stride, int n_out,
+                     const void* cache, int cache_format, int64_t n_rows,
+                     int page_size, int width, const int32_t* block_table,
+                     int64_t bt_stride, int max_blocks,
+                     const int32_t* cu_seq_lens, const int32_t* seq_starts,
+                     int B, void* stream);
+
+/* dsa_rotary_embedding: elements [rope_offset, rope_offset + rotary_dim) of
+ * every head of x rotated by row positions[t] (clamped into the table) of
+ * cos_sin [max_pos, rotary_dim] f32 = cos | sin; pairs (2i, 2i+1), or
+ * (i, i + rotary_dim/2) with rope_neox; the rest of the head is copied. x and
+ * out [n_tok, n_head, width] in dtype (f16, bf16 or f32), unit inner stride,
+ * token and head strides in elements. out may be x itself (same strides) or
+ * must not overlap it. Same arithmetic as the cache writers. width <= 2048. */
+int dsa_rotary_embedding(void* out, int64_t out_tok_stride,
+                         int64_t out_head_stride, const void* x,
+                         int64_t x_tok_stride, int64_t x_head_stride,
+                         int dtype, const int64_t* positions,
+                         const float* cos_sin, int64_t max_pos, int rotary_dim,
+                         int rope_offset, int rope_neox, int n_tok, int n_head,
+                         int width, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,176 @@
+"""CPU: host logic and refusals of the tree-verification operators."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+
+def _up(parents, i):
+    seen = [i]
+    while parents[seen[-1]] >= 0:
+        seen.append(parents[seen[-1]])
+    return seen
+
+
+@pytest.mark.parametrize("T", [1, 2, 7, 31, 64])
+def test_draft_tree_masks_follow_the_parents(dsa, T):
+    rng = np.random.default_rng(T)
+    parents = np.stack([np.array([rng.integers(-1, i) if i else -1 for i in range(T)]),
+                        np.arange(T) - 1,            # a line: depth grows by one, log2 T doublings are needed
+                        np.full(T, -1)])             # all roots
+    mask, depth = dsa.mla_sparse.draft_tree_masks(torch.tensor(parents, dtype=torch.int32))
+    for b in range(3):
+        for i in range(T):
+            path = _up(parents[b], i)
+            want = sum(1 << int(j) for j in path)
+            assert int(mask[b, i]) & (2 ** 64 - 1) == want, (b, i)
+            assert int(depth[b, i]) == len(path) - 1
+
+
+def test_draft_tree_masks_take_bad_parents_as_roots(dsa):
+    mask, depth = dsa.mla_sparse.draft_tree_masks(torch.tensor([[3, 5, 2, -9]]))
+    assert mask.tolist() == [[1, 2, 4, 8]] and depth.tolist() == [[0, 0, 0, 0]]
+    mask, depth = dsa.mla_sparse.draft_tree_masks(torch.empty(2, 0, dtype=torch.int32))
+    assert mask.shape == (2, 0) and depth.shape == (2, 0)
+    with pytest.raises(RuntimeError, match="64 drafts"):
+        dsa.mla_sparse.draft_tree_masks(torch.zeros(1, 65, dtype=torch.int32))
+
+
+def test_rope_table_without_scaling_and_far_positions(dsa):
+    t = dsa.rope.rope_cos_sin_cache(64, 180_001, base=1e6)
+    p, i = 180_000, np.arange(32)
+    a = np.float64(p) * 1e6 ** (-2.0 * i / 64)
+    # one rounding to f32 of a value of at most 1, and f64's error of an angle below 2e5 (2^-53 * 2e5)
+    assert np.abs(t[p, :32].double().numpy() - np.cos(a)).max() <= 2.0 ** -24 + 1e-10
+    assert np.abs(t[p, 32:].double().numpy() - np.sin(a)).max() <= 2.0 ** -24 + 1e-10
+
+
+def test_rope_table_scalings(dsa):
+    r = dsa.rope
+    plain, g = r.rope_inv_freq(64)
+    assert g == 1.0
+    lin, _ = r.rope_inv_freq(64, scaling={"type": "linear", "factor": 4.0})
+    assert torch.equal(lin, plain / 4.0)
+    ntk, _ = r.rope_inv_freq(64, scaling={"type": "ntk", "factor": 8.0})
+    assert ntk[0] == 1.0 and abs(float(ntk[31] / plain[31]) - 1 / 8.0) < 1e-12  # last pair: wavelength times the factor
+    y, g = r.rope_inv_freq(64, scaling={"type": "yarn", "factor": 40.0, "original_max_position": 4096})
+    assert abs(g - (0.1 * math.log(40.0) + 1.0)) < 1e-12
+    turns = 4096 * plain / (2 * math.pi)
+    # floor / ceil widen the ramp to whole pairs: one pair past the thresholds all is kept / divided
+    assert torch.equal(y[turns > 32 * 10000 ** (2 / 64)], plain[turns > 32 * 10000 ** (2 / 64)])
+    assert torch.allclose(y[turns < 1], plain[turns < 1] / 40.0, rtol=1e-14, atol=0)
+    mid = (y < plain) & (y > plain / 40.0)
+    assert 5 < int(mid.sum()) < 20 and bool((y[1:] < y[:-1]).all())
+    same, g = r.rope_inv_freq(64, scaling={"type": "yarn", "factor": 40.0, "original_max_position": 4096,
+                                           "mscale": 1.0, "mscale_all_dim": 1.0})
+    assert g == 1.0 and torch.equal(same, y)
+    for bad in ({"type": "no"}, {"type": "linear", "factor": 0.0}):
+        with pytest.raises(RuntimeError):
+            r.rope_inv_freq(64, scaling=bad)
+    with pytest.raises(RuntimeError):
+        r.rope_inv_freq(63)
+    with pytest.raises(RuntimeError):
+        r.rope_cos_sin_cache(64, 0)
+
+
+def _ops(dsa):
+    return dsa.ops
+
+
+def test_wrappers_refuse_cpu_tensors(dsa):
+    ops = _ops(dsa)
+    i32 = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops._tree_mla_decode_impl(torch.empty(1, 1, 1, 512), torch.empty(1, 1, 1), torch.empty(1, 1, 1, 576),
+                                  torch.empty(1, 64, 576), i32[None], i32, torch.zeros(1, 1, dtype=torch.int64), None, 1.0)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops._commit_draft_rows_impl([torch.empty(1, 64, 576)], i32[None], i32, i32[None], i32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops._gather_cache_impl(torch.empty(1, 576), torch.empty(1, 64, 576), i32[None], i32, None)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops._rotary_embedding_impl(torch.empty(1, 1, 64), torch.empty(1, 1, 64), torch.zeros(1, dtype=torch.int64),
+                                   torch.empty(1, 64), False, 0)
+    ops._commit_draft_rows_impl([], i32[None], i32, i32[None], i32)  # nothing to do
+
+
+def _tree(lib, **k):
+    P = ctypes.c_void_p
+    a = dict(o=P(1024), o_dtype=1, lse=P(1024), q=P(1024), q_dtype=1, kv=P(1024), fmt=3, n_rows=640, page=64, bt=P(1024),
+             bts=4, mb=4, seq=P(1024), dl=None, mask=P(1024), ms=8, B=1, T=8, H=8, scale=1.0, ws=None, wsb=0, stream=None)
+    a.update(k)
+    return lib.dsa_tree_mla_decode(*a.values())
+
+
+def test_tree_entry_refuses_bad_arguments(dsa):
+    L, lib = dsa._lib, dsa._lib.lib()
+    P = ctypes.c_void_p
+    for bad, code in [(dict(B=-1), L.DSA_ERR_INVALID), (dict(T=65, ms=65), L.DSA_ERR_UNSUPPORTED),
+                      (dict(q_dtype=2), L.DSA_ERR_INVALID), (dict(o_dtype=2), L.DSA_ERR_INVALID),
+                      (dict(fmt=4), L.DSA_ERR_INVALID), (dict(fmt=1, q_dtype=0), L.DSA_ERR_UNSUPPORTED),
+                      (dict(page=0), L.DSA_ERR_INVALID), (dict(n_rows=2 ** 31), L.DSA_ERR_INVALID),
+                      (dict(bts=3), L.DSA_ERR_INVALID), (dict(ms=7), L.DSA_ERR_INVALID), (dict(q=None), L.DSA_ERR_INVALID),
+                      (dict(mask=None), L.DSA_ERR_INVALID), (dict(bt=None), L.DSA_ERR_INVALID),
+                      (dict(kv=P(1032)), L.DSA_ERR_INVALID), (dict(o=P(1032)), L.DSA_ERR_INVALID),
+                      (dict(H=2000), L.DSA_ERR_UNSUPPORTED)]:
+        assert _tree(lib, **bad) == code, bad
+    assert _tree(lib, B=0) == L.DSA_OK and _tree(lib, T=0) == L.DSA_OK and _tree(lib, H=0) == L.DSA_OK
+
+
+def test_rotary_entry_refuses_bad_arguments(dsa):
+    L, lib = dsa._lib, dsa._lib.lib()
+    P = ctypes.c_void_p
+
+    def call(**k):
+        a = dict(out=P(1024), ot=64, oh=64, x=P(1024), xt=64, xh=64, dt=1, pos=P(1024), cs=P(1024), mp=10, r=64, off=0,
+                 neox=0, n=4, h=1, w=64, s=None)
+        a.update(k)
+        return lib.dsa_rotary_embedding(*a.values())
+
+    for bad, code in [(dict(dt=3), L.DSA_ERR_INVALID), (dict(r=63), L.DSA_ERR_INVALID), (dict(r=0), L.DSA_ERR_INVALID),
+                      (dict(off=1), L.DSA_ERR_INVALID), (dict(off=-2), L.DSA_ERR_INVALID), (dict(n=-1), L.DSA_ERR_INVALID),
+                      (dict(mp=0), L.DSA_ERR_INVALID), (dict(x=None), L.DSA_ERR_INVALID), (dict(w=0), L.DSA_ERR_INVALID),
+                      (dict(w=4096), L.DSA_ERR_UNSUPPORTED), (dict(h=70000), L.DSA_ERR_UNSUPPORTED)]:
+        assert call(**bad) == code, bad
+    assert call(n=0) == L.DSA_OK and call(h=0) == L.DSA_OK
+
+
+def test_gather_and_commit_entries_refuse_bad_arguments(dsa):
+    L, lib = dsa._lib, dsa._lib.lib()
+    P = ctypes.c_void_p
+
+    def gather(**k):
+        a = dict(out=P(1024), od=1, os=576, n=4, c=P(1024), fmt=3, rows=640, page=64, w=576, bt=P(1024), bts=4, mb=4,
+                 cu=P(1024), st=None, B=1, s=None)
+        a.update(k)
+        return lib.dsa_gather_cache(*a.values())
+
+    for bad in [dict(od=2), dict(fmt=2), dict(w=128), dict(fmt=4), dict(fmt=0, w=20, os=24), dict(n=-1), dict(page=0),
+                dict(bts=3), dict(os=512), dict(os=580), dict(out=P(1028)), dict(c=P(1028)), dict(cu=None),
+                dict(bt=None), dict(c=None)]:
+        assert gather(**bad) == L.DSA_ERR_INVALID, bad
+    assert gather(n=0) == L.DSA_OK and gather(B=0) == L.DSA_OK
+
+    def commit(ptrs=(1024,), **k):
+        arr = (ctypes.c_void_p * max(1, len(ptrs)))(*ptrs)
+        a = dict(c=arr, nc=len(ptrs), rows=640, page=64, rb=656, bt=P(1024), bts=4, mb=4, seq=P(1024), dl=P(1024), nd=64,
+                 acc=P(1024), acs=8, na=8, B=1, s=None)
+        a.update(k)
+        return lib.dsa_commit_draft_rows(*a.values())
+
+    for bad, code in [(dict(nd=65), L.DSA_ERR_UNSUPPORTED), (dict(na=65, acs=65), L.DSA_ERR_UNSUPPORTED),
+                      (dict(rb=654), L.DSA_ERR_UNSUPPORTED), (dict(rb=1168), L.DSA_ERR_UNSUPPORTED),
+                      (dict(rb=260), L.DSA_ERR_UNSUPPORTED), (dict(acs=7), L.DSA_ERR_INVALID), (dict(B=-1), L.DSA_ERR_INVALID),
+                      (dict(acc=None), L.DSA_ERR_INVALID), (dict(ptrs=(1028,)), L.DSA_ERR_INVALID),
+                      (dict(ptrs=(1024, 0)), L.DSA_ERR_INVALID)]:
+        assert commit(**bad) == code, bad
+    assert commit(ptrs=()) == L.DSA_OK and commit(B=0) == L.DSA_OK and commit(na=0) == L.DSA_OK
+
+
+def test_new_ops_registered(dsa):
+    ns = torch.ops.dsa_b200
+    assert [a.name for a in ns.tree_mla_decode.default._schema.arguments] == [
+        "o", "lse", "q", "kv_cache", "block_table", "seq_lens", "tree_mask", "draft_lens", "scale"]
+    for name in ("tree_mla_decode", "commit_draft_rows", "gather_cache", "rotary_embedding"):
+        assert hasattr(ns, name) and callable(getattr(dsa, name))
