@@ -1,4 +1,5 @@
-// Attention of a tree of drafted tokens over the paged latent cache.
+// Attention of a tree of drafted tokens over the paged latent cache, on the
+// 5th-generation tensor cores (tcgen05 + TMEM, CTA pairs).
 //
 // Request b has s = seq_lens[b] positions, the last n = draft_lens[b] of them
 // its drafts. Row (i, h), the query of draft i and head h, sees position p when
@@ -6,14 +7,84 @@
 //   z_p = scale * q[b,i,h,:576] . kv_p,  lse = log sum_p exp(z_p),
 //   o = sum_p exp(z_p - lse) kv_p[:512];  nothing visible: o = 0, lse = -inf.
 //
-// One block: 16 rows of one request, keys in tiles of 16 held as f32 in shared
-// memory, the softmax's running maximum and sum in f32.
-#include "common.cuh"
+// All T * H rows of a request read the same keys, so rows are the M side: one
+// cluster of two CTAs takes 128 consecutive rows (64 per CTA) and a run of
+// 128-key tiles, one pass with a running maximum and sum. Per tile
+//   S[128 x 128]  = Q[128 x 576] . K^T     each CTA holds 64 of the keys
+//   O[128 x 512] += P[128 x 128] . V       each CTA holds 256 of the columns
+// as cta_group::2 MMAs (M = 128, N = 128 and 2 x 256). Why pairs: an f32 state
+// of 512 columns lets an SM hold 64 rows (half of TMEM, the other half S), and
+// alone such an SM would read every key operand from its own shared memory for
+// 64 rows only; in a pair each SM stores half of each operand and the hardware
+// shares it, which takes 24 KB of shared-memory traffic per key and SM pair
+// instead of 35.
+//
+// Work split: the (request, row tile, key tile) triples of a call form one
+// list; pair p of P takes an equal run of it, whatever the lengths of the
+// requests are. A run that holds all key tiles of a row tile writes o and lse;
+// the first and last segments of a run may hold only some, and leave their
+// unnormalised state in one of the pair's two workspace slots for the merge
+// kernel, which finds them by the same arithmetic (no counters, nothing to
+// reset, the same bits in every run).
+//
+// Roles (28 warps): warps 0-15 load the cache rows (any page size) two buffers
+// ahead in registers, expand e4m3 to f16 and store K (keys x 576, K-major) and V
+// (this CTA's 256 columns, MN-major); warps 16-23 are the softmax, a thread a
+// row and 32 keys (rows are TMEM lanes: no shuffles); one thread of CTA 0 issues
+// QK(t+1) before PV(t), so K(t+1) is stored under PV(t-1), V(t) under QK(t+1),
+// and the softmax of t runs under PV(t-1). The roles meet at mbarriers only, and
+// run on through the segments: the epilogue of one overlaps the loads of the
+// next. Every wait is bounded by device time.
+//
+// Arithmetic: f16 operands (bf16 for a bf16 cache), f32 sums, maximum and state.
+// A dequantised value code * scale is rounded once to f16, half a step 2^-11:
+// over contexts of at most 512 positions, where few keys average that error out
+// of lse, its remainder is multiplied too, by a second QK pass into the same S.
+// bf16 q is shifted by a power of two per row into f16's range, which the row's
+// scale undoes exactly. The running maximum moves only when a score exceeds it
+// by 2^8, so P <= 256 and O is rarely rescaled.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+#include <type_traits>
+
+#include "sparse_mla.cuh"
+#include "tc_common.cuh"
 
 namespace dsa {
 namespace {
 
-constexpr int TR = 16, TK = 16, DK = 576, DV = 512, NT = 256;
+using namespace tc;
+
+constexpr int kPairRows = 128;  // rows of a cluster
+constexpr int kRows = 64;       // rows of a CTA
+constexpr int kKeys = 128;      // keys of a tile
+constexpr int DK = 576, DV = 512;
+constexpr int kProducers = 16;
+constexpr int kSoftmax0 = 16, kSoftmaxWarps = 8;
+constexpr int kMmaWarp = 24;
+constexpr int kThreads = 28 * 32;
+constexpr uint32_t kBlk = 64 * 128;    // 64 rows x 64 16-bit values: 8 KB
+constexpr uint32_t kVBlk = 128 * 128;  // 128 keys x 64 columns: 16 KB
+constexpr uint32_t SM_Q = 0;
+constexpr uint32_t SM_K = SM_Q + 9 * kBlk;
+constexpr uint32_t SM_V = SM_K + 9 * kBlk;
+constexpr uint32_t SM_P = SM_V + 4 * kVBlk;
+constexpr uint32_t SM_MISC = SM_P + 2 * kBlk;
+constexpr uint32_t kMiscBytes = 2048;
+constexpr uint32_t SMEM_BYTES = SM_MISC + kMiscBytes + 1024;  // + alignment slack
+constexpr uint32_t S_COL = 256;        // S buffer x at [256 + 64x, +64); O half h at [128h, +128)
+constexpr uint32_t TMEM_COLS = 512;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kNoMax = -1e30f;
+constexpr int kNoRow = (int)0x80000000;
+constexpr int kMaxSeq = 0x7fffff00;   // tile ends stay in 32 bits
+constexpr float kRescale = 8.0f;       // log2 units
+constexpr int kTwoPassKeys = 512;      // fp8: the remainder of the rounding is multiplied up to here
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kSlotF = DV + 2;         // f32 of a row's partial state: o, then m and l
+
+static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 
 struct TreeArgs {
   const void* q;
@@ -24,108 +95,821 @@ struct TreeArgs {
   const int64_t* mask;
   void* o;
   float* lse;
+  float* part_o;   // [2 * pairs][slot_rows][512]
+  float* part_ml;  // [2 * pairs][slot_rows][2]
   int64_t n_kv_rows, bt_stride, mask_stride;
-  int fmt, page, max_blocks, T, H, q_bf16, o_bf16;
+  int page, max_blocks, B, T, H, pairs, slot_rows;
+  int q_bf16, o_bf16;
   float scale_log2;
 };
 
-__device__ float kv_value(const TreeArgs& p, int64_t row, int d) {
-  if (row < 0) return 0.f;
-  if (p.fmt == DSA_FP8_DS_MLA) {
-    const uint8_t* r = p.kv + row * 656;
-    if (d >= 512) return __half2float(reinterpret_cast<const __half*>(r + 528)[d - 512]);
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(r[d], __NV_E4M3);
-    return __half2float(*reinterpret_cast<const __half*>(&h)) * reinterpret_cast<const float*>(r + 512)[d >> 7];
-  }
-  if (p.fmt == DSA_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.kv)[row * DK + d]);
-  return __half2float(reinterpret_cast<const __half*>(p.kv)[row * DK + d]);
+// Request b's size: key tiles and row tiles (0 tiles: nothing to do).
+struct Req {
+  int seq, nd, nt, nrt;
+};
+__device__ __forceinline__ Req load_req(const TreeArgs& p, int b) {
+  Req r;
+  r.seq = min(max(p.seq_lens[b], 0), kMaxSeq);
+  r.nd = p.draft_lens ? min(max(p.draft_lens[b], 0), p.T) : p.T;
+  r.nrt = (r.nd * p.H + kPairRows - 1) / kPairRows;
+  r.nt = r.nd > 0 ? (int)(((int64_t)r.seq + kKeys - 1) / kKeys) : 0;
+  return r;
 }
 
-__global__ void __launch_bounds__(NT) tree_simple_kernel(const TreeArgs p) {
-  extern __shared__ float sm[];
-  float* q = sm;                 // [TR][DK]
-  float* kv = q + TR * DK;       // [TK][DK]
-  float* s = kv + TK * DK;       // [TR][TK]
-  float* m = s + TR * TK;        // [TR]
-  float* l = m + TR;
-  float* al = l + TR;
-  const int b = blockIdx.y, r0 = blockIdx.x * TR, R = p.T * p.H;
-  const int nd = p.draft_lens ? min(max(p.draft_lens[b], 0), p.T) : p.T;
-  const int seq = p.seq_lens[b], pre = seq - nd;
-  for (int i = threadIdx.x; i < TR * DK; i += NT) {
-    const int r = r0 + i / DK;
-    float v = 0.f;
-    if (r < R) {
-      const int64_t at = ((int64_t)b * R + r) * DK + i % DK;
-      v = p.q_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.q)[at])
-                   : __half2float(reinterpret_cast<const __half*>(p.q)[at]);
-    }
-    q[i] = v;
+// Sum of nt * nrt over requests [0, n), by one warp; every lane gets it.
+__device__ __forceinline__ long long warp_work(const TreeArgs& p, int n, int lane) {
+  long long w = 0;
+  for (int b = lane; b < n; b += 32) {
+    const Req r = load_req(p, b);
+    w += (long long)r.nt * r.nrt;
   }
-  if (threadIdx.x < TR) {
-    m[threadIdx.x] = -INFINITY;
-    l[threadIdx.x] = 0.f;
-  }
-  uint64_t seen = 0;  // draft columns that some row of the request sees: the others are not read
-  for (int t = 0; t < nd; ++t) seen |= (uint64_t)p.mask[(int64_t)b * p.mask_stride + t];
-  float acc[TR][2] = {};
-  const int row = threadIdx.x / TK, key = threadIdx.x % TK;
-  const int gr = r0 + row, i = gr / p.H;
-  const uint64_t bits = (gr < R && i < nd) ? (uint64_t)p.mask[(int64_t)b * p.mask_stride + i] : 0;
-  for (int k0 = 0; k0 < seq; k0 += TK) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < TK * DK; e += NT) {
-      const int pos = k0 + e / DK;
-      int64_t phys = -1;
-      if (pos < seq && pos / p.page < p.max_blocks && (pos < pre || ((seen >> (pos - pre)) & 1))) {
-        phys = (int64_t)p.bt[(int64_t)b * p.bt_stride + pos / p.page] * p.page + pos % p.page;
-        if (phys < 0 || phys >= p.n_kv_rows) phys = -1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+  return w;
+}
+
+__device__ __forceinline__ long long chunk_of(long long work, int pairs) { return (work + pairs - 1) / pairs; }
+
+// One pair's walk over its run of tiles.
+struct Cursor {
+  int left;        // tiles left, this one included
+  int b, rt, tile, seg;
+  bool first;      // first tile of a segment
+  Req r;
+  __device__ __forceinline__ bool last() const { return tile + 1 == r.nt || left == 1; }
+  __device__ __forceinline__ void next(const TreeArgs& p) {
+    first = false;
+    ++tile;
+    if (--left == 0) return;
+    if (tile == r.nt) {
+      tile = 0;
+      first = true;
+      ++seg;
+      if (++rt == r.nrt) {
+        rt = 0;
+        do r = load_req(p, ++b);
+        while (r.nt == 0 || r.nrt == 0);
       }
-      kv[e] = kv_value(p, phys, e % DK);
     }
-    __syncthreads();
-    float z = 0.f;
-    for (int d = 0; d < DK; ++d) z += q[row * DK + d] * kv[key * DK + d];
-    const int pos = k0 + key;
-    const bool sees = gr < R && i < nd && pos < seq && (pos < pre || ((bits >> (pos - pre)) & 1));
-    s[row * TK + key] = sees ? z * p.scale_log2 : -INFINITY;
-    __syncthreads();
-    if (threadIdx.x < TR) {
-      float mx = m[threadIdx.x];
-      for (int k = 0; k < TK; ++k) mx = fmaxf(mx, s[threadIdx.x * TK + k]);
-      const float a = m[threadIdx.x] == -INFINITY ? 0.f : exp2f(m[threadIdx.x] - mx);
-      float sum = l[threadIdx.x] * a;
-      for (int k = 0; k < TK; ++k) {
-        const float v = s[threadIdx.x * TK + k];
-        const float e = v == -INFINITY ? 0.f : exp2f(v - mx);
-        s[threadIdx.x * TK + k] = e;
-        sum += e;
-      }
-      m[threadIdx.x] = mx;
-      l[threadIdx.x] = sum;
-      al[threadIdx.x] = a;
-    }
-    __syncthreads();
-    for (int r = 0; r < TR; ++r)
-      for (int c = 0; c < 2; ++c) {
-        float v = acc[r][c] * al[r];
-        for (int k = 0; k < TK; ++k) v += s[r * TK + k] * kv[k * DK + threadIdx.x + 256 * c];
-        acc[r][c] = v;
-      }
   }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// How a group of codes is expanded to f16: the product code * scale rounded
+// once, by f16 arithmetic where scale * 256 keeps every product normal
+// (kFast), by f32 elsewhere (kWide), or what that rounding left (kRest).
+enum { kFast, kWide, kRest };
+__device__ __forceinline__ bool fast_scale(float sc) { return sc >= 0x1p-15f && sc <= 128.0f; }
+
+template <int HOW>
+__device__ __forceinline__ void dequant16(const uint4& r, float sc, uint32_t (&q)[8]) {
+  e4m3x4_to_half2x2_div256(r.x, q[0], q[1]);
+  e4m3x4_to_half2x2_div256(r.y, q[2], q[3]);
+  e4m3x4_to_half2x2_div256(r.z, q[4], q[5]);
+  e4m3x4_to_half2x2_div256(r.w, q[6], q[7]);
+  const float s256 = sc * 256.0f;
+  if constexpr (HOW == kFast) {
+    // scale = hi + lo with hi cut to 7 significant bits: a code (4 bits) times
+    // hi is exact in f16's 11 bits, so the fma rounds the whole product once
+    const float hi7 = __uint_as_float(__float_as_uint(s256) & 0xFFFE0000u);
+    const __half2 s_hi = __float2half2_rn(hi7);
+    const __half2 s_lo = __float2half2_rn(s256 - hi7);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const __half2 x = *reinterpret_cast<const __half2*>(&q[e]);
+      const __half2 v = __hfma2(x, s_lo, __hmul2(x, s_hi));
+      q[e] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[e]));
+      q[e] = pack_half2(f.x * s256, f.y * s256);
+      if constexpr (HOW == kRest) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&q[e]));
+        q[e] = pack_half2(fmaf(f.x, s256, -v.x), fmaf(f.y, s256, -v.y));
+      }
+    }
+  }
+}
+
+// Lane (l & 7)'s 16 values of a 128-wide group as two 16-byte chunks of row
+// `row` in 64-column blocks at `blk` and `blk + stride`. The upper four lanes
+// store their chunks in the other order, so that the eight lanes of a row cover
+// all banks with each store.
+__device__ __forceinline__ void store_group(uint8_t* blk, uint32_t stride, int row, int lane, const uint32_t (&q)[8]) {
+  const int l8 = lane & 7;
+  uint8_t* d = blk + (l8 >> 2) * stride;
+  const int c0 = 2 * (l8 & 3);
+  const bool sw = (l8 >> 2) != 0;
+  *reinterpret_cast<uint4*>(d + sw128_off(row, c0 + (sw ? 1 : 0))) =
+      sw ? make_uint4(q[4], q[5], q[6], q[7]) : make_uint4(q[0], q[1], q[2], q[3]);
+  *reinterpret_cast<uint4*>(d + sw128_off(row, c0 + (sw ? 0 : 1))) =
+      sw ? make_uint4(q[0], q[1], q[2], q[3]) : make_uint4(q[4], q[5], q[6], q[7]);
+}
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t saddr, const void* gptr, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(saddr), "l"(gptr), "r"(on ? 16 : 0));
+}
+
+// Draft columns of request b that some draft sees (the others are not read).
+__device__ __forceinline__ uint64_t seen_columns(const TreeArgs& p, int b, int nd, int lane) {
+  uint64_t m = 0;
+  for (int i = lane; i < nd; i += 32) m |= (uint64_t)p.mask[(int64_t)b * p.mask_stride + i];
+  const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)m);
+  const uint32_t hi = __reduce_or_sync(0xffffffffu, (uint32_t)(m >> 32));
+  return ((uint64_t)hi << 32) | lo;
+}
+
+// Cache row of position pos, or -1 (reads as zeros).
+__device__ __forceinline__ int row_code(const TreeArgs& p, int b, const Req& r, uint64_t seen, int pos) {
+  const int j = pos - (r.seq - r.nd);
+  if (pos >= r.seq || (j >= 0 && !((seen >> j) & 1))) return -1;
+  const int blk = pos / p.page;
+  if (blk >= p.max_blocks) return -1;
+  const int64_t row = (int64_t)p.bt[(int64_t)b * p.bt_stride + blk] * p.page + (pos - blk * p.page);
+  return row >= 0 && row < p.n_kv_rows ? (int)row : -1;
+}
+
+// This CTA's 64 query rows into shared memory (f16, or bf16 as it is): warp w
+// rows 4w + lane / 8, eight lanes a row. qe[row]: the power of two that a bf16
+// row was divided by.
+template <int FMT>
+__device__ __forceinline__ void load_q(const TreeArgs& p, uint8_t* sm_q, int8_t* qe, int b, int row0, int w, int lane) {
+  const int row = 4 * w + (lane >> 3), l8 = lane & 7;
+  const bool on = row0 + row < p.T * p.H;
+  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
+                                                    ((int64_t)b * p.T * p.H + row0 + row) * DK * 2);
+  int e = 0;
+  if (FMT != DSA_BF16 && p.q_bf16) {
+    uint32_t bits = 0;
+    if (on) {
+#pragma unroll 3
+      for (int c = 0; c < 9; ++c) bits = max(bits, bf16x8_max_abs_bits(__ldg(src + l8 + 8 * c)));
+    }
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
+    e = bf16_fp16_shift(bits);
+  }
+#pragma unroll 3
+  for (int c = 0; c < 9; ++c) {
+    uint4 v = on ? __ldg(src + l8 + 8 * c) : make_uint4(0, 0, 0, 0);
+    if (FMT != DSA_BF16 && p.q_bf16) v = bf16x8_to_half8_scaled(v, e);
+    *reinterpret_cast<uint4*>(sm_q + c * kBlk + sw128_off(row, l8)) = v;
+  }
+  if (l8 == 0) qe[row] = (int8_t)e;
+}
+
+// FMT: the cache's format.
+template <int FMT>
+__global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p, int32_t* err) {
+  constexpr bool kFp8 = FMT == DSA_FP8_DS_MLA;
+  constexpr bool kBf16 = FMT == DSA_BF16;
+  constexpr uint32_t IDESC_QK = idesc_f16(kPairRows, kKeys, false, false, kBf16);
+  constexpr uint32_t IDESC_PV = idesc_f16(kPairRows, 256, false, true, kBf16);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  uint8_t* sm = smem_raw + (base - raw_base);
+  uint8_t* misc = sm + SM_MISC;
+  // misc: [0, 104) 13 mbarriers | 104 TMEM base | 108 abort | [112, 144) the
+  // pair's run | [192, 448) qe[4][64] | [448, 1472) rowx[4][64]
+  const uint32_t mb = smem_u32(misc);
+  const uint32_t mb_k_full = mb, mb_k_free = mb + 8, mb_v_full = mb + 16, mb_v_free = mb + 24, mb_p_full = mb + 32,
+                 mb_o_free = mb + 40, mb_done = mb + 48, mb_s_full = mb + 56 /* [2] */, mb_q_full = mb + 72 /* [4] */;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 104);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 108);
+  int* run_left = reinterpret_cast<int*>(misc + 112);
+  int* run_at = reinterpret_cast<int*>(misc + 116);  // b, rt, tile
+  int8_t* qe = reinterpret_cast<int8_t*>(misc + 192);
+  float* rowx = reinterpret_cast<float*>(misc + 448);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank();
+  const int pair = blockIdx.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_init(mb_k_full, 2 * kProducers);
+      mbar_init(mb_k_free, 1);
+      mbar_init(mb_v_full, 2 * kProducers);
+      mbar_init(mb_v_free, 1);
+      mbar_init(mb_p_full, 2 * kSoftmaxWarps);
+      mbar_init(mb_o_free, 2 * kSoftmaxWarps);
+      mbar_init(mb_done, 1);
+      for (int x = 0; x < 2; ++x) mbar_init(mb_s_full + 8 * x, 1);
+      for (int x = 0; x < 4; ++x) mbar_init(mb_q_full + 8 * x, kProducers);
+      mbar_init_fence();
+      *abort_flag = 0;
+    }
+    __syncwarp();
+    tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+  } else if (warp == 1) {
+    // this pair's run of the list of tiles
+    const long long work = warp_work(p, p.B, lane);
+    const long long chunk = chunk_of(work, p.pairs);
+    const long long w0 = chunk * pair;
+    const long long left = max(min(chunk, work - w0), 0ll);
+    if (left > 0) {
+      long long before = 0;
+      for (int b0 = 0;; b0 += 32) {
+        Req r{0, 0, 0, 0};
+        if (b0 + lane < p.B) r = load_req(p, b0 + lane);
+        const long long mine = (long long)r.nt * r.nrt;
+        long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w0);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            const long long at = w0 - (before + incl - mine);
+            run_at[0] = b0 + lane;
+            run_at[1] = (int)(at / r.nt);
+            run_at[2] = (int)(at % r.nt);
+          }
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    if (lane == 0) *run_left = (int)left;
+  }
+  fence_before_sync();
   __syncthreads();
-  for (int r = 0; r < TR && r0 + r < R; ++r) {
-    const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
-    const int64_t at = ((int64_t)b * R + r0 + r);
-    for (int c = 0; c < 2; ++c) {
-      const int64_t e = at * DV + threadIdx.x + 256 * c;
-      if (p.o_bf16)
-        reinterpret_cast<__nv_bfloat16*>(p.o)[e] = __float2bfloat16_rn(acc[r][c] * inv);
-      else
-        reinterpret_cast<__half*>(p.o)[e] = __float2half_rn(acc[r][c] * inv);
+  cluster_sync();  // both CTAs' barriers exist and TMEM is allocated
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  Cursor start;
+  start.left = *run_left;
+  start.b = run_at[0];
+  start.rt = run_at[1];
+  start.tile = run_at[2];
+  start.seg = 0;
+  start.first = true;
+  start.r = Req{0, 0, 0, 0};
+  if (start.left > 0) start.r = load_req(p, start.b);
+
+  bool ok = true;
+  // After a wait that ran out (`ok` false, abort flag set) every thread still
+  // executes its role's barriers and arrivals, and later waits return at once.
+  if (warp < kProducers) {
+    // ------------------------------------------------------------- producers
+    const int w = warp;
+    const uint32_t k_full0 = cluster_map(mb_k_full, 0), v_full0 = cluster_map(mb_v_full, 0);
+    // K runs one tile ahead of V: K(t+1) is stored before V(t)
+    Cursor c = start;               // the tile whose K is stored next
+    int kc = 0;                     // K stores so far (two per tile in two-pass segments)
+    uint64_t seen = 0;
+    // rows of tile c: lanes 0-3 K keys 4w + lane of this CTA's half, lanes 4-11 V keys 8w + lane - 4
+    auto codes = [&]() {
+      if (c.first || kc == 0) seen = seen_columns(p, c.b, c.r.nd, lane);
+      int code = -1;
+      if (lane < 12)
+        code = row_code(p, c.b, c.r, seen, c.tile * kKeys + (lane < 4 ? 64 * rank + 4 * w + lane : 8 * w + lane - 4));
+      return code;
+    };
+    auto start_segment = [&]() {
+      if (ok) load_q<FMT>(p, sm + SM_Q, qe + 64 * (c.seg & 3), c.b, c.rt * kPairRows + kRows * rank, w, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb_q_full + 8 * (c.seg & 3));
+    };
+    const int krow = 4 * w + (lane >> 3), vrow = 8 * w + (lane >> 3);
+    const int total = c.left;
+    if constexpr (kFp8) {
+      uint4 kd[4], kr, vd[4];  // K: 4 groups and the rotary tail of this lane's key | V: [key][group]
+      float4 ks;
+      float vs[4];
+      auto load_k = [&](int codes_at) {
+        const int code = __shfl_sync(0xffffffffu, codes_at, lane >> 3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kd[j] = make_uint4(0, 0, 0, 0);
+        ks = make_float4(1.f, 1.f, 1.f, 1.f);
+        kr = make_uint4(0, 0, 0, 0);
+        if (code >= 0) {
+          const uint8_t* row = p.kv + (int64_t)code * 656 + 16 * (lane & 7);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kd[j] = ldg_nc16(row + 128 * j);
+          kr = ldg_nc16(row + 528);
+          const uint4 x = ldg_nc16(row + 512 - 16 * (lane & 7));
+          ks = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+        }
+      };
+      auto load_v = [&](int codes_at) {
+#pragma unroll
+        for (int rs = 0; rs < 2; ++rs) {
+          const int code = __shfl_sync(0xffffffffu, codes_at, 4 + (lane >> 3) + 4 * rs);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            vd[2 * rs + h] = make_uint4(0, 0, 0, 0);
+            vs[2 * rs + h] = 1.f;
+            if (code >= 0) {
+              const uint8_t* row = p.kv + (int64_t)code * 656;
+              vd[2 * rs + h] = ldg_nc16(row + 16 * ((lane & 7) + 8 * (2 * h + rank)));
+              vs[2 * rs + h] = __ldg(reinterpret_cast<const float*>(row + 512) + 2 * h + rank);
+            }
+          }
+        }
+      };
+      // In two-pass tiles the first pass rounds in f32 too: the second takes its remainder.
+      auto put_k = [&](auto how) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t q[8];
+          dequant16<decltype(how)::value>(kd[j], j == 0 ? ks.x : j == 1 ? ks.y : j == 2 ? ks.z : ks.w, q);
+          store_group(sm + SM_K + 2 * j * kBlk, kBlk, krow, lane, q);
+        }
+      };
+      auto put_v = [&](auto how) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t q[8];
+          dequant16<decltype(how)::value>(vd[x], vs[x], q);
+          store_group(sm + SM_V + 2 * (x & 1) * kVBlk, kVBlk, vrow + 4 * (x >> 1), lane, q);
+        }
+      };
+      // K of tile c: wait for the buffer, store, announce
+      auto store_k = [&]() {
+        if (kc > 0) ok = ok && mbar_wait_cluster(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+        if (c.first) start_segment();
+        const int passes = c.r.seq <= kTwoPassKeys ? 2 : 1;
+#pragma unroll 1
+        for (int s = 0; s < passes; ++s) {
+          if (s > 0) ok = ok && mbar_wait_cluster(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+          if (ok) {
+            if (s > 0)
+              put_k(std::integral_constant<int, kRest>());
+            else if (passes == 1 && __all_sync(0xffffffffu, fast_scale(ks.x) && fast_scale(ks.y) && fast_scale(ks.z) &&
+                                                                fast_scale(ks.w)))
+              put_k(std::integral_constant<int, kFast>());
+            else
+              put_k(std::integral_constant<int, kWide>());
+            *reinterpret_cast<uint4*>(sm + SM_K + 8 * kBlk + sw128_off(krow, lane & 7)) =
+                s > 0 ? make_uint4(0, 0, 0, 0) : kr;
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(k_full0);
+          ++kc;
+        }
+        c.next(p);
+      };
+      int code0 = -1, code1 = -1;  // rows of the tile of the next V load, and of the tile after it
+      if (total > 0) {
+        code0 = codes();
+        load_k(code0);
+        load_v(code0);
+        store_k();
+        if (c.left > 0) {
+          code0 = codes();
+          load_k(code0);
+        }
+      }
+      for (int t = 0; t < total; ++t) {
+        if (t + 1 < total) {
+          store_k();
+          if (c.left > 0) {
+            code1 = codes();
+            load_k(code1);
+          }
+        }
+        if (t > 0) ok = ok && mbar_wait_cluster(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
+        if (ok) {
+          if (__all_sync(0xffffffffu, fast_scale(vs[0]) && fast_scale(vs[1]) && fast_scale(vs[2]) && fast_scale(vs[3])))
+            put_v(std::integral_constant<int, kFast>());
+          else
+            put_v(std::integral_constant<int, kWide>());
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(v_full0);
+        if (t + 1 < total) load_v(code0);
+        code0 = code1;
+      }
+    } else {
+      auto store_k = [&](int codes_at) {
+        const int code = __shfl_sync(0xffffffffu, codes_at, lane >> 3);
+        if (kc > 0) ok = ok && mbar_wait_cluster(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+        if (ok) {
+          const uint8_t* row = p.kv + (int64_t)max(code, 0) * (DK * 2) + 16 * (lane & 7);
+#pragma unroll
+          for (int x = 0; x < 9; ++x)
+            cp_async16_zfill(base + SM_K + x * kBlk + sw128_off(krow, lane & 7), row + 128 * x, code >= 0);
+        }
+        cp_async_commit();
+        if (c.first) start_segment();
+        cp_async_wait<0>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(k_full0);
+        ++kc;
+        c.next(p);
+      };
+      int code0 = -1, code1 = -1;
+      if (total > 0) {
+        code0 = codes();
+        store_k(code0);
+      }
+      for (int t = 0; t < total; ++t) {
+        if (t + 1 < total) {
+          code1 = codes();
+          store_k(code1);
+        }
+        if (t > 0) ok = ok && mbar_wait_cluster(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
+#pragma unroll
+        for (int rs = 0; rs < 2; ++rs) {
+          const int code = __shfl_sync(0xffffffffu, code0, 4 + (lane >> 3) + 4 * rs);
+          const uint8_t* row = p.kv + (int64_t)max(code, 0) * (DK * 2) + 256 * rank + 16 * (lane & 7);
+          if (ok) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)  // block x: columns [256 (x / 2) + 128 rank + 64 (x % 2), +64)
+              cp_async16_zfill(base + SM_V + x * kVBlk + sw128_off(vrow + 4 * rs, lane & 7),
+                               row + 512 * (x >> 1) + 128 * (x & 1), code >= 0);
+          }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(v_full0);
+        code0 = code1;
+      }
     }
-    if (threadIdx.x == 0) p.lse[at] = l[r] > 0.f ? (m[r] + log2f(l[r])) * 0.69314718055994530942f : -INFINITY;
+  } else if (warp == kMmaWarp) {
+    // ----------------------------------------------------------- MMA issue
+    if (rank == 0 && lane == 0) {
+      // made anew for each tile: kept across the loop, the 104 advanced descriptors would take all registers
+      auto desc = [&](uint32_t at, uint32_t lbo) {
+        asm volatile("" : "+r"(at));
+        return sw128_desc(base + at, lbo, 1024);
+      };
+      Cursor cq = start, cp = start;
+      int kc = 0, gq = 0, gp = 0;
+      auto qk = [&]() {
+        const int passes = kFp8 && cq.r.seq <= kTwoPassKeys ? 2 : 1;
+        for (int s = 0; s < passes; ++s) {
+          ok = ok && mbar_wait_cluster(mb_k_full, kc & 1, abort_flag, err, kWaitNs);
+          if (ok) {
+            fence_after_sync();
+            const uint64_t dq = desc(SM_Q, 16), dk = desc(SM_K, 16);
+#pragma unroll
+            for (int kb = 0; kb < 9; ++kb)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_f16_ss_pair(tmem + S_COL + 64 * (gq & 1), dq + ((kb * kBlk + 32 * k) >> 4),
+                                dk + ((kb * kBlk + 32 * k) >> 4), IDESC_QK, (kb | k) != 0 || s > 0);
+            mma_commit_pair(mb_k_free);
+          }
+          ++kc;
+        }
+        if (ok) mma_commit_pair(mb_s_full + 8 * (gq & 1));
+        ++gq;
+        cq.next(p);
+      };
+      if (cq.left > 0) qk();
+      while (cp.left > 0 && ok) {
+        if (cq.left > 0) qk();
+        ok = ok && mbar_wait_cluster(mb_v_full, gp & 1, abort_flag, err, kWaitNs) &&
+             mbar_wait_cluster(mb_p_full, gp & 1, abort_flag, err, kWaitNs);
+        // the accumulator of the segment before has been read
+        if (cp.first && cp.seg > 0) ok = ok && mbar_wait_cluster(mb_o_free, (cp.seg - 1) & 1, abort_flag, err, kWaitNs);
+        if (ok) {
+          fence_after_sync();
+          const uint64_t dp = desc(SM_P, 16), dv = desc(SM_V, kVBlk);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < kKeys / 16; ++s)
+              mma_f16_ss_pair(tmem + 128 * h, dp + (((s >> 2) * kBlk + 32 * (s & 3)) >> 4),
+                              dv + ((2 * h * kVBlk + 2048 * s) >> 4), IDESC_PV, !cp.first || s > 0);
+          mma_commit_pair(mb_v_free);
+        }
+        ++gp;
+        cp.next(p);
+      }
+      mma_commit_pair(mb_done);  // every MMA of this thread
+    }
+    __syncwarp();
+  } else if (warp >= kSoftmax0 && warp < kSoftmax0 + kSoftmaxWarps) {
+    // ------------------------------------------------------------- softmax
+    const int sp = warp & 3;                    // TMEM sub-partition: lanes [32 sp, +32)
+    const int hh = (warp - kSoftmax0) >> 2;     // S columns [32 hh, +32), O half hh
+    const int row = 32 * (sp & 1) + lane;       // of this CTA
+    const int q4 = 2 * (sp >> 1) + hh;          // this thread's quarter of the row's keys
+    const int kofs = 64 * (sp >> 1) + 32 * hh;  // its first key
+    const uint32_t t_sp = tmem + ((uint32_t)(32 * sp) << 16);
+    const uint32_t p_full0 = cluster_map(mb_p_full, 0), o_free0 = cluster_map(mb_o_free, 0);
+    uint8_t* prow = sm + SM_P + (sp >> 1) * kBlk;
+    Cursor c = start;
+    int g = 0;
+    float m = kNoMax, L = 0.f, rs = 0.f;
+    int pre = 0;           // context positions; kNoRow for a row of no draft
+    bool full = false;     // the segment holds every key tile
+    for (; c.left > 0;) {
+      if (c.first) {
+        ok = ok && mbar_wait(mb_q_full + 8 * (c.seg & 3), (c.seg >> 2) & 1, abort_flag, err, kWaitNs);
+        const int r = c.rt * kPairRows + kRows * rank + row;
+        const int i = r / p.H;
+        const bool on = i < c.r.nd;
+        rs = p.scale_log2 * __int_as_float((127 + (int)qe[64 * (c.seg & 3) + row]) << 23);
+        pre = on ? c.r.seq - c.r.nd : kNoRow;
+        full = c.tile == 0 && c.left >= c.r.nt;
+        m = kNoMax;
+        L = 0.f;
+      }
+      const bool first = c.first;
+      // keys this thread's row sees, one bit each
+      const int d = pre == kNoRow ? -64 : pre - (c.tile * kKeys + kofs);
+      uint32_t allow = d >= 32 ? 0xffffffffu : d > 0 ? (1u << d) - 1 : 0u;
+      if (d < 32 && d > -64) {  // drafts among the keys
+        uint64_t bits = (uint64_t)p.mask[(int64_t)c.b * p.mask_stride + (c.rt * kPairRows + kRows * rank + row) / p.H];
+        if (c.r.nd < 64) bits &= (1ull << c.r.nd) - 1;
+        allow |= (uint32_t)(d >= 0 ? bits << d : bits >> -d);
+      }
+      ok = ok && mbar_wait_cluster(mb_s_full + 8 * (g & 1), (g >> 1) & 1, abort_flag, err, kWaitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      fence_after_sync();
+      uint32_t s[32];
+      if (ok) {
+        tmem_ld32(t_sp + S_COL + 64 * (g & 1) + 32 * hh, s);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[j] = 0u;
+      }
+      float mx = -INFINITY;
+      if (allow == 0xffffffffu) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float z = __uint_as_float(s[j]) * rs;
+          s[j] = __float_as_uint(z);
+          mx = fmaxf(mx, z);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float z = (allow >> j) & 1 ? __uint_as_float(s[j]) * rs : -INFINITY;
+          s[j] = __float_as_uint(z);
+          mx = fmaxf(mx, z);
+        }
+      }
+      float alpha = 1.f;
+      const bool any = named_bar_or(1, kSoftmaxWarps * 32, mx > m + kRescale);
+      if (any) {
+        rowx[64 * q4 + row] = mx;
+        named_bar(1, kSoftmaxWarps * 32);
+        const float rm = fmaxf(fmaxf(rowx[row], rowx[64 + row]), fmaxf(rowx[128 + row], rowx[192 + row]));
+        if (rm > m + kRescale) {
+          alpha = ex2(m - rm);
+          m = rm;
+          L *= alpha;
+        }
+      }
+      uint32_t pk[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float a = ex2(__uint_as_float(s[2 * j]) - m), b = ex2(__uint_as_float(s[2 * j + 1]) - m);
+        L += a + b;
+        if (kBf16) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+          pk[j] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          pk[j] = pack_half2(a, b);
+        }
+      }
+      if (!first) {  // P's buffer and O are free once PV(t-1) has completed (the epilogue waited for the last one)
+        ok = ok && mbar_wait_cluster(mb_v_free, (g - 1) & 1, abort_flag, err, kWaitNs);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok && __any_sync(0xffffffffu, alpha != 1.f)) {
+          fence_after_sync();
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            uint32_t o[32];
+            const uint32_t at = t_sp + 128 * hh + 32 * k;
+            tmem_ld32(at, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st32(at, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      if (ok) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) =
+              make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
+      }
+      fence_proxy_async();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(p_full0);
+      const bool last = c.last();
+      if (last) {
+        // ------------------------------------------- epilogue of the segment
+        named_bar(1, kSoftmaxWarps * 32);  // rowx: every thread is past its use as maxima
+        rowx[64 * q4 + row] = L;
+        named_bar(1, kSoftmaxWarps * 32);
+        L = (rowx[row] + rowx[64 + row]) + (rowx[128 + row] + rowx[192 + row]);
+        named_bar(1, kSoftmaxWarps * 32);
+        ok = ok && mbar_wait_cluster(mb_v_free, g & 1, abort_flag, err, kWaitNs);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          fence_after_sync();
+          const bool mine = c.rt * kPairRows + kRows * rank + row < p.T * p.H;
+          const int slot = 2 * pair + (c.seg == 0 ? 0 : 1);
+          const int col0 = 256 * hh + 128 * (sp >> 1);
+          const int64_t grow = (int64_t)c.b * p.T * p.H + c.rt * kPairRows + kRows * rank + row;
+          const int64_t prow_i = (int64_t)slot * p.slot_rows + kRows * rank + row;
+          const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            uint32_t o[32];
+            tmem_ld32(t_sp + 128 * hh + 32 * k, o);
+            tmem_wait_ld();
+            if (!mine) continue;
+            if (full) {
+              uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.o) + (grow * DV + col0 + 32 * k) * 2);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t v[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float a = __uint_as_float(o[8 * e + 2 * x]) * inv, b = __uint_as_float(o[8 * e + 2 * x + 1]) * inv;
+                  if (p.o_bf16) {
+                    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+                    v[x] = *reinterpret_cast<const uint32_t*>(&t);
+                  } else {
+                    v[x] = pack_half2(a, b);
+                  }
+                }
+                dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
+              }
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(p.part_o + prow_i * DV + col0 + 32 * k);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+          }
+          if (mine && q4 == 0) {
+            if (full) {
+              p.lse[grow] = L > 0.f ? (m + log2f(L)) * kLn2 : -INFINITY;
+            } else {
+              p.part_ml[prow_i * 2] = m;
+              p.part_ml[prow_i * 2 + 1] = L;
+            }
+          }
+        }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(o_free0);
+      }
+      ++g;
+      c.next(p);
+    }
   }
+  // every MMA has completed before TMEM is released, and no CTA leaves while the
+  // other may still read its shared memory or arrive on its barriers
+  __syncthreads();
+  mbar_wait_drain(mb_done, 0, kWaitNs);
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 0) {
+    fence_after_sync();
+    tmem_dealloc_pair(tmem, TMEM_COLS);
+  }
+}
+
+// Rows whose key tiles lie in several segments: o = sum_s w_s o_s / sum_s w_s l_s
+// with w_s = 2^(m_s - max m); rows of no segment: o = 0, lse = -inf. One block
+// per 8 rows, a warp a row, 16 columns a lane; the segments are found as the
+// main kernel cut them.
+constexpr int kMergeRows = 8;
+__global__ void __launch_bounds__(32 * kMergeRows) tree_merge_kernel(const TreeArgs p) {
+  const int lane = threadIdx.x & 31;
+  const int rt = blockIdx.y / (kPairRows / kMergeRows);
+  const int row = (blockIdx.y % (kPairRows / kMergeRows)) * kMergeRows + (threadIdx.x >> 5);  // of the row tile
+  const int b = blockIdx.x;
+  const int64_t r = (int64_t)rt * kPairRows + row;
+  if (r >= (int64_t)p.T * p.H) return;
+  const int64_t grow = (int64_t)b * p.T * p.H + r;
+  const Req q = load_req(p, b);
+  float acc[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  float M = -INFINITY, L = 0.f;
+  if (q.nt > 0 && rt < q.nrt) {
+    const long long chunk = chunk_of(warp_work(p, p.B, lane), p.pairs);
+    const long long w0 = warp_work(p, b, lane) + (long long)rt * q.nt;
+    const int p0 = (int)(w0 / chunk), p1 = (int)((w0 + q.nt - 1) / chunk);
+    if (p0 == p1) return;  // one segment: the main kernel wrote the row
+    for (int s = p0; s <= p1; ++s) {
+      // the segment that starts a row tile inside its pair's run is the run's last: slot 1
+      const int64_t at = (int64_t)(2 * s + (s == p0 && w0 > s * chunk ? 1 : 0)) * p.slot_rows + row;
+      const float l = p.part_ml[at * 2 + 1];
+      if (!(l > 0.f)) {
+        if (l != l) L = l;  // NaN scores stay NaN
+        continue;
+      }
+      const float m = p.part_ml[at * 2];
+      const float Mn = fmaxf(M, m);
+      const float a = M == -INFINITY ? 0.f : exp2f(M - Mn), w = exp2f(m - Mn);
+      M = Mn;
+      L = L * a + l * w;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DV + 128 * c + 4 * lane);
+        acc[4 * c] = acc[4 * c] * a + v.x * w;
+        acc[4 * c + 1] = acc[4 * c + 1] * a + v.y * w;
+        acc[4 * c + 2] = acc[4 * c + 2] * a + v.z * w;
+        acc[4 * c + 3] = acc[4 * c + 3] * a + v.w * w;
+      }
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint2 v;
+    if (p.o_bf16) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(acc[4 * c] * inv, acc[4 * c + 1] * inv);
+      const __nv_bfloat162 y = __floats2bfloat162_rn(acc[4 * c + 2] * inv, acc[4 * c + 3] * inv);
+      v = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    } else {
+      v = make_uint2(pack_half2(acc[4 * c] * inv, acc[4 * c + 1] * inv),
+                     pack_half2(acc[4 * c + 2] * inv, acc[4 * c + 3] * inv));
+    }
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.o) + (grow * DV + 128 * c + 4 * lane) * 2) = v;
+  }
+  if (lane == 0) p.lse[grow] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+}
+
+std::once_flag g_once[kMaxDevices];
+int g_status[kMaxDevices];
+int32_t* g_err[kMaxDevices];
+int g_pairs[kMaxDevices];
+
+template <int FMT>
+cudaError_t setup_kernel() {
+  return cudaFuncSetAttribute(tree_mla_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+}
+
+cudaLaunchConfig_t pair_config(int pairs, cudaStream_t s, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = s;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = 2;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+int ensure_setup(int dev) {
+  if (dev < 0 || dev >= kMaxDevices) {
+    set_error("tree_mla_decode: device index %d out of range", dev);
+    return DSA_ERR_UNSUPPORTED;
+  }
+  std::call_once(g_once[dev], [dev] {
+    cudaError_t e = setup_kernel<DSA_FP8_DS_MLA>();
+    if (e == cudaSuccess) e = setup_kernel<DSA_F16>();
+    if (e == cudaSuccess) e = setup_kernel<DSA_BF16>();
+    int n = 0;
+    if (e == cudaSuccess) {
+      cudaLaunchAttribute attr{};
+      const cudaLaunchConfig_t cfg = pair_config(sm_count(dev) / 2, nullptr, &attr);
+      e = cudaOccupancyMaxActiveClusters(&n, tree_mla_kernel<DSA_FP8_DS_MLA>, &cfg);
+    }
+    if (e == cudaSuccess && tc_error_word(dev, &g_err[dev]) != DSA_OK) e = cudaErrorUnknown;
+    g_pairs[dev] = n;
+    g_status[dev] = (int)e;
+  });
+  if (g_status[dev] != 0 || g_pairs[dev] <= 0) {
+    set_error("tree_mla_decode setup: %s (%d clusters of two CTAs fit)", cudaGetErrorString((cudaError_t)g_status[dev]),
+              g_pairs[dev]);
+    return DSA_ERR_CUDA;
+  }
+  return DSA_OK;
+}
+
+template <int FMT>
+cudaError_t launch_main(const TreeArgs& p, int dev, cudaStream_t s) {
+  cudaLaunchAttribute attr{};
+  const cudaLaunchConfig_t cfg = pair_config(p.pairs, s, &attr);
+  return cudaLaunchKernelEx(&cfg, tree_mla_kernel<FMT>, p, g_err[dev]);
 }
 
 }  // namespace
@@ -133,7 +917,16 @@ __global__ void __launch_bounds__(NT) tree_simple_kernel(const TreeArgs p) {
 
 using namespace dsa;
 
-extern "C" size_t dsa_tree_mla_decode_workspace_bytes(int B, int T, int n_head) { return 0; }
+// Two partial states per pair, of the rows that a pair can hold.
+static size_t tree_workspace(int T, int n_head, int pairs) {
+  const int64_t rows = std::min<int64_t>(kPairRows, (int64_t)T * n_head);
+  return (size_t)2 * pairs * rows * kSlotF * sizeof(float);
+}
+
+extern "C" size_t dsa_tree_mla_decode_workspace_bytes(int B, int T, int n_head) {
+  if (B <= 0 || T <= 0 || n_head <= 0) return 0;
+  return tree_workspace(T, n_head, sm_count(current_device()) / 2);
+}
 
 extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void* q, int q_dtype, const void* kv_cache,
                                    int kv_format, int64_t n_kv_rows, int page_size, const int32_t* block_table,
@@ -161,12 +954,48 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
               DSA_ERR_INVALID, "tree_mla_decode: null pointer");
   DSA_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)kv_cache & 15) == 0 && ((uintptr_t)o & 15) == 0, DSA_ERR_INVALID,
               "tree_mla_decode: q, kv_cache and o must be 16-byte aligned");
-  TreeArgs p{q, reinterpret_cast<const uint8_t*>(kv_cache), block_table, seq_lens, draft_lens, tree_mask, o, lse,
-             n_kv_rows, bt_stride, mask_stride, kv_format, page_size, max_blocks, T, n_head, q_dtype == DSA_BF16,
-             o_dtype == DSA_BF16, (float)(scale * 1.4426950408889634)};
-  constexpr int kSmem = (TR * DK + TK * DK + TR * TK + 3 * TR) * 4;
-  DSA_CUDA_TRY(cudaFuncSetAttribute(tree_simple_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
-               "tree_mla_decode setup");
-  tree_simple_kernel<<<dim3((T * n_head + TR - 1) / TR, B), NT, kSmem, as_stream(stream)>>>(p);
-  return check_launch("tree_simple_kernel");
+  const int64_t most = (int64_t)B * (((int64_t)T * n_head + kPairRows - 1) / kPairRows) *
+                       std::max<int64_t>(1, ((int64_t)max_blocks * page_size + kKeys - 1) / kKeys);
+  const int dev = current_device();
+  const int st = ensure_setup(dev);
+  if (st != DSA_OK) return st;
+  TreeArgs p{};
+  p.q = q;
+  p.kv = reinterpret_cast<const uint8_t*>(kv_cache);
+  p.bt = block_table;
+  p.seq_lens = seq_lens;
+  p.draft_lens = draft_lens;
+  p.mask = tree_mask;
+  p.o = o;
+  p.lse = lse;
+  p.n_kv_rows = n_kv_rows;
+  p.bt_stride = bt_stride;
+  p.mask_stride = mask_stride;
+  p.page = page_size;
+  p.max_blocks = max_blocks;
+  p.B = B;
+  p.T = T;
+  p.H = n_head;
+  p.pairs = (int)std::min<int64_t>(std::min(g_pairs[dev], sm_count(dev) / 2), most);
+  p.slot_rows = (int)std::min<int64_t>(kPairRows, (int64_t)T * n_head);
+  p.q_bf16 = q_dtype == DSA_BF16;
+  p.o_bf16 = o_dtype == DSA_BF16;
+  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  const size_t need = tree_workspace(T, n_head, p.pairs);
+  DSA_REQUIRE(workspace != nullptr && workspace_bytes >= need, DSA_ERR_WORKSPACE,
+              "tree_mla_decode: workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  DSA_REQUIRE(((uintptr_t)workspace & 15) == 0, DSA_ERR_INVALID, "tree_mla_decode: workspace must be 16-byte aligned");
+  p.part_o = reinterpret_cast<float*>(workspace);
+  p.part_ml = p.part_o + (size_t)2 * p.pairs * p.slot_rows * DV;
+  cudaStream_t s = as_stream(stream);
+  const cudaError_t e = kv_format == DSA_FP8_DS_MLA ? launch_main<DSA_FP8_DS_MLA>(p, dev, s)
+                        : kv_format == DSA_F16      ? launch_main<DSA_F16>(p, dev, s)
+                                                    : launch_main<DSA_BF16>(p, dev, s);
+  if (e != cudaSuccess) {
+    set_error("tree_mla_kernel launch: %s", cudaGetErrorString(e));
+    return DSA_ERR_CUDA;
+  }
+  const int rt = (T * n_head + kPairRows - 1) / kPairRows;
+  tree_merge_kernel<<<dim3(B, rt * (kPairRows / kMergeRows)), 32 * kMergeRows, 0, s>>>(p);
+  return check_launch("tree_merge_kernel");
 }
