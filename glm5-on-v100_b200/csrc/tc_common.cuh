@@ -303,36 +303,11 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 // Arrive on an mbarrier of any CTA of the cluster (a shared::cluster address).
+// What it announces are this CTA's own shared-memory writes, made visible to
+// the tensor cores by fence_proxy_async before: no cluster-scope release, which
+// would drain this warp's outstanding global loads too.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mbar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t mbar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred P1;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, P1;\n\t}"
-      : "=r"(ok)
-      : "r"(mbar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// mbar_wait with cluster-scope acquire: for phases that the other CTA completes.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t mbar, uint32_t parity, volatile int* abort, int32_t* err,
-                                                  uint64_t timeout_ns) {
-  if (mbar_try_wait_cluster(mbar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait_cluster(mbar, parity)) return true;
-    if ((it & 255u) == 0) {
-      if (*abort) return false;
-      if (globaltimer_ns() - t0 > timeout_ns) {
-        *abort = 1;
-        if (err) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
-        return false;
-      }
-    }
-  }
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
 // Named barrier that also ORs a predicate over its threads.
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool pred) {

@@ -44,6 +44,7 @@
 // scale undoes exactly. The running maximum moves only when a score exceeds it
 // by 2^8, so P <= 256 and O is rarely rescaled.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -98,9 +99,10 @@ struct TreeArgs {
   float* part_o;   // [2 * pairs][slot_rows][512]
   float* part_ml;  // [2 * pairs][slot_rows][2]
   int64_t n_kv_rows, bt_stride, mask_stride;
-  int page, max_blocks, B, T, H, pairs, slot_rows;
+  int page, page_shift, max_blocks, B, T, H, pairs, slot_rows;  // page_shift < 0: no power of two
   int q_bf16, o_bf16;
-  float scale_log2;
+  uint32_t q_sign;   // 0x80008000 for a negative scale
+  float scale_log2;  // its magnitude
 };
 
 // Request b's size: key tiles and row tiles (0 tiles: nothing to do).
@@ -160,57 +162,64 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// How a group of codes is expanded to f16: the product code * scale rounded
-// once, by f16 arithmetic where scale * 256 keeps every product normal
+// How codes are expanded to f16: the product code * scale rounded once, by f16
+// arithmetic where the scale's parts and the products stay in f16's range
 // (kFast), by f32 elsewhere (kWide), or what that rounding left (kRest).
 enum { kFast, kWide, kRest };
-__device__ __forceinline__ bool fast_scale(float sc) { return sc >= 0x1p-15f && sc <= 128.0f; }
+__device__ __forceinline__ bool fast_scale(float sc) { return sc >= 0x1p-10f && sc <= 128.0f; }
 
+// Volatile: else the expansions that the three ways share are formed before the
+// choice between them and held for all 64 codes of a lane.
+__device__ __forceinline__ uint32_t pinned(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+
+// A scale for kFast: hi cut to 7 significant bits, so that a code (4 bits) times
+// hi is exact in f16's 11 bits and fma(code, lo, code * hi) rounds the whole
+// product once (lo = scale - hi keeps the scale to 2^-15 of it or better).
+struct Scale {
+  float f;
+  __half2 hi, lo;
+  __device__ __forceinline__ explicit Scale(float sc) : f(sc) {
+    const float h = __uint_as_float(__float_as_uint(sc) & 0xFFFE0000u);
+    hi = __float2half2_rn(h);
+    lo = __float2half2_rn(sc - h);
+  }
+};
+
+// Eight codes -> eight f16 values.
 template <int HOW>
-__device__ __forceinline__ void dequant16(const uint4& r, float sc, uint32_t (&q)[8]) {
-  e4m3x4_to_half2x2_div256(r.x, q[0], q[1]);
-  e4m3x4_to_half2x2_div256(r.y, q[2], q[3]);
-  e4m3x4_to_half2x2_div256(r.z, q[4], q[5]);
-  e4m3x4_to_half2x2_div256(r.w, q[6], q[7]);
-  const float s256 = sc * 256.0f;
-  if constexpr (HOW == kFast) {
-    // scale = hi + lo with hi cut to 7 significant bits: a code (4 bits) times
-    // hi is exact in f16's 11 bits, so the fma rounds the whole product once
-    const float hi7 = __uint_as_float(__float_as_uint(s256) & 0xFFFE0000u);
-    const __half2 s_hi = __float2half2_rn(hi7);
-    const __half2 s_lo = __float2half2_rn(s256 - hi7);
+__device__ __forceinline__ uint4 dequant8(uint2 v, const Scale& sc) {
+  __half2 x[4];
+  e4m3x4_to_half2x2(pinned(v.x), x[0], x[1]);
+  e4m3x4_to_half2x2(pinned(v.y), x[2], x[3]);
+  uint32_t q[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const __half2 x = *reinterpret_cast<const __half2*>(&q[e]);
-      const __half2 v = __hfma2(x, s_lo, __hmul2(x, s_hi));
-      q[e] = *reinterpret_cast<const uint32_t*>(&v);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[e]));
-      q[e] = pack_half2(f.x * s256, f.y * s256);
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (HOW == kFast) {
+      const __half2 y = __hfma2(x[e], sc.lo, __hmul2(x[e], sc.hi));
+      q[e] = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+      const float2 f = __half22float2(x[e]);
+      q[e] = pack_half2(f.x * sc.f, f.y * sc.f);
       if constexpr (HOW == kRest) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&q[e]));
-        q[e] = pack_half2(fmaf(f.x, s256, -v.x), fmaf(f.y, s256, -v.y));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&q[e]));
+        q[e] = pack_half2(fmaf(f.x, sc.f, -y.x), fmaf(f.y, sc.f, -y.y));
       }
     }
   }
+  return make_uint4(q[0], q[1], q[2], q[3]);
 }
 
-// Lane (l & 7)'s 16 values of a 128-wide group as two 16-byte chunks of row
-// `row` in 64-column blocks at `blk` and `blk + stride`. The upper four lanes
-// store their chunks in the other order, so that the eight lanes of a row cover
-// all banks with each store.
-__device__ __forceinline__ void store_group(uint8_t* blk, uint32_t stride, int row, int lane, const uint32_t (&q)[8]) {
-  const int l8 = lane & 7;
-  uint8_t* d = blk + (l8 >> 2) * stride;
-  const int c0 = 2 * (l8 & 3);
-  const bool sw = (l8 >> 2) != 0;
-  *reinterpret_cast<uint4*>(d + sw128_off(row, c0 + (sw ? 1 : 0))) =
-      sw ? make_uint4(q[4], q[5], q[6], q[7]) : make_uint4(q[0], q[1], q[2], q[3]);
-  *reinterpret_cast<uint4*>(d + sw128_off(row, c0 + (sw ? 0 : 1))) =
-      sw ? make_uint4(q[0], q[1], q[2], q[3]) : make_uint4(q[4], q[5], q[6], q[7]);
+__device__ __forceinline__ uint2 ldg_nc8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void sts16(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t saddr, const void* gptr, bool on) {
@@ -230,7 +239,7 @@ __device__ __forceinline__ uint64_t seen_columns(const TreeArgs& p, int b, int n
 __device__ __forceinline__ int row_code(const TreeArgs& p, int b, const Req& r, uint64_t seen, int pos) {
   const int j = pos - (r.seq - r.nd);
   if (pos >= r.seq || (j >= 0 && !((seen >> j) & 1))) return -1;
-  const int blk = pos / p.page;
+  const int blk = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page;
   if (blk >= p.max_blocks) return -1;
   const int64_t row = (int64_t)p.bt[(int64_t)b * p.bt_stride + blk] * p.page + (pos - blk * p.page);
   return row >= 0 && row < p.n_kv_rows ? (int)row : -1;
@@ -261,6 +270,7 @@ __device__ __forceinline__ void load_q(const TreeArgs& p, uint8_t* sm_q, int8_t*
   for (int c = 0; c < 9; ++c) {
     uint4 v = on ? __ldg(src + l8 + 8 * c) : make_uint4(0, 0, 0, 0);
     if (FMT != DSA_BF16 && p.q_bf16) v = bf16x8_to_half8_scaled(v, e);
+    v = make_uint4(v.x ^ p.q_sign, v.y ^ p.q_sign, v.z ^ p.q_sign, v.w ^ p.q_sign);
     *reinterpret_cast<uint4*>(sm_q + c * kBlk + sw128_off(row, l8)) = v;
   }
   if (l8 == 0) qe[row] = (int8_t)e;
@@ -271,6 +281,7 @@ template <int FMT>
 __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p, int32_t* err) {
   constexpr bool kFp8 = FMT == DSA_FP8_DS_MLA;
   constexpr bool kBf16 = FMT == DSA_BF16;
+  constexpr int kRowBytes = kFp8 ? 656 : 2 * DK;
   constexpr uint32_t IDESC_QK = idesc_f16(kPairRows, kKeys, false, false, kBf16);
   constexpr uint32_t IDESC_PV = idesc_f16(kPairRows, 256, false, true, kBf16);
   extern __shared__ uint8_t smem_raw[];
@@ -365,17 +376,29 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     // ------------------------------------------------------------- producers
     const int w = warp;
     const uint32_t k_full0 = cluster_map(mb_k_full, 0), v_full0 = cluster_map(mb_v_full, 0);
-    // K runs one tile ahead of V: K(t+1) is stored before V(t)
+    // Per tile t: store K(t+1), load V(t), store V(t), load K(t+2): K(t+1) is
+    // stored under PV(t-1) and V(t) under QK(t+1), and only one of the two is in
+    // registers at a time. The rows of tile t+3 are found, and fetched into L2,
+    // meanwhile.
     Cursor c = start;               // the tile whose K is stored next
+    Cursor ahead = start;           // the tile whose rows are looked up next
     int kc = 0;                     // K stores so far (two per tile in two-pass segments)
     uint64_t seen = 0;
-    // rows of tile c: lanes 0-3 K keys 4w + lane of this CTA's half, lanes 4-11 V keys 8w + lane - 4
-    auto codes = [&]() {
-      if (c.first || kc == 0) seen = seen_columns(p, c.b, c.r.nd, lane);
+    const int total = start.left;
+    // rows of tile `ahead`: lanes 0-3 K keys 4w + lane of this CTA's half, lanes 4-11 V keys 8w + lane - 4
+    auto look_up = [&]() {
       int code = -1;
-      if (lane < 12)
-        code = row_code(p, c.b, c.r, seen, c.tile * kKeys + (lane < 4 ? 64 * rank + 4 * w + lane : 8 * w + lane - 4));
+      if (ahead.left > 0) {
+        if (ahead.first || ahead.left == total) seen = seen_columns(p, ahead.b, ahead.r.nd, lane);
+        if (lane < 12)
+          code = row_code(p, ahead.b, ahead.r, seen,
+                          ahead.tile * kKeys + (lane < 4 ? 64 * rank + 4 * w + lane : 8 * w + lane - 4));
+        ahead.next(p);
+      }
       return code;
+    };
+    auto fetch = [&](int code) {  // this CTA's keys into L2; the other CTA fetches the rest of V's
+      if (lane < 4 && code >= 0) prefetch_l2(p.kv + (int64_t)code * kRowBytes, kRowBytes);
     };
     auto start_segment = [&]() {
       if (ok) load_q<FMT>(p, sm + SM_Q, qe + 64 * (c.seg & 3), c.b, c.rt * kPairRows + kRows * rank, w, lane);
@@ -383,77 +406,82 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (lane == 0) mbar_arrive(mb_q_full + 8 * (c.seg & 3));
     };
     const int krow = 4 * w + (lane >> 3), vrow = 8 * w + (lane >> 3);
-    const int total = c.left;
     if constexpr (kFp8) {
-      uint4 kd[4], kr, vd[4];  // K: 4 groups and the rotary tail of this lane's key | V: [key][group]
-      float4 ks;
-      float vs[4];
-      auto load_k = [&](int codes_at) {
-        const int code = __shfl_sync(0xffffffffu, codes_at, lane >> 3);
+      // K: the four groups and the rotary tail of this lane's key | V: [key][group].
+      // A lane takes chunk l & 7 of each 64-column block (8 bytes of codes, 16 of
+      // f16), so its shared-memory offset is the same in every block and the eight
+      // lanes of a row cover all banks.
+      uint2 d[8];
+      uint4 tail;
+      float4 sc;
+      auto load_k = [&](int codes) {
+        const int code = __shfl_sync(0xffffffffu, codes, lane >> 3);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kd[j] = make_uint4(0, 0, 0, 0);
-        ks = make_float4(1.f, 1.f, 1.f, 1.f);
-        kr = make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 8; ++j) d[j] = make_uint2(0, 0);
+        sc = make_float4(1.f, 1.f, 1.f, 1.f);
+        tail = make_uint4(0, 0, 0, 0);
         if (code >= 0) {
-          const uint8_t* row = p.kv + (int64_t)code * 656 + 16 * (lane & 7);
+          const uint8_t* row = p.kv + (int64_t)code * kRowBytes;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) kd[j] = ldg_nc16(row + 128 * j);
-          kr = ldg_nc16(row + 528);
-          const uint4 x = ldg_nc16(row + 512 - 16 * (lane & 7));
-          ks = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+          for (int j = 0; j < 8; ++j) d[j] = ldg_nc8(row + 8 * (lane & 7) + 64 * j);
+          tail = ldg_nc16(row + 528 + 16 * (lane & 7));
+          const uint4 x = ldg_nc16(row + 512);
+          sc = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
         }
       };
-      auto load_v = [&](int codes_at) {
+      auto load_v = [&](int codes) {
+        float f[4];
 #pragma unroll
         for (int rs = 0; rs < 2; ++rs) {
-          const int code = __shfl_sync(0xffffffffu, codes_at, 4 + (lane >> 3) + 4 * rs);
+          const int code = __shfl_sync(0xffffffffu, codes, 4 + (lane >> 3) + 4 * rs);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            vd[2 * rs + h] = make_uint4(0, 0, 0, 0);
-            vs[2 * rs + h] = 1.f;
-            if (code >= 0) {
-              const uint8_t* row = p.kv + (int64_t)code * 656;
-              vd[2 * rs + h] = ldg_nc16(row + 16 * ((lane & 7) + 8 * (2 * h + rank)));
-              vs[2 * rs + h] = __ldg(reinterpret_cast<const float*>(row + 512) + 2 * h + rank);
-            }
+          for (int j = 0; j < 4; ++j) d[4 * rs + j] = make_uint2(0, 0);
+          f[2 * rs] = f[2 * rs + 1] = 1.f;
+          if (code >= 0) {
+            const uint8_t* row = p.kv + (int64_t)code * kRowBytes;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // block j & 1 of group 2 (j / 2) + rank
+              d[4 * rs + j] = ldg_nc8(row + 8 * (lane & 7) + 128 * rank + 256 * (j >> 1) + 64 * (j & 1));
+            f[2 * rs] = __ldg(reinterpret_cast<const float*>(row + 512) + rank);
+            f[2 * rs + 1] = __ldg(reinterpret_cast<const float*>(row + 512) + 2 + rank);
           }
         }
+        sc = make_float4(f[0], f[1], f[2], f[3]);
       };
-      // In two-pass tiles the first pass rounds in f32 too: the second takes its remainder.
-      auto put_k = [&](auto how) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t q[8];
-          dequant16<decltype(how)::value>(kd[j], j == 0 ? ks.x : j == 1 ? ks.y : j == 2 ? ks.z : ks.w, q);
-          store_group(sm + SM_K + 2 * j * kBlk, kBlk, krow, lane, q);
-        }
+      auto all_fast = [&]() {
+        return __all_sync(0xffffffffu, fast_scale(sc.x) && fast_scale(sc.y) && fast_scale(sc.z) && fast_scale(sc.w));
       };
-      auto put_v = [&](auto how) {
+      const uint32_t k_at = base + SM_K + sw128_off(krow, lane & 7), v_at = base + SM_V + sw128_off(vrow, lane & 7);
+      auto put = [&](auto how, auto is_k) {
+        constexpr int HOW = decltype(how)::value;
+        const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          uint32_t q[8];
-          dequant16<decltype(how)::value>(vd[x], vs[x], q);
-          store_group(sm + SM_V + 2 * (x & 1) * kVBlk, kVBlk, vrow + 4 * (x >> 1), lane, q);
+          const Scale s(s4[x]);
+          // V: key vrow + 4 (x / 2): half a swizzle atom on, so chunks flip bit 2
+          const uint32_t at = decltype(is_k)::value ? k_at + 2 * x * kBlk
+                                                    : ((v_at + 512 * (x >> 1)) ^ (64 * (x >> 1))) + 2 * (x & 1) * kVBlk;
+          sts16(at, dequant8<HOW>(d[2 * x], s));
+          sts16(at + (decltype(is_k)::value ? kBlk : kVBlk), dequant8<HOW>(d[2 * x + 1], s));
         }
       };
-      // K of tile c: wait for the buffer, store, announce
+      // K of tile c: wait for the buffer, store, announce. In two-pass tiles the
+      // first pass rounds in f32: the second stores its remainder.
       auto store_k = [&]() {
-        if (kc > 0) ok = ok && mbar_wait_cluster(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+        if (kc > 0) ok = ok && mbar_wait(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
         if (c.first) start_segment();
         const int passes = c.r.seq <= kTwoPassKeys ? 2 : 1;
 #pragma unroll 1
         for (int s = 0; s < passes; ++s) {
-          if (s > 0) ok = ok && mbar_wait_cluster(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+          if (s > 0) ok = ok && mbar_wait(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
           if (ok) {
             if (s > 0)
-              put_k(std::integral_constant<int, kRest>());
-            else if (passes == 1 && __all_sync(0xffffffffu, fast_scale(ks.x) && fast_scale(ks.y) && fast_scale(ks.z) &&
-                                                                fast_scale(ks.w)))
-              put_k(std::integral_constant<int, kFast>());
+              put(std::integral_constant<int, kRest>(), std::true_type());
+            else if (passes == 1 && all_fast())
+              put(std::integral_constant<int, kFast>(), std::true_type());
             else
-              put_k(std::integral_constant<int, kWide>());
-            *reinterpret_cast<uint4*>(sm + SM_K + 8 * kBlk + sw128_off(krow, lane & 7)) =
-                s > 0 ? make_uint4(0, 0, 0, 0) : kr;
+              put(std::integral_constant<int, kWide>(), std::true_type());
+            sts16(k_at + 8 * kBlk, s > 0 ? make_uint4(0, 0, 0, 0) : tail);
           }
           fence_proxy_async();
           __syncwarp();
@@ -462,42 +490,38 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         }
         c.next(p);
       };
-      int code0 = -1, code1 = -1;  // rows of the tile of the next V load, and of the tile after it
+      int code0 = look_up(), code1 = look_up(), code2 = look_up();  // tiles t, t+1, t+2
+      fetch(code1);
+      fetch(code2);
       if (total > 0) {
-        code0 = codes();
         load_k(code0);
-        load_v(code0);
         store_k();
-        if (c.left > 0) {
-          code0 = codes();
-          load_k(code0);
-        }
+        load_k(code1);
       }
+#pragma unroll 1
       for (int t = 0; t < total; ++t) {
-        if (t + 1 < total) {
-          store_k();
-          if (c.left > 0) {
-            code1 = codes();
-            load_k(code1);
-          }
-        }
-        if (t > 0) ok = ok && mbar_wait_cluster(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
+        if (t + 1 < total) store_k();
+        load_v(code0);
+        if (t > 0) ok = ok && mbar_wait(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
         if (ok) {
-          if (__all_sync(0xffffffffu, fast_scale(vs[0]) && fast_scale(vs[1]) && fast_scale(vs[2]) && fast_scale(vs[3])))
-            put_v(std::integral_constant<int, kFast>());
+          if (all_fast())
+            put(std::integral_constant<int, kFast>(), std::false_type());
           else
-            put_v(std::integral_constant<int, kWide>());
+            put(std::integral_constant<int, kWide>(), std::false_type());
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(v_full0);
-        if (t + 1 < total) load_v(code0);
+        load_k(code2);
         code0 = code1;
+        code1 = code2;
+        code2 = look_up();
+        fetch(code2);
       }
     } else {
       auto store_k = [&](int codes_at) {
         const int code = __shfl_sync(0xffffffffu, codes_at, lane >> 3);
-        if (kc > 0) ok = ok && mbar_wait_cluster(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+        if (kc > 0) ok = ok && mbar_wait(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
         if (ok) {
           const uint8_t* row = p.kv + (int64_t)max(code, 0) * (DK * 2) + 16 * (lane & 7);
 #pragma unroll
@@ -513,17 +537,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         ++kc;
         c.next(p);
       };
-      int code0 = -1, code1 = -1;
-      if (total > 0) {
-        code0 = codes();
-        store_k(code0);
-      }
+      int code0 = look_up(), code1 = look_up(), code2 = look_up();  // tiles t, t+1, t+2
+      fetch(code1);
+      fetch(code2);
+      if (total > 0) store_k(code0);
+#pragma unroll 1
       for (int t = 0; t < total; ++t) {
-        if (t + 1 < total) {
-          code1 = codes();
-          store_k(code1);
-        }
-        if (t > 0) ok = ok && mbar_wait_cluster(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
+        if (t + 1 < total) store_k(code1);
+        if (t > 0) ok = ok && mbar_wait(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
 #pragma unroll
         for (int rs = 0; rs < 2; ++rs) {
           const int code = __shfl_sync(0xffffffffu, code0, 4 + (lane >> 3) + 4 * rs);
@@ -541,6 +562,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(v_full0);
         code0 = code1;
+        code1 = code2;
+        code2 = look_up();
+        fetch(code2);
       }
     }
   } else if (warp == kMmaWarp) {
@@ -556,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       auto qk = [&]() {
         const int passes = kFp8 && cq.r.seq <= kTwoPassKeys ? 2 : 1;
         for (int s = 0; s < passes; ++s) {
-          ok = ok && mbar_wait_cluster(mb_k_full, kc & 1, abort_flag, err, kWaitNs);
+          ok = ok && mbar_wait(mb_k_full, kc & 1, abort_flag, err, kWaitNs);
           if (ok) {
             fence_after_sync();
             const uint64_t dq = desc(SM_Q, 16), dk = desc(SM_K, 16);
@@ -577,10 +601,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (cq.left > 0) qk();
       while (cp.left > 0 && ok) {
         if (cq.left > 0) qk();
-        ok = ok && mbar_wait_cluster(mb_v_full, gp & 1, abort_flag, err, kWaitNs) &&
-             mbar_wait_cluster(mb_p_full, gp & 1, abort_flag, err, kWaitNs);
+        ok = ok && mbar_wait(mb_v_full, gp & 1, abort_flag, err, kWaitNs) &&
+             mbar_wait(mb_p_full, gp & 1, abort_flag, err, kWaitNs);
         // the accumulator of the segment before has been read
-        if (cp.first && cp.seg > 0) ok = ok && mbar_wait_cluster(mb_o_free, (cp.seg - 1) & 1, abort_flag, err, kWaitNs);
+        if (cp.first && cp.seg > 0) ok = ok && mbar_wait(mb_o_free, (cp.seg - 1) & 1, abort_flag, err, kWaitNs);
         if (ok) {
           fence_after_sync();
           const uint64_t dp = desc(SM_P, 16), dv = desc(SM_V, kVBlk);
@@ -619,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         const int r = c.rt * kPairRows + kRows * rank + row;
         const int i = r / p.H;
         const bool on = i < c.r.nd;
-        rs = p.scale_log2 * __int_as_float((127 + (int)qe[64 * (c.seg & 3) + row]) << 23);
+        // not 0, so that a hidden key's -inf stays one
+        rs = fmaxf(p.scale_log2 * __int_as_float((127 + (int)qe[64 * (c.seg & 3) + row]) << 23), FLT_MIN);
         pre = on ? c.r.seq - c.r.nd : kNoRow;
         full = c.tile == 0 && c.left >= c.r.nt;
         m = kNoMax;
@@ -634,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (c.r.nd < 64) bits &= (1ull << c.r.nd) - 1;
         allow |= (uint32_t)(d >= 0 ? bits << d : bits >> -d);
       }
-      ok = ok && mbar_wait_cluster(mb_s_full + 8 * (g & 1), (g >> 1) & 1, abort_flag, err, kWaitNs);
+      ok = ok && mbar_wait(mb_s_full + 8 * (g & 1), (g >> 1) & 1, abort_flag, err, kWaitNs);
       ok = __all_sync(0xffffffffu, ok);
       fence_after_sync();
       uint32_t s[32];
@@ -645,22 +670,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll
         for (int j = 0; j < 32; ++j) s[j] = 0u;
       }
-      float mx = -INFINITY;
-      if (allow == 0xffffffffu) {
+      if (allow != 0xffffffffu) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float z = __uint_as_float(s[j]) * rs;
-          s[j] = __float_as_uint(z);
-          mx = fmaxf(mx, z);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float z = (allow >> j) & 1 ? __uint_as_float(s[j]) * rs : -INFINITY;
-          s[j] = __float_as_uint(z);
-          mx = fmaxf(mx, z);
-        }
+        for (int j = 0; j < 32; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;  // -inf
       }
+      float mx = __uint_as_float(s[0]);
+#pragma unroll
+      for (int j = 1; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(s[j]));
+      mx *= rs;  // rs >= 0
       float alpha = 1.f;
       const bool any = named_bar_or(1, kSoftmaxWarps * 32, mx > m + kRescale);
       if (any) {
@@ -676,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       uint32_t pk[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float a = ex2(__uint_as_float(s[2 * j]) - m), b = ex2(__uint_as_float(s[2 * j + 1]) - m);
+        const float a = ex2(fmaf(__uint_as_float(s[2 * j]), rs, -m)), b = ex2(fmaf(__uint_as_float(s[2 * j + 1]), rs, -m));
         L += a + b;
         if (kBf16) {
           const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -685,10 +702,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           pk[j] = pack_half2(a, b);
         }
       }
-      if (!first) {  // P's buffer and O are free once PV(t-1) has completed (the epilogue waited for the last one)
-        ok = ok && mbar_wait_cluster(mb_v_free, (g - 1) & 1, abort_flag, err, kWaitNs);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && __any_sync(0xffffffffu, alpha != 1.f)) {
+      // P's buffer and O are free once PV(t-1) has completed (the epilogue waited for a segment's last)
+      if (!first) ok = ok && mbar_wait(mb_v_free, (g - 1) & 1, abort_flag, err, kWaitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) =
+              make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
+        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
           fence_after_sync();
 #pragma unroll 1
           for (int k = 0; k < 4; ++k) {
@@ -703,12 +725,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           tmem_wait_st();
         }
       }
-      if (ok) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) =
-              make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
-      }
       fence_proxy_async();
       fence_before_sync();
       __syncwarp();
@@ -721,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         named_bar(1, kSoftmaxWarps * 32);
         L = (rowx[row] + rowx[64 + row]) + (rowx[128 + row] + rowx[192 + row]);
         named_bar(1, kSoftmaxWarps * 32);
-        ok = ok && mbar_wait_cluster(mb_v_free, g & 1, abort_flag, err, kWaitNs);
+        ok = ok && mbar_wait(mb_v_free, g & 1, abort_flag, err, kWaitNs);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           fence_after_sync();
@@ -948,6 +964,7 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
                   bt_stride >= max_blocks && mask_stride >= T,
               DSA_ERR_INVALID, "tree_mla_decode: bad cache geometry or strides (page=%d max_blocks=%d rows=%lld)",
               page_size, max_blocks, (long long)n_kv_rows);
+  DSA_REQUIRE(std::isfinite(scale), DSA_ERR_INVALID, "tree_mla_decode: scale must be finite");
   if (B == 0 || T == 0 || n_head == 0) return DSA_OK;
   DSA_REQUIRE(n_head <= 1024 && B <= 65535, DSA_ERR_UNSUPPORTED, "tree_mla_decode: at most 65535 requests of 1024 heads");
   DSA_REQUIRE(o && lse && q && seq_lens && tree_mask && (n_kv_rows == 0 || kv_cache) && (max_blocks == 0 || block_table),
@@ -972,6 +989,9 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
   p.bt_stride = bt_stride;
   p.mask_stride = mask_stride;
   p.page = page_size;
+  p.page_shift = -1;
+  for (int k = 0; k < 31; ++k)
+    if (page_size == 1 << k) p.page_shift = k;
   p.max_blocks = max_blocks;
   p.B = B;
   p.T = T;
@@ -980,7 +1000,8 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
   p.slot_rows = (int)std::min<int64_t>(kPairRows, (int64_t)T * n_head);
   p.q_bf16 = q_dtype == DSA_BF16;
   p.o_bf16 = o_dtype == DSA_BF16;
-  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.q_sign = scale < 0 ? 0x80008000u : 0u;
+  p.scale_log2 = (float)(std::fabs(scale) * 1.4426950408889634);
   const size_t need = tree_workspace(T, n_head, p.pairs);
   DSA_REQUIRE(workspace != nullptr && workspace_bytes >= need, DSA_ERR_WORKSPACE,
               "tree_mla_decode: workspace needs %zu bytes, got %zu", need, workspace_bytes);

@@ -157,6 +157,13 @@ def test_tree_bf16_q_outside_fp16_range(dsa, oracle, mul):
     run_tree(dsa, oracle, "fp8", BF, BF, 3, 8, [700, 60], None, seed=6, q_mul=mul, scale=SCALE / mul)
 
 
+@pytest.mark.parametrize("scale", [0.0, -SCALE, 1e-30])
+def test_tree_other_scales(dsa, oracle, scale):
+    """A scale of zero weighs all seen positions alike; a negative one turns the scores."""
+    run_tree(dsa, oracle, "fp8", BF, BF, 3, 8, [300, 3, 700], [3, 2, 1], seed=8, scale=scale)
+    run_tree(dsa, oracle, "bf16", BF, BF, 3, 8, [300, 3], None, seed=8, scale=scale)
+
+
 def test_tree_rows_of_very_different_magnitude(dsa, oracle):
     """Each row of q has its own exponent range."""
     bt, pages = tables([300], 64, 1)
