@@ -309,6 +309,25 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mbar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
+// mbar_wait that reads the clock only once a wait has become long: the first
+// test of globaltimer costs about a microsecond, more than most waits here.
+__device__ __forceinline__ bool mbar_wait_lazy(uint32_t mbar, uint32_t parity, volatile int* abort, int32_t* err,
+                                               uint64_t timeout_ns) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(mbar, parity)) return true;
+    if ((it & 63u) == 0) {
+      if (*abort) return false;
+      const uint64_t t = globaltimer_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > timeout_ns) {
+        *abort = 1;
+        if (err) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
 // Named barrier that also ORs a predicate over its threads.
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool pred) {
   uint32_t r;

@@ -63,7 +63,8 @@ constexpr int kKeys = 128;      // keys of a tile
 constexpr int DK = 576, DV = 512;
 constexpr int kProducers = 16;
 constexpr int kSoftmax0 = 16, kSoftmaxWarps = 8;
-constexpr int kMmaWarp = 24;
+constexpr int kMmaWarp = 24, kRowWarp = 25, kFetch0 = 26, kFetchWarps = 2;
+constexpr int kRing = 3;        // tiles whose cache rows are known ahead
 constexpr int kThreads = 28 * 32;
 constexpr uint32_t kBlk = 64 * 128;    // 64 rows x 64 16-bit values: 8 KB
 constexpr uint32_t kVBlk = 128 * 128;  // 128 keys x 64 columns: 16 KB
@@ -72,20 +73,20 @@ constexpr uint32_t SM_K = SM_Q + 9 * kBlk;
 constexpr uint32_t SM_V = SM_K + 9 * kBlk;
 constexpr uint32_t SM_P = SM_V + 4 * kVBlk;
 constexpr uint32_t SM_MISC = SM_P + 2 * kBlk;
-constexpr uint32_t kMiscBytes = 2048;
-constexpr uint32_t SMEM_BYTES = SM_MISC + kMiscBytes + 1024;  // + alignment slack
+constexpr int kSegs = 6;        // segment descriptors kept: the row warp is at most five tiles ahead of an epilogue
+constexpr int kQeSegs = 3;      // Q is at most two segments ahead of the softmax
+// the misc block: 18 mbarriers | TMEM base, abort flag, tiles of the run | qe | row maxima / sums | rows ahead | segments
+constexpr uint32_t kQeAt = 160, kRowxAt = kQeAt + kQeSegs * 64, kRingAt = kRowxAt + 4 * 64 * 4,
+                   kSegAt = kRingAt + kRing * kKeys * 4;
 constexpr uint32_t S_COL = 256;        // S buffer x at [256 + 64x, +64); O half h at [128h, +128)
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kNoMax = -1e30f;
-constexpr int kNoRow = (int)0x80000000;
 constexpr int kMaxSeq = 0x7fffff00;   // tile ends stay in 32 bits
 constexpr float kRescale = 8.0f;       // log2 units
 constexpr int kTwoPassKeys = 512;      // fp8: the remainder of the rounding is multiplied up to here
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kSlotF = DV + 2;         // f32 of a row's partial state: o, then m and l
-
-static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 
 struct TreeArgs {
   const void* q;
@@ -132,13 +133,24 @@ __device__ __forceinline__ long long warp_work(const TreeArgs& p, int n, int lan
 
 __device__ __forceinline__ long long chunk_of(long long work, int pairs) { return (work + pairs - 1) / pairs; }
 
+// A run of key tiles of one row tile, as the row warp hands it to the others.
+struct Segment {
+  int b, rt;
+  int n;      // key tiles
+  int pre;    // context positions less those before the first tile
+  int nd;     // drafts of the request
+  int flags;  // kTwo: two-pass products | kFull: every key tile of the row tile
+};
+enum { kTwo = 1, kFull = 2 };
+constexpr uint32_t SMEM_BYTES = SM_MISC + kSegAt + kSegs * (uint32_t)sizeof(Segment);
+static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+
 // One pair's walk over its run of tiles.
 struct Cursor {
   int left;        // tiles left, this one included
-  int b, rt, tile, seg;
+  int b, rt, tile;
   bool first;      // first tile of a segment
   Req r;
-  __device__ __forceinline__ bool last() const { return tile + 1 == r.nt || left == 1; }
   __device__ __forceinline__ void next(const TreeArgs& p) {
     first = false;
     ++tile;
@@ -146,7 +158,6 @@ struct Cursor {
     if (tile == r.nt) {
       tile = 0;
       first = true;
-      ++seg;
       if (++rt == r.nrt) {
         rt = 0;
         do r = load_req(p, ++b);
@@ -156,10 +167,69 @@ struct Cursor {
   }
 };
 
+// The start of a pair's run, by one warp.
+__device__ __forceinline__ Cursor find_run(const TreeArgs& p, int pair, int lane) {
+  const long long work = warp_work(p, p.B, lane);
+  const long long chunk = chunk_of(work, p.pairs);
+  const long long w0 = chunk * pair;
+  Cursor c{};
+  c.left = (int)max(min(chunk, work - w0), 0ll);
+  c.first = true;
+  if (c.left == 0) return c;
+  long long before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    Req r{0, 0, 0, 0};
+    if (b0 + lane < p.B) r = load_req(p, b0 + lane);
+    const long long mine = (long long)r.nt * r.nrt;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w0);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      c.b = b0 + src;
+      c.r = load_req(p, c.b);
+      const long long at = w0 - (before + __shfl_sync(0xffffffffu, incl - mine, src));
+      c.rt = (int)(at / c.r.nt);
+      c.tile = (int)(at % c.r.nt);
+      return c;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two f32 lanes per instruction, and a maximum of three (sm_100).
+__device__ __forceinline__ uint64_t pack64(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack64(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // How codes are expanded to f16: the product code * scale rounded once, by f16
@@ -212,12 +282,6 @@ __device__ __forceinline__ uint4 dequant8(uint2 v, const Scale& sc) {
   return make_uint4(q[0], q[1], q[2], q[3]);
 }
 
-__device__ __forceinline__ uint2 ldg_nc8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
 __device__ __forceinline__ void sts16(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -235,14 +299,26 @@ __device__ __forceinline__ uint64_t seen_columns(const TreeArgs& p, int b, int n
   return ((uint64_t)hi << 32) | lo;
 }
 
-// Cache row of position pos, or -1 (reads as zeros).
-__device__ __forceinline__ int row_code(const TreeArgs& p, int b, const Req& r, uint64_t seen, int pos) {
-  const int j = pos - (r.seq - r.nd);
-  if (pos >= r.seq || (j >= 0 && !((seen >> j) & 1))) return -1;
-  const int blk = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page;
-  if (blk >= p.max_blocks) return -1;
-  const int64_t row = (int64_t)p.bt[(int64_t)b * p.bt_stride + blk] * p.page + (pos - blk * p.page);
-  return row >= 0 && row < p.n_kv_rows ? (int)row : -1;
+// Cache rows of positions pos0 + 32k + lane, k < 4, or -1 (reads as zeros); the
+// four block-table loads are in flight together.
+__device__ __forceinline__ void row_codes(const TreeArgs& p, int b, const Req& r, uint64_t seen, int pos0, int lane,
+                                          int (&code)[4]) {
+  const int32_t* bt = p.bt + (int64_t)b * p.bt_stride;
+  int blk[4], page_row[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int pos = pos0 + 32 * k + lane;
+    blk[k] = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page;
+    page_row[k] = p.max_blocks > 0 ? __ldg(bt + min(blk[k], p.max_blocks - 1)) : -1;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int pos = pos0 + 32 * k + lane;
+    const int j = pos - (r.seq - r.nd);
+    const int64_t row = (int64_t)page_row[k] * p.page + (pos - blk[k] * p.page);
+    const bool on = pos < r.seq && (j < 0 || ((seen >> j) & 1)) && blk[k] < p.max_blocks && row >= 0 && row < p.n_kv_rows;
+    code[k] = on ? (int)row : -1;
+  }
 }
 
 // This CTA's 64 query rows into shared memory (f16, or bf16 as it is): warp w
@@ -284,27 +360,30 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   constexpr int kRowBytes = kFp8 ? 656 : 2 * DK;
   constexpr uint32_t IDESC_QK = idesc_f16(kPairRows, kKeys, false, false, kBf16);
   constexpr uint32_t IDESC_PV = idesc_f16(kPairRows, 256, false, true, kBf16);
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_base = smem_u32(smem_raw);
-  const uint32_t base = (raw_base + 1023u) & ~1023u;
-  uint8_t* sm = smem_raw + (base - raw_base);
+  extern __shared__ __align__(1024) uint8_t sm[];  // 1024: the swizzle atoms' alignment
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023u) {  // never, with no static shared memory in this kernel
+    if (threadIdx.x == 0) atomicExch(err, (int32_t)DSA_ERR_CUDA);
+    return;
+  }
   uint8_t* misc = sm + SM_MISC;
-  // misc: [0, 104) 13 mbarriers | 104 TMEM base | 108 abort | [112, 144) the
-  // pair's run | [192, 448) qe[4][64] | [448, 1472) rowx[4][64]
   const uint32_t mb = smem_u32(misc);
   const uint32_t mb_k_full = mb, mb_k_free = mb + 8, mb_v_full = mb + 16, mb_v_free = mb + 24, mb_p_full = mb + 32,
-                 mb_o_free = mb + 40, mb_done = mb + 48, mb_s_full = mb + 56 /* [2] */, mb_q_full = mb + 72 /* [4] */;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 104);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 108);
-  int* run_left = reinterpret_cast<int*>(misc + 112);
-  int* run_at = reinterpret_cast<int*>(misc + 116);  // b, rt, tile
-  int8_t* qe = reinterpret_cast<int8_t*>(misc + 192);
-  float* rowx = reinterpret_cast<float*>(misc + 448);
+                 mb_o_free = mb + 40, mb_done = mb + 48, mb_s_full = mb + 56 /* [2] */, mb_q_full = mb + 72 /* [3] */,
+                 mb_r_full = mb + 96 /* [3] */, mb_r_free = mb + 120 /* [3] */;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 144);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 148);
+  int* run_tiles = reinterpret_cast<int*>(misc + 152);
+  int8_t* qe = reinterpret_cast<int8_t*>(misc + kQeAt);         // [kQeSegs][64]
+  float* rowx = reinterpret_cast<float*>(misc + kRowxAt);       // [4][64]
+  int* ring = reinterpret_cast<int*>(misc + kRingAt);           // [kRing][128]
+  Segment* segs = reinterpret_cast<Segment*>(misc + kSegAt);    // [kSegs]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int pair = blockIdx.x >> 1;
 
+  Cursor c{};  // the row warp's
   if (warp == 0) {
     if (lane == 0) {
       mbar_init(mb_k_full, 2 * kProducers);
@@ -315,196 +394,176 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       mbar_init(mb_o_free, 2 * kSoftmaxWarps);
       mbar_init(mb_done, 1);
       for (int x = 0; x < 2; ++x) mbar_init(mb_s_full + 8 * x, 1);
-      for (int x = 0; x < 4; ++x) mbar_init(mb_q_full + 8 * x, kProducers);
+      for (int x = 0; x < kQeSegs; ++x) mbar_init(mb_q_full + 8 * x, kProducers);
+      for (int x = 0; x < kRing; ++x) {
+        mbar_init(mb_r_full + 8 * x, 1);
+        mbar_init(mb_r_free + 8 * x, kProducers + (kFp8 ? 0 : kFetchWarps));
+      }
       mbar_init_fence();
       *abort_flag = 0;
     }
     __syncwarp();
     tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
-  } else if (warp == 1) {
-    // this pair's run of the list of tiles
-    const long long work = warp_work(p, p.B, lane);
-    const long long chunk = chunk_of(work, p.pairs);
-    const long long w0 = chunk * pair;
-    const long long left = max(min(chunk, work - w0), 0ll);
-    if (left > 0) {
-      long long before = 0;
-      for (int b0 = 0;; b0 += 32) {
-        Req r{0, 0, 0, 0};
-        if (b0 + lane < p.B) r = load_req(p, b0 + lane);
-        const long long mine = (long long)r.nt * r.nrt;
-        long long incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w0);
-        if (hit) {
-          if (lane == __ffs(hit) - 1) {
-            const long long at = w0 - (before + incl - mine);
-            run_at[0] = b0 + lane;
-            run_at[1] = (int)(at / r.nt);
-            run_at[2] = (int)(at % r.nt);
-          }
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31);
-      }
-    }
-    if (lane == 0) *run_left = (int)left;
+  } else if (warp == kRowWarp) {
+    c = find_run(p, pair, lane);
+    if (lane == 0) *run_tiles = c.left;
   }
   fence_before_sync();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist and TMEM is allocated
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  Cursor start;
-  start.left = *run_left;
-  start.b = run_at[0];
-  start.rt = run_at[1];
-  start.tile = run_at[2];
-  start.seg = 0;
-  start.first = true;
-  start.r = Req{0, 0, 0, 0};
-  if (start.left > 0) start.r = load_req(p, start.b);
+  const int total = *run_tiles;
 
   bool ok = true;
+  // By a whole warp: `ok` stays uniform.
+  auto wait = [&](uint32_t mbar, uint32_t parity) {
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_lazy(mbar, parity, abort_flag, err, kWaitNs));
+  };
   // After a wait that ran out (`ok` false, abort flag set) every thread still
   // executes its role's barriers and arrivals, and later waits return at once.
   if (warp < kProducers) {
     // ------------------------------------------------------------- producers
     const int w = warp;
     const uint32_t k_full0 = cluster_map(mb_k_full, 0), v_full0 = cluster_map(mb_v_full, 0);
-    // Per tile t: store K(t+1), load V(t), store V(t), load K(t+2): K(t+1) is
-    // stored under PV(t-1) and V(t) under QK(t+1), and only one of the two is in
-    // registers at a time. The rows of tile t+3 are found, and fetched into L2,
-    // meanwhile.
-    Cursor c = start;               // the tile whose K is stored next
-    Cursor ahead = start;           // the tile whose rows are looked up next
-    int kc = 0;                     // K stores so far (two per tile in two-pass segments)
-    uint64_t seen = 0;
-    const int total = start.left;
-    // rows of tile `ahead`: lanes 0-3 K keys 4w + lane of this CTA's half, lanes 4-11 V keys 8w + lane - 4
-    auto look_up = [&]() {
-      int code = -1;
-      if (ahead.left > 0) {
-        if (ahead.first || ahead.left == total) seen = seen_columns(p, ahead.b, ahead.r.nd, lane);
-        if (lane < 12)
-          code = row_code(p, ahead.b, ahead.r, seen,
-                          ahead.tile * kKeys + (lane < 4 ? 64 * rank + 4 * w + lane : 8 * w + lane - 4));
-        ahead.next(p);
-      }
-      return code;
+    // Per tile t: store K(t+1) and load K(t+2), store V(t) and load V(t+1): K(t+1)
+    // is stored under PV(t-1) and V(t) under QK(t+1), and a load has most of a
+    // tile's time to arrive.
+    int kc = 0;             // K stores so far (two per tile in two-pass segments)
+    int seg = 0, left = 0;  // the segment of the next K store, and its tiles left
+    bool two = false;
+    // Lane (l & 15) of a half warp takes the 16 bytes of codes at 16 cx of a
+    // 128-wide group, of the first row for l & 4 = 0, else of the second: the eight
+    // lanes of a store hold even chunks of an even and an odd row, which the swizzle
+    // puts on different banks.
+    const int cx = (lane & 3) + 4 * ((lane >> 3) & 1);
+    const int lrow = 2 * (lane >> 4) + ((lane >> 2) & 1);
+    const int krow = 4 * w + lrow, vrow = 8 * w + lrow;
+    // rows of tile t: the ring is filled by the row warp
+    auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
+    auto wait_rows = [&](int t) {
+      wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
     };
-    auto fetch = [&](int code) {  // this CTA's keys into L2; the other CTA fetches the rest of V's
-      if (lane < 4 && code >= 0) prefetch_l2(p.kv + (int64_t)code * kRowBytes, kRowBytes);
-    };
-    auto start_segment = [&]() {
-      if (ok) load_q<FMT>(p, sm + SM_Q, qe + 64 * (c.seg & 3), c.b, c.rt * kPairRows + kRows * rank, w, lane);
+    auto free_rows = [&](int t) {
       __syncwarp();
-      if (lane == 0) mbar_arrive(mb_q_full + 8 * (c.seg & 3));
+      if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
     };
-    const int krow = 4 * w + (lane >> 3), vrow = 8 * w + (lane >> 3);
+    // before a K store: the next segment's Q, when its first tile is due
+    auto enter = [&]() {
+      if (left > 0) return;
+      const Segment& sg = segs[seg % kSegs];  // visible: the wait for this tile's rows
+      left = sg.n;
+      two = (sg.flags & kTwo) != 0;
+      if (ok) load_q<FMT>(p, sm + SM_Q, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb_q_full + 8 * (seg % kQeSegs));
+      ++seg;
+    };
     if constexpr (kFp8) {
-      // K: the four groups and the rotary tail of this lane's key | V: [key][group].
-      // A lane takes chunk l & 7 of each 64-column block (8 bytes of codes, 16 of
-      // f16), so its shared-memory offset is the same in every block and the eight
-      // lanes of a row cover all banks.
-      uint2 d[8];
-      uint4 tail;
-      float4 sc;
-      auto load_k = [&](int codes) {
-        const int code = __shfl_sync(0xffffffffu, codes, lane >> 3);
+      uint4 kd[4], tail, vd[4];  // K: the four groups and the rotary tail of this lane's key | V: [key][group]
+      float4 ks, vs;             // their scales
+      auto load_k = [&](int t) {
+        wait_rows(t);
+        const int code = ok ? rows_of(t)[64 * rank + krow] : -1;
+        const uint8_t* row = p.kv + (int64_t)code * kRowBytes;
+        auto get = [&]() {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = make_uint2(0, 0);
-        sc = make_float4(1.f, 1.f, 1.f, 1.f);
-        tail = make_uint4(0, 0, 0, 0);
-        if (code >= 0) {
-          const uint8_t* row = p.kv + (int64_t)code * kRowBytes;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] = ldg_nc8(row + 8 * (lane & 7) + 64 * j);
-          tail = ldg_nc16(row + 528 + 16 * (lane & 7));
+          for (int j = 0; j < 4; ++j) kd[j] = ldg_nc16(row + 16 * cx + 128 * j);
+          tail = ldg_nc16(row + 528 + 16 * cx);
           const uint4 x = ldg_nc16(row + 512);
-          sc = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+          ks = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+        };
+        if (__all_sync(0xffffffffu, code >= 0)) {
+          get();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kd[j] = make_uint4(0, 0, 0, 0);
+          ks = make_float4(1.f, 1.f, 1.f, 1.f);
+          tail = make_uint4(0, 0, 0, 0);
+          if (code >= 0) get();
         }
       };
-      auto load_v = [&](int codes) {
-        float f[4];
+      auto load_v = [&](int t) {
+        int code[2];
+        code[0] = ok ? rows_of(t)[vrow] : -1;
+        code[1] = ok ? rows_of(t)[vrow + 4] : -1;
+        free_rows(t);
+        auto get = [&](int x) {
+          const uint8_t* row = p.kv + (int64_t)code[x] * kRowBytes;
+          vd[2 * x] = ldg_nc16(row + 16 * cx + 128 * rank);
+          vd[2 * x + 1] = ldg_nc16(row + 16 * cx + 128 * rank + 256);
+          (x ? vs.z : vs.x) = __ldg(reinterpret_cast<const float*>(row + 512) + rank);
+          (x ? vs.w : vs.y) = __ldg(reinterpret_cast<const float*>(row + 512) + rank + 2);
+        };
+        if (__all_sync(0xffffffffu, code[0] >= 0 && code[1] >= 0)) {
+          get(0);
+          get(1);
+        } else {
 #pragma unroll
-        for (int rs = 0; rs < 2; ++rs) {
-          const int code = __shfl_sync(0xffffffffu, codes, 4 + (lane >> 3) + 4 * rs);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) d[4 * rs + j] = make_uint2(0, 0);
-          f[2 * rs] = f[2 * rs + 1] = 1.f;
-          if (code >= 0) {
-            const uint8_t* row = p.kv + (int64_t)code * kRowBytes;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)  // block j & 1 of group 2 (j / 2) + rank
-              d[4 * rs + j] = ldg_nc8(row + 8 * (lane & 7) + 128 * rank + 256 * (j >> 1) + 64 * (j & 1));
-            f[2 * rs] = __ldg(reinterpret_cast<const float*>(row + 512) + rank);
-            f[2 * rs + 1] = __ldg(reinterpret_cast<const float*>(row + 512) + 2 + rank);
-          }
+          for (int j = 0; j < 4; ++j) vd[j] = make_uint4(0, 0, 0, 0);
+          vs = make_float4(1.f, 1.f, 1.f, 1.f);
+          if (code[0] >= 0) get(0);
+          if (code[1] >= 0) get(1);
         }
-        sc = make_float4(f[0], f[1], f[2], f[3]);
       };
-      auto all_fast = [&]() {
-        return __all_sync(0xffffffffu, fast_scale(sc.x) && fast_scale(sc.y) && fast_scale(sc.z) && fast_scale(sc.w));
+      auto all_fast = [](const float4& f) {
+        return __all_sync(0xffffffffu, fast_scale(f.x) && fast_scale(f.y) && fast_scale(f.z) && fast_scale(f.w));
       };
-      const uint32_t k_at = base + SM_K + sw128_off(krow, lane & 7), v_at = base + SM_V + sw128_off(vrow, lane & 7);
+      const uint32_t k_at = base + SM_K + (cx >> 2) * kBlk + sw128_off(krow, 2 * (cx & 3));
+      const uint32_t v_at = base + SM_V + (cx >> 2) * kVBlk + sw128_off(vrow, 2 * (cx & 3));
       auto put = [&](auto how, auto is_k) {
         constexpr int HOW = decltype(how)::value;
-        const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
+        constexpr bool K = decltype(is_k)::value;
+        const float4 f = K ? ks : vs;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const Scale s(s4[x]);
+          const Scale s(x == 0 ? f.x : x == 1 ? f.y : x == 2 ? f.z : f.w);
+          const uint4 d = K ? kd[x] : vd[x];
           // V: key vrow + 4 (x / 2): half a swizzle atom on, so chunks flip bit 2
-          const uint32_t at = decltype(is_k)::value ? k_at + 2 * x * kBlk
-                                                    : ((v_at + 512 * (x >> 1)) ^ (64 * (x >> 1))) + 2 * (x & 1) * kVBlk;
-          sts16(at, dequant8<HOW>(d[2 * x], s));
-          sts16(at + (decltype(is_k)::value ? kBlk : kVBlk), dequant8<HOW>(d[2 * x + 1], s));
+          const uint32_t at =
+              K ? k_at + 2 * x * kBlk : ((v_at + 512 * (x >> 1)) ^ (64 * (x >> 1))) + 2 * (x & 1) * kVBlk;
+          sts16(at, dequant8<HOW>(make_uint2(d.x, d.y), s));
+          sts16(at ^ 16, dequant8<HOW>(make_uint2(d.z, d.w), s));
         }
       };
       // K of tile c: wait for the buffer, store, announce. In two-pass tiles the
       // first pass rounds in f32: the second stores its remainder.
       auto store_k = [&]() {
-        if (kc > 0) ok = ok && mbar_wait(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
-        if (c.first) start_segment();
-        const int passes = c.r.seq <= kTwoPassKeys ? 2 : 1;
+        if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
+        enter();
+        const int passes = two ? 2 : 1;
 #pragma unroll 1
         for (int s = 0; s < passes; ++s) {
-          if (s > 0) ok = ok && mbar_wait(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+          if (s > 0) wait(mb_k_free, (kc - 1) & 1);
           if (ok) {
             if (s > 0)
               put(std::integral_constant<int, kRest>(), std::true_type());
-            else if (passes == 1 && all_fast())
+            else if (passes == 1 && all_fast(ks))
               put(std::integral_constant<int, kFast>(), std::true_type());
             else
               put(std::integral_constant<int, kWide>(), std::true_type());
-            sts16(k_at + 8 * kBlk, s > 0 ? make_uint4(0, 0, 0, 0) : tail);
+            sts16(base + SM_K + 8 * kBlk + sw128_off(krow, cx), s > 0 ? make_uint4(0, 0, 0, 0) : tail);
           }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(k_full0);
           ++kc;
         }
-        c.next(p);
+        --left;
       };
-      int code0 = look_up(), code1 = look_up(), code2 = look_up();  // tiles t, t+1, t+2
-      fetch(code1);
-      fetch(code2);
       if (total > 0) {
-        load_k(code0);
+        load_k(0);
+        load_v(0);
         store_k();
-        load_k(code1);
+        if (total > 1) load_k(1);
       }
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
         if (t + 1 < total) store_k();
-        load_v(code0);
-        if (t > 0) ok = ok && mbar_wait(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
+        if (t + 2 < total) load_k(t + 2);
+        if (t > 0) wait(mb_v_free, (t - 1) & 1);
         if (ok) {
-          if (all_fast())
+          if (all_fast(vs))
             put(std::integral_constant<int, kFast>(), std::false_type());
           else
             put(std::integral_constant<int, kWide>(), std::false_type());
@@ -512,48 +571,46 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(v_full0);
-        load_k(code2);
-        code0 = code1;
-        code1 = code2;
-        code2 = look_up();
-        fetch(code2);
+        if (t + 1 < total) load_v(t + 1);
       }
     } else {
-      auto store_k = [&](int codes_at) {
-        const int code = __shfl_sync(0xffffffffu, codes_at, lane >> 3);
-        if (kc > 0) ok = ok && mbar_wait(mb_k_free, (kc - 1) & 1, abort_flag, err, kWaitNs);
+      const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
+      auto store_k = [&](int t) {
+        wait_rows(t);
+        const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
+        if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
         if (ok) {
-          const uint8_t* row = p.kv + (int64_t)max(code, 0) * (DK * 2) + 16 * (lane & 7);
+          const uint8_t* row = p.kv + (int64_t)max(code, 0) * kRowBytes + 16 * l8;
 #pragma unroll
           for (int x = 0; x < 9; ++x)
-            cp_async16_zfill(base + SM_K + x * kBlk + sw128_off(krow, lane & 7), row + 128 * x, code >= 0);
+            cp_async16_zfill(base + SM_K + x * kBlk + sw128_off(4 * w + r4, l8), row + 128 * x, code >= 0);
         }
         cp_async_commit();
-        if (c.first) start_segment();
+        enter();
         cp_async_wait<0>();
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(k_full0);
         ++kc;
-        c.next(p);
+        --left;
       };
-      int code0 = look_up(), code1 = look_up(), code2 = look_up();  // tiles t, t+1, t+2
-      fetch(code1);
-      fetch(code2);
-      if (total > 0) store_k(code0);
+      if (total > 0) store_k(0);
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
-        if (t + 1 < total) store_k(code1);
-        if (t > 0) ok = ok && mbar_wait(mb_v_free, (t - 1) & 1, abort_flag, err, kWaitNs);
+        if (t + 1 < total) store_k(t + 1);
+        int code[2];
+        code[0] = ok ? rows_of(t)[8 * w + r4] : -1;
+        code[1] = ok ? rows_of(t)[8 * w + r4 + 4] : -1;
+        free_rows(t);
+        if (t > 0) wait(mb_v_free, (t - 1) & 1);
 #pragma unroll
         for (int rs = 0; rs < 2; ++rs) {
-          const int code = __shfl_sync(0xffffffffu, code0, 4 + (lane >> 3) + 4 * rs);
-          const uint8_t* row = p.kv + (int64_t)max(code, 0) * (DK * 2) + 256 * rank + 16 * (lane & 7);
+          const uint8_t* row = p.kv + (int64_t)max(code[rs], 0) * kRowBytes + 256 * rank + 16 * l8;
           if (ok) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)  // block x: columns [256 (x / 2) + 128 rank + 64 (x % 2), +64)
-              cp_async16_zfill(base + SM_V + x * kVBlk + sw128_off(vrow + 4 * rs, lane & 7),
-                               row + 512 * (x >> 1) + 128 * (x & 1), code >= 0);
+              cp_async16_zfill(base + SM_V + x * kVBlk + sw128_off(8 * w + r4 + 4 * rs, l8),
+                               row + 512 * (x >> 1) + 128 * (x & 1), code[rs] >= 0);
           }
         }
         cp_async_commit();
@@ -561,11 +618,49 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(v_full0);
-        code0 = code1;
-        code1 = code2;
-        code2 = look_up();
-        fetch(code2);
       }
+    }
+  } else if (warp == kRowWarp) {
+    // ------------------------------------------------------ rows of the tiles
+    // Block table -> cache row of each key, kRing tiles ahead.
+    uint64_t seen = 0;
+    int seg = 0;
+#pragma unroll 1
+    for (int t = 0; t < total; ++t) {
+      if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
+      int code[4];
+      row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
+      if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
+      if (ok) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
+        if (c.first && lane == 0) {
+          Segment sg;
+          sg.b = c.b;
+          sg.rt = c.rt;
+          sg.n = min(c.r.nt - c.tile, c.left);
+          sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
+          sg.nd = c.r.nd;
+          sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
+          segs[seg % kSegs] = sg;
+        }
+      }
+      if (c.first) ++seg;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb_r_full + 8 * (t % kRing));
+      c.next(p);
+    }
+  } else if (!kFp8 && warp >= kFetch0) {
+    // 16-bit rows go to shared memory when their buffer is free, without a stop in
+    // registers: these warps bring this CTA's half of the tile's keys into L2 (the
+    // other CTA brings the rest of V's).
+#pragma unroll 1
+    for (int t = 0; t < total; ++t) {
+      wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
+      const int code = ok ? ring[(t % kRing) * kKeys + 64 * rank + 32 * (warp - kFetch0) + lane] : -1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
+      if (code >= 0) prefetch_l2(p.kv + (int64_t)code * kRowBytes, kRowBytes);
     }
   } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------- MMA issue
@@ -575,36 +670,47 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         asm volatile("" : "+r"(at));
         return sw128_desc(base + at, lbo, 1024);
       };
-      Cursor cq = start, cp = start;
-      int kc = 0, gq = 0, gp = 0;
+      int kc = 0, gq = 0;
+      int qseg = 0, qleft = 0, passes = 1;  // segment of the next QK
       auto qk = [&]() {
-        const int passes = kFp8 && cq.r.seq <= kTwoPassKeys ? 2 : 1;
-        for (int s = 0; s < passes; ++s) {
-          ok = ok && mbar_wait(mb_k_full, kc & 1, abort_flag, err, kWaitNs);
-          if (ok) {
-            fence_after_sync();
-            const uint64_t dq = desc(SM_Q, 16), dk = desc(SM_K, 16);
-#pragma unroll
-            for (int kb = 0; kb < 9; ++kb)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_f16_ss_pair(tmem + S_COL + 64 * (gq & 1), dq + ((kb * kBlk + 32 * k) >> 4),
-                                dk + ((kb * kBlk + 32 * k) >> 4), IDESC_QK, (kb | k) != 0 || s > 0);
-            mma_commit_pair(mb_k_free);
+#pragma unroll 1
+        for (int s = 0; s < passes || s == 0; ++s) {
+          ok = ok && mbar_wait_lazy(mb_k_full, kc & 1, abort_flag, err, kWaitNs);
+          if (!ok) return;
+          if (qleft == 0) {  // its first tile is stored, so its descriptor is visible
+            qleft = segs[qseg % kSegs].n;
+            passes = segs[qseg % kSegs].flags & kTwo ? 2 : 1;
+            ++qseg;
           }
+          fence_after_sync();
+          const uint64_t dq = desc(SM_Q, 16), dk = desc(SM_K, 16);
+#pragma unroll
+          for (int kb = 0; kb < 9; ++kb)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_f16_ss_pair(tmem + S_COL + 64 * (gq & 1), dq + ((kb * kBlk + 32 * k) >> 4),
+                              dk + ((kb * kBlk + 32 * k) >> 4), IDESC_QK, (kb | k) != 0 || s > 0);
+          mma_commit_pair(mb_k_free);
           ++kc;
         }
-        if (ok) mma_commit_pair(mb_s_full + 8 * (gq & 1));
+        mma_commit_pair(mb_s_full + 8 * (gq & 1));
+        --qleft;
         ++gq;
-        cq.next(p);
       };
-      if (cq.left > 0) qk();
-      while (cp.left > 0 && ok) {
-        if (cq.left > 0) qk();
-        ok = ok && mbar_wait(mb_v_full, gp & 1, abort_flag, err, kWaitNs) &&
-             mbar_wait(mb_p_full, gp & 1, abort_flag, err, kWaitNs);
-        // the accumulator of the segment before has been read
-        if (cp.first && cp.seg > 0) ok = ok && mbar_wait(mb_o_free, (cp.seg - 1) & 1, abort_flag, err, kWaitNs);
+      if (total > 0) qk();
+      int pseg = 0, pleft = 0;
+#pragma unroll 1
+      for (int g = 0; g < total && ok; ++g) {
+        if (g + 1 < total) qk();
+        const bool first = pleft == 0;
+        ok = ok && mbar_wait_lazy(mb_v_full, g & 1, abort_flag, err, kWaitNs) &&
+             mbar_wait_lazy(mb_p_full, g & 1, abort_flag, err, kWaitNs);
+        if (first) {
+          // the accumulator of the segment before has been read
+          if (pseg > 0) ok = ok && mbar_wait_lazy(mb_o_free, (pseg - 1) & 1, abort_flag, err, kWaitNs);
+          if (ok) pleft = segs[pseg % kSegs].n;
+          ++pseg;
+        }
         if (ok) {
           fence_after_sync();
           const uint64_t dp = desc(SM_P, 16), dv = desc(SM_V, kVBlk);
@@ -613,11 +719,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll
             for (int s = 0; s < kKeys / 16; ++s)
               mma_f16_ss_pair(tmem + 128 * h, dp + (((s >> 2) * kBlk + 32 * (s & 3)) >> 4),
-                              dv + ((2 * h * kVBlk + 2048 * s) >> 4), IDESC_PV, !cp.first || s > 0);
+                              dv + ((2 * h * kVBlk + 2048 * s) >> 4), IDESC_PV, !first || s > 0);
           mma_commit_pair(mb_v_free);
         }
-        ++gp;
-        cp.next(p);
+        --pleft;
       }
       mma_commit_pair(mb_done);  // every MMA of this thread
     }
@@ -632,165 +737,167 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     const uint32_t t_sp = tmem + ((uint32_t)(32 * sp) << 16);
     const uint32_t p_full0 = cluster_map(mb_p_full, 0), o_free0 = cluster_map(mb_o_free, 0);
     uint8_t* prow = sm + SM_P + (sp >> 1) * kBlk;
-    Cursor c = start;
     int g = 0;
-    float m = kNoMax, L = 0.f, rs = 0.f;
-    int pre = 0;           // context positions; kNoRow for a row of no draft
-    bool full = false;     // the segment holds every key tile
-    for (; c.left > 0;) {
-      if (c.first) {
-        ok = ok && mbar_wait(mb_q_full + 8 * (c.seg & 3), (c.seg >> 2) & 1, abort_flag, err, kWaitNs);
-        const int r = c.rt * kPairRows + kRows * rank + row;
-        const int i = r / p.H;
-        const bool on = i < c.r.nd;
-        // not 0, so that a hidden key's -inf stays one
-        rs = fmaxf(p.scale_log2 * __int_as_float((127 + (int)qe[64 * (c.seg & 3) + row]) << 23), FLT_MIN);
-        pre = on ? c.r.seq - c.r.nd : kNoRow;
-        full = c.tile == 0 && c.left >= c.r.nt;
-        m = kNoMax;
-        L = 0.f;
-      }
-      const bool first = c.first;
-      // keys this thread's row sees, one bit each
-      const int d = pre == kNoRow ? -64 : pre - (c.tile * kKeys + kofs);
-      uint32_t allow = d >= 32 ? 0xffffffffu : d > 0 ? (1u << d) - 1 : 0u;
-      if (d < 32 && d > -64) {  // drafts among the keys
-        uint64_t bits = (uint64_t)p.mask[(int64_t)c.b * p.mask_stride + (c.rt * kPairRows + kRows * rank + row) / p.H];
-        if (c.r.nd < 64) bits &= (1ull << c.r.nd) - 1;
-        allow |= (uint32_t)(d >= 0 ? bits << d : bits >> -d);
-      }
-      ok = ok && mbar_wait(mb_s_full + 8 * (g & 1), (g >> 1) & 1, abort_flag, err, kWaitNs);
-      ok = __all_sync(0xffffffffu, ok);
-      fence_after_sync();
-      uint32_t s[32];
-      if (ok) {
-        tmem_ld32(t_sp + S_COL + 64 * (g & 1) + 32 * hh, s);
-        tmem_wait_ld();
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = 0u;
-      }
-      if (allow != 0xffffffffu) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;  // -inf
-      }
-      float mx = __uint_as_float(s[0]);
-#pragma unroll
-      for (int j = 1; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(s[j]));
-      mx *= rs;  // rs >= 0
-      float alpha = 1.f;
-      const bool any = named_bar_or(1, kSoftmaxWarps * 32, mx > m + kRescale);
-      if (any) {
-        rowx[64 * q4 + row] = mx;
-        named_bar(1, kSoftmaxWarps * 32);
-        const float rm = fmaxf(fmaxf(rowx[row], rowx[64 + row]), fmaxf(rowx[128 + row], rowx[192 + row]));
-        if (rm > m + kRescale) {
-          alpha = ex2(m - rm);
-          m = rm;
-          L *= alpha;
-        }
-      }
-      uint32_t pk[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float a = ex2(fmaf(__uint_as_float(s[2 * j]), rs, -m)), b = ex2(fmaf(__uint_as_float(s[2 * j + 1]), rs, -m));
-        L += a + b;
-        if (kBf16) {
-          const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-          pk[j] = *reinterpret_cast<const uint32_t*>(&v);
-        } else {
-          pk[j] = pack_half2(a, b);
-        }
-      }
-      // P's buffer and O are free once PV(t-1) has completed (the epilogue waited for a segment's last)
-      if (!first) ok = ok && mbar_wait(mb_v_free, (g - 1) & 1, abort_flag, err, kWaitNs);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) =
-              make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
-        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
-          fence_after_sync();
 #pragma unroll 1
-          for (int k = 0; k < 4; ++k) {
-            uint32_t o[32];
-            const uint32_t at = t_sp + 128 * hh + 32 * k;
-            tmem_ld32(at, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            tmem_st32(at, o);
-          }
-          tmem_wait_st();
+    for (int seg = 0; g < total; ++seg) {
+      wait(mb_q_full + 8 * (seg % kQeSegs), (seg / kQeSegs) & 1);
+      ok = !named_bar_or(1, kSoftmaxWarps * 32, !ok);  // all take the same number of barriers
+      const Segment& sg = segs[seg % kSegs];
+      const int end = ok ? g + sg.n : total;
+      // positions before the drafts, from this thread's first key of the tile on
+      int d = -64;
+      if (ok && (sg.rt * kPairRows + kRows * rank + row) / p.H < sg.nd) d = max(sg.pre - kofs, -64);
+      // not 0, so that a hidden key's -inf stays one
+      const float rs = fmaxf(p.scale_log2 * __int_as_float((127 + (int)qe[64 * (seg % kQeSegs) + row]) << 23), FLT_MIN);
+      float m = kNoMax, L = 0.f;
+      bool first = true;
+#pragma unroll 1
+      for (; g < end; ++g) {
+        // keys this thread's row sees, one bit each
+        uint32_t allow = d >= 32 ? 0xffffffffu : d > 0 ? (1u << d) - 1 : 0u;
+        if (d < 32 && d > -64) {  // drafts among the keys
+          uint64_t bits = (uint64_t)p.mask[(int64_t)sg.b * p.mask_stride + (sg.rt * kPairRows + kRows * rank + row) / p.H];
+          if (sg.nd < 64) bits &= (1ull << sg.nd) - 1;
+          allow |= (uint32_t)(d >= 0 ? bits << d : bits >> -d);
         }
-      }
-      fence_proxy_async();
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(p_full0);
-      const bool last = c.last();
-      if (last) {
-        // ------------------------------------------- epilogue of the segment
-        named_bar(1, kSoftmaxWarps * 32);  // rowx: every thread is past its use as maxima
-        rowx[64 * q4 + row] = L;
-        named_bar(1, kSoftmaxWarps * 32);
-        L = (rowx[row] + rowx[64 + row]) + (rowx[128 + row] + rowx[192 + row]);
-        named_bar(1, kSoftmaxWarps * 32);
-        ok = ok && mbar_wait(mb_v_free, g & 1, abort_flag, err, kWaitNs);
-        ok = __all_sync(0xffffffffu, ok);
+        d = max(d - kKeys, -64);
+        wait(mb_s_full + 8 * (g & 1), (g >> 1) & 1);
+        fence_after_sync();
+        uint32_t s[32];
         if (ok) {
-          fence_after_sync();
-          const bool mine = c.rt * kPairRows + kRows * rank + row < p.T * p.H;
-          const int slot = 2 * pair + (c.seg == 0 ? 0 : 1);
-          const int col0 = 256 * hh + 128 * (sp >> 1);
-          const int64_t grow = (int64_t)c.b * p.T * p.H + c.rt * kPairRows + kRows * rank + row;
-          const int64_t prow_i = (int64_t)slot * p.slot_rows + kRows * rank + row;
-          const float inv = L > 0.f ? 1.f / L : 0.f;
-#pragma unroll 1
-          for (int k = 0; k < 4; ++k) {
-            uint32_t o[32];
-            tmem_ld32(t_sp + 128 * hh + 32 * k, o);
-            tmem_wait_ld();
-            if (!mine) continue;
-            if (full) {
-              uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.o) + (grow * DV + col0 + 32 * k) * 2);
+          tmem_ld32(t_sp + S_COL + 64 * (g & 1) + 32 * hh, s);
+          tmem_wait_ld();
+        } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t v[4];
+          for (int j = 0; j < 32; ++j) s[j] = 0u;
+        }
+        if (allow != 0xffffffffu) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const float a = __uint_as_float(o[8 * e + 2 * x]) * inv, b = __uint_as_float(o[8 * e + 2 * x + 1]) * inv;
-                  if (p.o_bf16) {
-                    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-                    v[x] = *reinterpret_cast<const uint32_t*>(&t);
-                  } else {
-                    v[x] = pack_half2(a, b);
-                  }
-                }
-                dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
-              }
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(p.part_o + prow_i * DV + col0 + 32 * k);
+          for (int j = 0; j < 32; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;  // -inf
+        }
+        float mx = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
 #pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            }
-          }
-          if (mine && q4 == 0) {
-            if (full) {
-              p.lse[grow] = L > 0.f ? (m + log2f(L)) * kLn2 : -INFINITY;
-            } else {
-              p.part_ml[prow_i * 2] = m;
-              p.part_ml[prow_i * 2 + 1] = L;
-            }
+        for (int j = 2; j < 32; j += 2) mx = max3(mx, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+        mx *= rs;  // rs >= 0
+        float alpha = 1.f;
+        const bool any = named_bar_or(1, kSoftmaxWarps * 32, mx > m + kRescale);
+        if (any) {
+          rowx[64 * q4 + row] = mx;
+          named_bar(1, kSoftmaxWarps * 32);
+          const float rm = fmaxf(fmaxf(rowx[row], rowx[64 + row]), fmaxf(rowx[128 + row], rowx[192 + row]));
+          if (rm > m + kRescale) {
+            alpha = ex2(m - rm);
+            m = rm;
+            L *= alpha;
           }
         }
+        uint32_t pk[16];
+        const uint64_t rs2 = pack64(rs, rs), nm2 = pack64(-m, -m);
+        uint64_t sum2 = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float a, b;
+          unpack64(fma2(pack64(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), rs2, nm2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          sum2 = add2(sum2, pack64(a, b));
+          if (kBf16) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+            pk[j] = *reinterpret_cast<const uint32_t*>(&v);
+          } else {
+            pk[j] = pack_half2(a, b);
+          }
+        }
+        {
+          float a, b;
+          unpack64(sum2, a, b);
+          L += a + b;
+        }
+        // P's buffer and O are free once PV(t-1) has completed (the epilogue waited for a segment's last)
+        if (!first) wait(mb_v_free, (g - 1) & 1);
+        if (ok) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) =
+                make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
+          if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
+            fence_after_sync();
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) {
+              uint32_t o[32];
+              const uint32_t at = t_sp + 128 * hh + 32 * k;
+              tmem_ld32(at, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              tmem_st32(at, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        fence_proxy_async();
         fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(o_free0);
+        if (lane == 0) mbar_arrive_cluster(p_full0);
+        first = false;
       }
-      ++g;
-      c.next(p);
+      // ------------------------------------------- epilogue of the segment
+      named_bar(1, kSoftmaxWarps * 32);  // rowx: every thread is past its use as maxima
+      rowx[64 * q4 + row] = L;
+      named_bar(1, kSoftmaxWarps * 32);
+      L = (rowx[row] + rowx[64 + row]) + (rowx[128 + row] + rowx[192 + row]);
+      named_bar(1, kSoftmaxWarps * 32);
+      wait(mb_v_free, (g - 1) & 1);
+      if (ok) {
+        fence_after_sync();
+        const bool mine = sg.rt * kPairRows + kRows * rank + row < p.T * p.H;
+        const bool full = (sg.flags & kFull) != 0;
+        const int slot = 2 * pair + (seg == 0 ? 0 : 1);
+        const int col0 = 256 * hh + 128 * (sp >> 1);
+        const int64_t grow = (int64_t)sg.b * p.T * p.H + sg.rt * kPairRows + kRows * rank + row;
+        const int64_t prow_i = (int64_t)slot * p.slot_rows + kRows * rank + row;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32(t_sp + 128 * hh + 32 * k, o);
+          tmem_wait_ld();
+          if (mine && full) {
+            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.o) + (grow * DV + col0 + 32 * k) * 2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t v[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float a = __uint_as_float(o[8 * e + 2 * x]) * inv, b = __uint_as_float(o[8 * e + 2 * x + 1]) * inv;
+                if (p.o_bf16) {
+                  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+                  v[x] = *reinterpret_cast<const uint32_t*>(&t);
+                } else {
+                  v[x] = pack_half2(a, b);
+                }
+              }
+              dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          } else if (mine) {
+            uint4* dst = reinterpret_cast<uint4*>(p.part_o + prow_i * DV + col0 + 32 * k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (mine && q4 == 0) {
+          if (full) {
+            p.lse[grow] = L == 0.f ? -INFINITY : (m + log2f(L)) * kLn2;
+          } else {
+            p.part_ml[prow_i * 2] = m;
+            p.part_ml[prow_i * 2 + 1] = L;
+          }
+        }
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(o_free0);
     }
   }
   // every MMA has completed before TMEM is released, and no CTA leaves while the
