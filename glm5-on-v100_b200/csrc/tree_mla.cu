@@ -61,7 +61,7 @@ constexpr int kPairRows = 128;  // rows of a cluster
 constexpr int kRows = 64;       // rows of a CTA
 constexpr int kKeys = 128;      // keys of a tile
 constexpr int DK = 576, DV = 512;
-constexpr int kProducers = 16;
+constexpr int kKWarps = 8, kVWarps = 8;  // warps 0-7: Q and K, warps 8-15: V
 constexpr int kSoftmax0 = 16, kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 24, kRowWarp = 25, kFetch0 = 26, kFetchWarps = 2;
 constexpr int kRing = 3;        // tiles whose cache rows are known ahead
@@ -105,6 +105,18 @@ struct TreeArgs {
   uint32_t q_sign;   // 0x80008000 for a negative scale
   float scale_log2;  // its magnitude
 };
+
+// A cache row of zeros: what positions without a row read, so that loads need no branch.
+struct alignas(16) ZeroRow {
+  uint8_t code[512];
+  float scale[4];
+  uint16_t rotary[64];
+};
+__device__ const ZeroRow g_zero_row = {{0}, {1.f, 1.f, 1.f, 1.f}, {0}};
+
+__device__ __forceinline__ const uint8_t* fp8_row(const uint8_t* kv, int code) {
+  return code >= 0 ? kv + (int64_t)code * 656 : reinterpret_cast<const uint8_t*>(&g_zero_row);
+}
 
 // Request b's size: key tiles and row tiles (0 tiles: nothing to do).
 struct Req {
@@ -262,8 +274,8 @@ struct Scale {
 template <int HOW>
 __device__ __forceinline__ uint4 dequant8(uint2 v, const Scale& sc) {
   __half2 x[4];
-  e4m3x4_to_half2x2(pinned(v.x), x[0], x[1]);
-  e4m3x4_to_half2x2(pinned(v.y), x[2], x[3]);
+  e4m3x4_to_half2x2(v.x, x[0], x[1]);
+  e4m3x4_to_half2x2(v.y, x[2], x[3]);
   uint32_t q[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -322,34 +334,38 @@ __device__ __forceinline__ void row_codes(const TreeArgs& p, int b, const Req& r
 }
 
 // This CTA's 64 query rows into shared memory (f16, or bf16 as it is): warp w
-// rows 4w + lane / 8, eight lanes a row. qe[row]: the power of two that a bf16
-// row was divided by.
+// rows 8w + lane / 8 and four on, eight lanes a row. qe[row]: the power of two
+// that a bf16 row was divided by.
 template <int FMT>
-__device__ __forceinline__ void load_q(const TreeArgs& p, uint8_t* sm_q, int8_t* qe, int b, int row0, int w, int lane) {
-  const int row = 4 * w + (lane >> 3), l8 = lane & 7;
-  const bool on = row0 + row < p.T * p.H;
-  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
-                                                    ((int64_t)b * p.T * p.H + row0 + row) * DK * 2);
-  int e = 0;
-  if (FMT != DSA_BF16 && p.q_bf16) {
-    uint32_t bits = 0;
-    if (on) {
+__device__ __forceinline__ void load_q(const TreeArgs& p, uint32_t sm_q, int8_t* qe, int b, int row0, int w, int lane) {
+  const int l8 = lane & 7;
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const int row = 8 * w + 4 * i + (lane >> 3);
+    const bool on = row0 + row < p.T * p.H;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
+                                                      ((int64_t)b * p.T * p.H + row0 + row) * DK * 2);
+    int e = 0;
+    if (FMT != DSA_BF16 && p.q_bf16) {
+      uint32_t bits = 0;
+      if (on) {
 #pragma unroll 3
-      for (int c = 0; c < 9; ++c) bits = max(bits, bf16x8_max_abs_bits(__ldg(src + l8 + 8 * c)));
+        for (int c = 0; c < 9; ++c) bits = max(bits, bf16x8_max_abs_bits(__ldg(src + l8 + 8 * c)));
+      }
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
+      e = bf16_fp16_shift(bits);
     }
-    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
-    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
-    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
-    e = bf16_fp16_shift(bits);
-  }
 #pragma unroll 3
-  for (int c = 0; c < 9; ++c) {
-    uint4 v = on ? __ldg(src + l8 + 8 * c) : make_uint4(0, 0, 0, 0);
-    if (FMT != DSA_BF16 && p.q_bf16) v = bf16x8_to_half8_scaled(v, e);
-    v = make_uint4(v.x ^ p.q_sign, v.y ^ p.q_sign, v.z ^ p.q_sign, v.w ^ p.q_sign);
-    *reinterpret_cast<uint4*>(sm_q + c * kBlk + sw128_off(row, l8)) = v;
+    for (int c = 0; c < 9; ++c) {
+      uint4 v = on ? __ldg(src + l8 + 8 * c) : make_uint4(0, 0, 0, 0);
+      if (FMT != DSA_BF16 && p.q_bf16) v = bf16x8_to_half8_scaled(v, e);
+      v = make_uint4(v.x ^ p.q_sign, v.y ^ p.q_sign, v.z ^ p.q_sign, v.w ^ p.q_sign);
+      sts16(sm_q + c * kBlk + sw128_off(row, l8), v);
+    }
+    if (l8 == 0) qe[row] = (int8_t)e;
   }
-  if (l8 == 0) qe[row] = (int8_t)e;
 }
 
 // FMT: the cache's format.
@@ -386,18 +402,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   Cursor c{};  // the row warp's
   if (warp == 0) {
     if (lane == 0) {
-      mbar_init(mb_k_full, 2 * kProducers);
+      mbar_init(mb_k_full, 2 * kKWarps);
       mbar_init(mb_k_free, 1);
-      mbar_init(mb_v_full, 2 * kProducers);
+      mbar_init(mb_v_full, 2 * kVWarps);
       mbar_init(mb_v_free, 1);
       mbar_init(mb_p_full, 2 * kSoftmaxWarps);
       mbar_init(mb_o_free, 2 * kSoftmaxWarps);
       mbar_init(mb_done, 1);
       for (int x = 0; x < 2; ++x) mbar_init(mb_s_full + 8 * x, 1);
-      for (int x = 0; x < kQeSegs; ++x) mbar_init(mb_q_full + 8 * x, kProducers);
+      for (int x = 0; x < kQeSegs; ++x) mbar_init(mb_q_full + 8 * x, kKWarps);
       for (int x = 0; x < kRing; ++x) {
         mbar_init(mb_r_full + 8 * x, 1);
-        mbar_init(mb_r_free + 8 * x, kProducers + (kFp8 ? 0 : kFetchWarps));
+        mbar_init(mb_r_free + 8 * x, kKWarps + kVWarps + (kFp8 ? 0 : kFetchWarps));
       }
       mbar_init_fence();
       *abort_flag = 0;
@@ -422,202 +438,202 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   };
   // After a wait that ran out (`ok` false, abort flag set) every thread still
   // executes its role's barriers and arrivals, and later waits return at once.
-  if (warp < kProducers) {
-    // ------------------------------------------------------------- producers
+  // rows of tile t, from the row warp: each reader of a slot frees it
+  auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
+  auto wait_rows = [&](int t) { wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1); };
+  auto free_rows = [&](int t) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
+  };
+  // what this warp has stored is the tensor cores' to read
+  auto announce = [&](uint32_t full_of_cta0) {
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(full_of_cta0);
+  };
+  // A lane of the expanding warps holds 16 neighbouring columns: chunks 2 (lane & 3)
+  // and the next of a 64-column block. Lanes of odd blocks store the second chunk
+  // first, so that the eight lanes of a store cover all banks.
+  const bool odd = (lane >> 2) & 1;
+  auto put16 = [&](auto how, uint32_t at, const uint4& v, float scale) {
+    constexpr int HOW = decltype(how)::value;
+    const uint4 d = make_uint4(pinned(v.x), pinned(v.y), pinned(v.z), pinned(v.w));
+    const Scale s(scale);
+    const uint4 first = dequant8<HOW>(odd ? make_uint2(d.z, d.w) : make_uint2(d.x, d.y), s);
+    const uint4 second = dequant8<HOW>(odd ? make_uint2(d.x, d.y) : make_uint2(d.z, d.w), s);
+    sts16(at, first);
+    sts16(at ^ 16, second);
+  };
+  auto all_fast = [](float f) { return __all_sync(0xffffffffu, fast_scale(f)); };
+
+  if (warp < kKWarps) {
+    // -------------------------------------------------------------- Q and K
+    // K(t+1) is stored under PV(t-1); its successor's loads have a tile's time to arrive.
     const int w = warp;
-    const uint32_t k_full0 = cluster_map(mb_k_full, 0), v_full0 = cluster_map(mb_v_full, 0);
-    // Per tile t: store K(t+1) and load K(t+2), store V(t) and load V(t+1): K(t+1)
-    // is stored under PV(t-1) and V(t) under QK(t+1), and a load has most of a
-    // tile's time to arrive.
+    const uint32_t k_full0 = cluster_map(mb_k_full, 0);
     int kc = 0;             // K stores so far (two per tile in two-pass segments)
     int seg = 0, left = 0;  // the segment of the next K store, and its tiles left
     bool two = false;
-    // Lane (l & 15) of a half warp takes the 16 bytes of codes at 16 cx of a
-    // 128-wide group, of the first row for l & 4 = 0, else of the second: the eight
-    // lanes of a store hold even chunks of an even and an odd row, which the swizzle
-    // puts on different banks.
-    const int cx = (lane & 3) + 4 * ((lane >> 3) & 1);
-    const int lrow = 2 * (lane >> 4) + ((lane >> 2) & 1);
-    const int krow = 4 * w + lrow, vrow = 8 * w + lrow;
-    // rows of tile t: the ring is filled by the row warp
-    auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
-    auto wait_rows = [&](int t) {
-      wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
-    };
-    auto free_rows = [&](int t) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
-    };
     // before a K store: the next segment's Q, when its first tile is due
     auto enter = [&]() {
       if (left > 0) return;
       const Segment& sg = segs[seg % kSegs];  // visible: the wait for this tile's rows
       left = sg.n;
       two = (sg.flags & kTwo) != 0;
-      if (ok) load_q<FMT>(p, sm + SM_Q, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
+      if (ok) load_q<FMT>(p, base + SM_Q, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(mb_q_full + 8 * (seg % kQeSegs));
       ++seg;
     };
     if constexpr (kFp8) {
-      uint4 kd[4], tail, vd[4];  // K: the four groups and the rotary tail of this lane's key | V: [key][group]
-      float4 ks, vs;             // their scales
-      auto load_k = [&](int t) {
+      // rows 8w + x, 16 codes a lane (a whole row a load: the fewest cache lines), 16
+      // bytes of the rotary tail of rows 8w + 4i + lane / 8, and scale lane & 3 of row
+      // 8w + lane / 4
+      uint4 d[8], tail[2];
+      float sc = 1.f;
+      auto load = [&](int t) {
         wait_rows(t);
-        const int code = ok ? rows_of(t)[64 * rank + krow] : -1;
-        const uint8_t* row = p.kv + (int64_t)code * kRowBytes;
-        auto get = [&]() {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) kd[j] = ldg_nc16(row + 16 * cx + 128 * j);
-          tail = ldg_nc16(row + 528 + 16 * cx);
-          const uint4 x = ldg_nc16(row + 512);
-          ks = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
-        };
-        if (__all_sync(0xffffffffu, code >= 0)) {
-          get();
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) kd[j] = make_uint4(0, 0, 0, 0);
-          ks = make_float4(1.f, 1.f, 1.f, 1.f);
-          tail = make_uint4(0, 0, 0, 0);
-          if (code >= 0) get();
-        }
-      };
-      auto load_v = [&](int t) {
-        int code[2];
-        code[0] = ok ? rows_of(t)[vrow] : -1;
-        code[1] = ok ? rows_of(t)[vrow + 4] : -1;
+        if (!ok) return;
+        const int* rows = rows_of(t) + 64 * rank + 8 * w;
+        const int4 c0 = *reinterpret_cast<const int4*>(rows), c1 = *reinterpret_cast<const int4*>(rows + 4);
+        const int t0 = rows[lane >> 3], t1 = rows[4 + (lane >> 3)], ts = rows[lane >> 2];
         free_rows(t);
-        auto get = [&](int x) {
-          const uint8_t* row = p.kv + (int64_t)code[x] * kRowBytes;
-          vd[2 * x] = ldg_nc16(row + 16 * cx + 128 * rank);
-          vd[2 * x + 1] = ldg_nc16(row + 16 * cx + 128 * rank + 256);
-          (x ? vs.z : vs.x) = __ldg(reinterpret_cast<const float*>(row + 512) + rank);
-          (x ? vs.w : vs.y) = __ldg(reinterpret_cast<const float*>(row + 512) + rank + 2);
-        };
-        if (__all_sync(0xffffffffu, code[0] >= 0 && code[1] >= 0)) {
-          get(0);
-          get(1);
-        } else {
+        const int code[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vd[j] = make_uint4(0, 0, 0, 0);
-          vs = make_float4(1.f, 1.f, 1.f, 1.f);
-          if (code[0] >= 0) get(0);
-          if (code[1] >= 0) get(1);
+        for (int x = 0; x < 8; ++x) {
+          d[x] = ldg_nc16(fp8_row(p.kv, code[x]) + 16 * lane);
         }
+        sc = __ldg(reinterpret_cast<const float*>(fp8_row(p.kv, ts) + 512) + (lane & 3));
+        tail[0] = ldg_nc16(fp8_row(p.kv, t0) + 528 + 16 * (lane & 7));
+        tail[1] = ldg_nc16(fp8_row(p.kv, t1) + 528 + 16 * (lane & 7));
       };
-      auto all_fast = [](const float4& f) {
-        return __all_sync(0xffffffffu, fast_scale(f.x) && fast_scale(f.y) && fast_scale(f.z) && fast_scale(f.w));
-      };
-      const uint32_t k_at = base + SM_K + (cx >> 2) * kBlk + sw128_off(krow, 2 * (cx & 3));
-      const uint32_t v_at = base + SM_V + (cx >> 2) * kVBlk + sw128_off(vrow, 2 * (cx & 3));
-      auto put = [&](auto how, auto is_k) {
-        constexpr int HOW = decltype(how)::value;
-        constexpr bool K = decltype(is_k)::value;
-        const float4 f = K ? ks : vs;
+      const uint32_t at = base + SM_K + (lane >> 2) * kBlk + sw128_off(8 * w, 2 * (lane & 3) + odd);
+      const uint32_t tail_at = base + SM_K + 8 * kBlk + sw128_off(8 * w + (lane >> 3), lane & 7);
+      auto put = [&](auto how) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const Scale s(x == 0 ? f.x : x == 1 ? f.y : x == 2 ? f.z : f.w);
-          const uint4 d = K ? kd[x] : vd[x];
-          // V: key vrow + 4 (x / 2): half a swizzle atom on, so chunks flip bit 2
-          const uint32_t at =
-              K ? k_at + 2 * x * kBlk : ((v_at + 512 * (x >> 1)) ^ (64 * (x >> 1))) + 2 * (x & 1) * kVBlk;
-          sts16(at, dequant8<HOW>(make_uint2(d.x, d.y), s));
-          sts16(at ^ 16, dequant8<HOW>(make_uint2(d.z, d.w), s));
-        }
+        for (int x = 0; x < 8; ++x)
+          put16(how, (at ^ (16 * x)) + 128 * x, d[x], __shfl_sync(0xffffffffu, sc, 4 * x + (lane >> 3)));
       };
-      // K of tile c: wait for the buffer, store, announce. In two-pass tiles the
-      // first pass rounds in f32: the second stores its remainder.
-      auto store_k = [&]() {
+      if (total > 0) load(0);
+#pragma unroll 1
+      for (int t = 0; t < total; ++t) {
         if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
         enter();
-        const int passes = two ? 2 : 1;
-#pragma unroll 1
-        for (int s = 0; s < passes; ++s) {
-          if (s > 0) wait(mb_k_free, (kc - 1) & 1);
+        if (ok) {
+          // two passes: the first rounds in f32, the second stores its remainder
+          if (!two && all_fast(sc))
+            put(std::integral_constant<int, kFast>());
+          else
+            put(std::integral_constant<int, kWide>());
+          sts16(tail_at, tail[0]);
+          sts16((tail_at ^ 64) + 512, tail[1]);
+        }
+        announce(k_full0);
+        ++kc;
+        if (two) {
+          wait(mb_k_free, (kc - 1) & 1);
           if (ok) {
-            if (s > 0)
-              put(std::integral_constant<int, kRest>(), std::true_type());
-            else if (passes == 1 && all_fast(ks))
-              put(std::integral_constant<int, kFast>(), std::true_type());
-            else
-              put(std::integral_constant<int, kWide>(), std::true_type());
-            sts16(base + SM_K + 8 * kBlk + sw128_off(krow, cx), s > 0 ? make_uint4(0, 0, 0, 0) : tail);
+            put(std::integral_constant<int, kRest>());
+            sts16(tail_at, make_uint4(0, 0, 0, 0));
+            sts16((tail_at ^ 64) + 512, make_uint4(0, 0, 0, 0));
           }
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(k_full0);
+          announce(k_full0);
           ++kc;
         }
         --left;
-      };
-      if (total > 0) {
-        load_k(0);
-        load_v(0);
-        store_k();
-        if (total > 1) load_k(1);
-      }
-#pragma unroll 1
-      for (int t = 0; t < total; ++t) {
-        if (t + 1 < total) store_k();
-        if (t + 2 < total) load_k(t + 2);
-        if (t > 0) wait(mb_v_free, (t - 1) & 1);
-        if (ok) {
-          if (all_fast(vs))
-            put(std::integral_constant<int, kFast>(), std::false_type());
-          else
-            put(std::integral_constant<int, kWide>(), std::false_type());
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(v_full0);
-        if (t + 1 < total) load_v(t + 1);
+        if (t + 1 < total) load(t + 1);
       }
     } else {
       const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
-      auto store_k = [&](int t) {
+#pragma unroll 1
+      for (int t = 0; t < total; ++t) {
         wait_rows(t);
-        const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
+        int code[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) code[i] = ok ? rows_of(t)[64 * rank + 8 * w + 4 * i + r4] : -1;
+        free_rows(t);
         if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
         if (ok) {
-          const uint8_t* row = p.kv + (int64_t)max(code, 0) * kRowBytes + 16 * l8;
 #pragma unroll
-          for (int x = 0; x < 9; ++x)
-            cp_async16_zfill(base + SM_K + x * kBlk + sw128_off(4 * w + r4, l8), row + 128 * x, code >= 0);
+          for (int i = 0; i < 2; ++i) {
+            const uint8_t* row = p.kv + (int64_t)max(code[i], 0) * kRowBytes + 16 * l8;
+#pragma unroll
+            for (int x = 0; x < 9; ++x)
+              cp_async16_zfill(base + SM_K + x * kBlk + sw128_off(8 * w + 4 * i + r4, l8), row + 128 * x, code[i] >= 0);
+          }
         }
         cp_async_commit();
         enter();
         cp_async_wait<0>();
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(k_full0);
+        announce(k_full0);
         ++kc;
         --left;
+      }
+    }
+  } else if (warp < kKWarps + kVWarps) {
+    // -------------------------------------------------------------------- V
+    // This CTA's 256 columns of all 128 keys; V(t) is stored under QK(t+1).
+    const int w = warp - kKWarps;
+    const uint32_t v_full0 = cluster_map(mb_v_full, 0);
+    if constexpr (kFp8) {
+      uint4 d[8];      // rows 16w + 2x + lane / 16
+      float sc = 1.f;  // of row 16w + lane / 2, group 2 rank + (lane & 1)
+      auto load = [&](int t) {
+        wait_rows(t);
+        if (!ok) return;
+        const int* rows = rows_of(t) + 16 * w;
+        int code[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) code[x] = rows[2 * x + (lane >> 4)];
+        const int ts = rows[lane >> 1];
+        free_rows(t);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) d[x] = ldg_nc16(fp8_row(p.kv, code[x]) + 256 * rank + 16 * (lane & 15));
+        sc = __ldg(reinterpret_cast<const float*>(fp8_row(p.kv, ts) + 512) + 2 * rank + (lane & 1));
       };
-      if (total > 0) store_k(0);
+      const uint32_t at =
+          base + SM_V + ((lane >> 2) & 3) * kVBlk + sw128_off(16 * w + (lane >> 4), 2 * (lane & 3) + odd);
+      auto put = [&](auto how) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          put16(how, (at ^ (32 * (x & 3))) + 256 * (x & 3) + 1024 * (x >> 2), d[x],
+                __shfl_sync(0xffffffffu, sc, 4 * x + 2 * (lane >> 4) + ((lane >> 3) & 1)));
+      };
+      if (total > 0) load(0);
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
-        if (t + 1 < total) store_k(t + 1);
-        int code[2];
-        code[0] = ok ? rows_of(t)[8 * w + r4] : -1;
-        code[1] = ok ? rows_of(t)[8 * w + r4 + 4] : -1;
+        if (t > 0) wait(mb_v_free, (t - 1) & 1);
+        if (ok) {
+          if (all_fast(sc))
+            put(std::integral_constant<int, kFast>());
+          else
+            put(std::integral_constant<int, kWide>());
+        }
+        announce(v_full0);
+        if (t + 1 < total) load(t + 1);
+      }
+    } else {
+      const int r4 = lane >> 3, l8 = lane & 7;
+#pragma unroll 1
+      for (int t = 0; t < total; ++t) {
+        wait_rows(t);
+        int code[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) code[i] = ok ? rows_of(t)[16 * w + 4 * i + r4] : -1;
         free_rows(t);
         if (t > 0) wait(mb_v_free, (t - 1) & 1);
+        if (ok) {
 #pragma unroll
-        for (int rs = 0; rs < 2; ++rs) {
-          const uint8_t* row = p.kv + (int64_t)max(code[rs], 0) * kRowBytes + 256 * rank + 16 * l8;
-          if (ok) {
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t* row = p.kv + (int64_t)max(code[i], 0) * kRowBytes + 512 * rank + 16 * l8;
 #pragma unroll
-            for (int x = 0; x < 4; ++x)  // block x: columns [256 (x / 2) + 128 rank + 64 (x % 2), +64)
-              cp_async16_zfill(base + SM_V + x * kVBlk + sw128_off(8 * w + r4 + 4 * rs, l8),
-                               row + 512 * (x >> 1) + 128 * (x & 1), code[rs] >= 0);
+            for (int x = 0; x < 4; ++x)
+              cp_async16_zfill(base + SM_V + x * kVBlk + sw128_off(16 * w + 4 * i + r4, l8), row + 128 * x, code[i] >= 0);
           }
         }
         cp_async_commit();
         cp_async_wait<0>();
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(v_full0);
+        announce(v_full0);
       }
     }
   } else if (warp == kRowWarp) {
@@ -630,6 +646,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
       int code[4];
       row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
+      if constexpr (kFp8) {
+        // this CTA's half into L2: neighbouring rows as one run
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int mine = rank ? code[2 + k] : code[k];
+          const int head = __shfl_sync(0xffffffffu, mine, 0);
+          if (__all_sync(0xffffffffu, mine >= 0 && mine == head + lane)) {
+            if (lane == 0) prefetch_l2(p.kv + (int64_t)mine * kRowBytes, 32 * kRowBytes);
+          } else if (mine >= 0) {
+            prefetch_l2(p.kv + (int64_t)mine * kRowBytes, kRowBytes);
+          }
+        }
+      }
       if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
       if (ok) {
 #pragma unroll
@@ -853,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         const bool mine = sg.rt * kPairRows + kRows * rank + row < p.T * p.H;
         const bool full = (sg.flags & kFull) != 0;
         const int slot = 2 * pair + (seg == 0 ? 0 : 1);
-        const int col0 = 256 * hh + 128 * (sp >> 1);
+        const int col0 = 256 * (sp >> 1) + 128 * hh;  // lanes 64-127: CTA 1's columns
         const int64_t grow = (int64_t)sg.b * p.T * p.H + sg.rt * kPairRows + kRows * rank + row;
         const int64_t prow_i = (int64_t)slot * p.slot_rows + kRows * rank + row;
         const float inv = L == 0.f ? 0.f : 1.f / L;
