@@ -61,24 +61,27 @@ constexpr int kPairRows = 128;  // rows of a cluster
 constexpr int kRows = 64;       // rows of a CTA
 constexpr int kKeys = 128;      // keys of a tile
 constexpr int DK = 576, DV = 512;
-constexpr int kKWarps = 8, kVWarps = 8;  // warps 0-7: Q and K, warps 8-15: V
+constexpr int kProducers = 16;  // warps 0-15
 constexpr int kSoftmax0 = 16, kSoftmaxWarps = 8;
-constexpr int kMmaWarp = 24, kRowWarp = 25, kFetch0 = 26, kFetchWarps = 2;
-constexpr int kRing = 3;        // tiles whose cache rows are known ahead
+constexpr int kMmaWarp = 24, kRowWarp = 25;
+constexpr int kTail0 = 26, kTailWarps = 2;  // fp8: the rotary part of K; 16-bit: L2 prefetch
+constexpr int kRing = 3;        // 16-bit caches: tiles whose cache rows are known ahead
 constexpr int kThreads = 28 * 32;
 constexpr uint32_t kBlk = 64 * 128;    // 64 rows x 64 16-bit values: 8 KB
 constexpr uint32_t kVBlk = 128 * 128;  // 128 keys x 64 columns: 16 KB
+constexpr int kQtBlks = 6;             // 64-column blocks of Q in tensor memory; the other three in shared memory
 constexpr uint32_t SM_Q = 0;
-constexpr uint32_t SM_K = SM_Q + 9 * kBlk;
+constexpr uint32_t SM_K = SM_Q + (9 - kQtBlks) * kBlk;
 constexpr uint32_t SM_V = SM_K + 9 * kBlk;
 constexpr uint32_t SM_P = SM_V + 4 * kVBlk;
-constexpr uint32_t SM_MISC = SM_P + 2 * kBlk;
+constexpr uint32_t SM_RAW = SM_P + 2 * kBlk;       // fp8: this CTA's 64 cache rows as they lie in the cache
+constexpr uint32_t SM_RING = SM_RAW + 64 * 656;    // 16-bit: rows[kRing][128]
+constexpr uint32_t SM_MISC = SM_RING + kRing * kKeys * 4;
 constexpr int kSegs = 6;        // segment descriptors kept: the row warp is at most five tiles ahead of an epilogue
 constexpr int kQeSegs = 3;      // Q is at most two segments ahead of the softmax
-// the misc block: 18 mbarriers | TMEM base, abort flag, tiles of the run | qe | row maxima / sums | rows ahead | segments
-constexpr uint32_t kQeAt = 160, kRowxAt = kQeAt + kQeSegs * 64, kRingAt = kRowxAt + 4 * 64 * 4,
-                   kSegAt = kRingAt + kRing * kKeys * 4;
-constexpr uint32_t S_COL = 256;        // S buffer x at [256 + 64x, +64); O half h at [128h, +128)
+// the misc block: mbarriers | TMEM base, abort flag, tiles of the run, valid rows | qe | row maxima / sums | segments
+constexpr uint32_t kBarAt = 0, kWordsAt = 192, kQeAt = 224, kRowxAt = kQeAt + kQeSegs * 64, kSegAt = kRowxAt + 4 * 64 * 4;
+constexpr uint32_t S_COL = 256, Q_COL = 320;  // O half h at [128h, +128), S at [256, +64), Q at [320, +192)
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kNoMax = -1e30f;
@@ -105,18 +108,6 @@ struct TreeArgs {
   uint32_t q_sign;   // 0x80008000 for a negative scale
   float scale_log2;  // its magnitude
 };
-
-// A cache row of zeros: what positions without a row read, so that loads need no branch.
-struct alignas(16) ZeroRow {
-  uint8_t code[512];
-  float scale[4];
-  uint16_t rotary[64];
-};
-__device__ const ZeroRow g_zero_row = {{0}, {1.f, 1.f, 1.f, 1.f}, {0}};
-
-__device__ __forceinline__ const uint8_t* fp8_row(const uint8_t* kv, int code) {
-  return code >= 0 ? kv + (int64_t)code * 656 : reinterpret_cast<const uint8_t*>(&g_zero_row);
-}
 
 // Request b's size: key tiles and row tiles (0 tiles: nothing to do).
 struct Req {
@@ -294,6 +285,30 @@ __device__ __forceinline__ uint4 dequant8(uint2 v, const Scale& sc) {
   return make_uint4(q[0], q[1], q[2], q[3]);
 }
 
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ float lds4(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ void sts16_cluster(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+// Bytes of global memory (both 16-byte aligned, a multiple of 16) into this CTA's shared memory.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(mbar)
+               : "memory");
+}
+
 __device__ __forceinline__ void sts16(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -311,20 +326,21 @@ __device__ __forceinline__ uint64_t seen_columns(const TreeArgs& p, int b, int n
   return ((uint64_t)hi << 32) | lo;
 }
 
-// Cache rows of positions pos0 + 32k + lane, k < 4, or -1 (reads as zeros); the
-// four block-table loads are in flight together.
+// Cache rows of positions pos0 + 32k + lane, k < N, or -1 (reads as zeros); the
+// block-table loads are in flight together.
+template <int N>
 __device__ __forceinline__ void row_codes(const TreeArgs& p, int b, const Req& r, uint64_t seen, int pos0, int lane,
-                                          int (&code)[4]) {
+                                          int (&code)[N]) {
   const int32_t* bt = p.bt + (int64_t)b * p.bt_stride;
-  int blk[4], page_row[4];
+  int blk[N], page_row[N];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < N; ++k) {
     const int pos = pos0 + 32 * k + lane;
     blk[k] = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page;
     page_row[k] = p.max_blocks > 0 ? __ldg(bt + min(blk[k], p.max_blocks - 1)) : -1;
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < N; ++k) {
     const int pos = pos0 + 32 * k + lane;
     const int j = pos - (r.seq - r.nd);
     const int64_t row = (int64_t)page_row[k] * p.page + (pos - blk[k] * p.page);
@@ -333,39 +349,56 @@ __device__ __forceinline__ void row_codes(const TreeArgs& p, int b, const Req& r
   }
 }
 
-// This CTA's 64 query rows into shared memory (f16, or bf16 as it is): warp w
-// rows 8w + lane / 8 and four on, eight lanes a row. qe[row]: the power of two
-// that a bf16 row was divided by.
+// This CTA's 64 query rows (f16, or bf16 as it is), by the producer warps: the last
+// three 64-column blocks into shared memory, the others by way of the K buffer,
+// which is free then, into tensor memory (twice, for its two lane halves). Warp w
+// loads rows 4w + lane / 8, eight lanes a row. qe[row]: the power of two that a
+// bf16 row was divided by.
 template <int FMT>
-__device__ __forceinline__ void load_q(const TreeArgs& p, uint32_t sm_q, int8_t* qe, int b, int row0, int w, int lane) {
-  const int l8 = lane & 7;
-#pragma unroll 1
-  for (int i = 0; i < 2; ++i) {
-    const int row = 8 * w + 4 * i + (lane >> 3);
-    const bool on = row0 + row < p.T * p.H;
-    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
-                                                      ((int64_t)b * p.T * p.H + row0 + row) * DK * 2);
-    int e = 0;
-    if (FMT != DSA_BF16 && p.q_bf16) {
-      uint32_t bits = 0;
-      if (on) {
+__device__ __forceinline__ void load_q(const TreeArgs& p, uint32_t base, uint32_t tmem, int8_t* qe, int b, int row0, int w,
+                                       int lane) {
+  const int row = 4 * w + (lane >> 3), l8 = lane & 7;
+  const bool on = row0 + row < p.T * p.H;
+  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
+                                                    ((int64_t)b * p.T * p.H + row0 + row) * DK * 2);
+  int e = 0;
+  if (FMT != DSA_BF16 && p.q_bf16) {
+    uint32_t bits = 0;
+    if (on) {
 #pragma unroll 3
-        for (int c = 0; c < 9; ++c) bits = max(bits, bf16x8_max_abs_bits(__ldg(src + l8 + 8 * c)));
-      }
-      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
-      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
-      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
-      e = bf16_fp16_shift(bits);
+      for (int c = 0; c < 9; ++c) bits = max(bits, bf16x8_max_abs_bits(__ldg(src + l8 + 8 * c)));
     }
-#pragma unroll 3
-    for (int c = 0; c < 9; ++c) {
-      uint4 v = on ? __ldg(src + l8 + 8 * c) : make_uint4(0, 0, 0, 0);
-      if (FMT != DSA_BF16 && p.q_bf16) v = bf16x8_to_half8_scaled(v, e);
-      v = make_uint4(v.x ^ p.q_sign, v.y ^ p.q_sign, v.z ^ p.q_sign, v.w ^ p.q_sign);
-      sts16(sm_q + c * kBlk + sw128_off(row, l8), v);
-    }
-    if (l8 == 0) qe[row] = (int8_t)e;
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
+    e = bf16_fp16_shift(bits);
   }
+#pragma unroll 3
+  for (int c = 0; c < 9; ++c) {
+    uint4 v = on ? __ldg(src + l8 + 8 * c) : make_uint4(0, 0, 0, 0);
+    if (FMT != DSA_BF16 && p.q_bf16) v = bf16x8_to_half8_scaled(v, e);
+    v = make_uint4(v.x ^ p.q_sign, v.y ^ p.q_sign, v.z ^ p.q_sign, v.w ^ p.q_sign);
+    sts16(base + (c < kQtBlks ? SM_K + c * kBlk : SM_Q + (c - kQtBlks) * kBlk) + sw128_off(row, l8), v);
+  }
+  if (l8 == 0) qe[row] = (int8_t)e;
+  named_bar(2, kProducers * 32);
+  // four warps a sub-partition: blocks w / 4 and w / 4 + 4
+  const int sp = w & 3, trow = (32 * sp + lane) & 63;
+#pragma unroll 1
+  for (int c = w >> 2; c < kQtBlks; c += 4) {
+    uint32_t r[32];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint4 v = lds16(base + SM_K + c * kBlk + sw128_off(trow, k));
+      r[4 * k] = v.x;
+      r[4 * k + 1] = v.y;
+      r[4 * k + 2] = v.z;
+      r[4 * k + 3] = v.w;
+    }
+    tmem_st32(tmem + ((uint32_t)(32 * sp) << 16) + Q_COL + 32 * c, r);
+  }
+  tmem_wait_st();
+  named_bar(2, kProducers * 32);  // the K buffer has been read
 }
 
 // FMT: the cache's format.
@@ -383,16 +416,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     return;
   }
   uint8_t* misc = sm + SM_MISC;
-  const uint32_t mb = smem_u32(misc);
+  const uint32_t mb = smem_u32(misc) + kBarAt;
   const uint32_t mb_k_full = mb, mb_k_free = mb + 8, mb_v_full = mb + 16, mb_v_free = mb + 24, mb_p_full = mb + 32,
-                 mb_o_free = mb + 40, mb_done = mb + 48, mb_s_full = mb + 56 /* [2] */, mb_q_full = mb + 72 /* [3] */,
-                 mb_r_full = mb + 96 /* [3] */, mb_r_free = mb + 120 /* [3] */;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 144);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 148);
-  int* run_tiles = reinterpret_cast<int*>(misc + 152);
+                 mb_o_free = mb + 40, mb_done = mb + 48, mb_s_full = mb + 56, mb_s_free = mb + 64,
+                 mb_q_full = mb + 72 /* [3] */, mb_r_full = mb + 96 /* [3] */, mb_r_free = mb + 120 /* [3] */;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + kWordsAt);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + kWordsAt + 4);
+  int* run_tiles = reinterpret_cast<int*>(misc + kWordsAt + 8);
+  uint32_t* raw_valid = reinterpret_cast<uint32_t*>(misc + kWordsAt + 16);  // [2]: rows that lie in the raw buffer
   int8_t* qe = reinterpret_cast<int8_t*>(misc + kQeAt);         // [kQeSegs][64]
   float* rowx = reinterpret_cast<float*>(misc + kRowxAt);       // [4][64]
-  int* ring = reinterpret_cast<int*>(misc + kRingAt);           // [kRing][128]
+  int* ring = reinterpret_cast<int*>(sm + SM_RING);             // [kRing][128]
   Segment* segs = reinterpret_cast<Segment*>(misc + kSegAt);    // [kSegs]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -402,18 +436,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   Cursor c{};  // the row warp's
   if (warp == 0) {
     if (lane == 0) {
-      mbar_init(mb_k_full, 2 * kKWarps);
+      mbar_init(mb_k_full, 2 * (kProducers + (kFp8 ? kTailWarps : 0)));
       mbar_init(mb_k_free, 1);
-      mbar_init(mb_v_full, 2 * kVWarps);
+      mbar_init(mb_v_full, 2 * kProducers);
       mbar_init(mb_v_free, 1);
       mbar_init(mb_p_full, 2 * kSoftmaxWarps);
       mbar_init(mb_o_free, 2 * kSoftmaxWarps);
       mbar_init(mb_done, 1);
-      for (int x = 0; x < 2; ++x) mbar_init(mb_s_full + 8 * x, 1);
-      for (int x = 0; x < kQeSegs; ++x) mbar_init(mb_q_full + 8 * x, kKWarps);
+      mbar_init(mb_s_full, 1);
+      mbar_init(mb_s_free, 2 * kSoftmaxWarps);
+      for (int x = 0; x < kQeSegs; ++x) mbar_init(mb_q_full + 8 * x, kProducers);
       for (int x = 0; x < kRing; ++x) {
         mbar_init(mb_r_full + 8 * x, 1);
-        mbar_init(mb_r_free + 8 * x, kKWarps + kVWarps + (kFp8 ? 0 : kFetchWarps));
+        mbar_init(mb_r_free + 8 * x, kProducers + kTailWarps);
       }
       mbar_init_fence();
       *abort_flag = 0;
@@ -431,6 +466,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   const uint32_t tmem = *tmem_slot;
   const int total = *run_tiles;
 
+  // 16 x 80 + 8 x 64 + 4 x 56 registers a lane: what the block's 28 warps of 72 were launched with
+  if (warp < kProducers)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
+  else if (warp < kMmaWarp)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  else
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   bool ok = true;
   // By a whole warp: `ok` stays uniform.
   auto wait = [&](uint32_t mbar, uint32_t parity) {
@@ -438,39 +480,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   };
   // After a wait that ran out (`ok` false, abort flag set) every thread still
   // executes its role's barriers and arrivals, and later waits return at once.
-  // rows of tile t, from the row warp: each reader of a slot frees it
-  auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
-  auto wait_rows = [&](int t) { wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1); };
-  auto free_rows = [&](int t) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
-  };
-  // what this warp has stored is the tensor cores' to read
-  auto announce = [&](uint32_t full_of_cta0) {
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) mbar_arrive_cluster(full_of_cta0);
-  };
-  // A lane of the expanding warps holds 16 neighbouring columns: chunks 2 (lane & 3)
-  // and the next of a 64-column block. Lanes of odd blocks store the second chunk
-  // first, so that the eight lanes of a store cover all banks.
-  const bool odd = (lane >> 2) & 1;
-  auto put16 = [&](auto how, uint32_t at, const uint4& v, float scale) {
-    constexpr int HOW = decltype(how)::value;
-    const uint4 d = make_uint4(pinned(v.x), pinned(v.y), pinned(v.z), pinned(v.w));
-    const Scale s(scale);
-    const uint4 first = dequant8<HOW>(odd ? make_uint2(d.z, d.w) : make_uint2(d.x, d.y), s);
-    const uint4 second = dequant8<HOW>(odd ? make_uint2(d.x, d.y) : make_uint2(d.z, d.w), s);
-    sts16(at, first);
-    sts16(at ^ 16, second);
-  };
-  auto all_fast = [](float f) { return __all_sync(0xffffffffu, fast_scale(f)); };
-
-  if (warp < kKWarps) {
-    // -------------------------------------------------------------- Q and K
-    // K(t+1) is stored under PV(t-1); its successor's loads have a tile's time to arrive.
+  if (warp < kProducers) {
+    // ------------------------------------------------------------- producers
+    // Per tile t: store K(t+1) (under PV(t-1)), store V(t) (under QK(t+1)), take tile t+2.
     const int w = warp;
-    const uint32_t k_full0 = cluster_map(mb_k_full, 0);
+    const uint32_t k_full0 = cluster_map(mb_k_full, 0), v_full0 = cluster_map(mb_v_full, 0);
     int kc = 0;             // K stores so far (two per tile in two-pass segments)
     int seg = 0, left = 0;  // the segment of the next K store, and its tiles left
     bool two = false;
@@ -478,218 +492,318 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     auto enter = [&]() {
       if (left > 0) return;
       const Segment& sg = segs[seg % kSegs];  // visible: the wait for this tile's rows
-      left = sg.n;
-      two = (sg.flags & kTwo) != 0;
-      if (ok) load_q<FMT>(p, base + SM_Q, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
+      const bool live = !named_bar_or(2, kProducers * 32, !ok);  // all take the same number of barriers
+      left = live ? sg.n : 1 << 30;
+      two = live && (sg.flags & kTwo) != 0;
+      if (live)
+        load_q<FMT>(p, base, tmem, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
+      ok = ok && live;
       __syncwarp();
       if (lane == 0) mbar_arrive(mb_q_full + 8 * (seg % kQeSegs));
       ++seg;
     };
     if constexpr (kFp8) {
-      // rows 8w + x, 16 codes a lane (a whole row a load: the fewest cache lines), 16
-      // bytes of the rotary tail of rows 8w + 4i + lane / 8, and scale lane & 3 of row
-      // 8w + lane / 4
-      uint4 d[8], tail[2];
-      float sc = 1.f;
-      auto load = [&](int t) {
-        wait_rows(t);
-        if (!ok) return;
-        const int* rows = rows_of(t) + 64 * rank + 8 * w;
-        const int4 c0 = *reinterpret_cast<const int4*>(rows), c1 = *reinterpret_cast<const int4*>(rows + 4);
-        const int t0 = rows[lane >> 3], t1 = rows[4 + (lane >> 3)], ts = rows[lane >> 2];
-        free_rows(t);
-        const int code[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      // This CTA's 64 keys land in shared memory as they lie in the cache (bulk
+      // copies of the row warp: loads would pass through an L1 of 28 KB and hold up
+      // the other accesses). Rows 4w + x are this warp's, 16 codes a lane; in
+      // registers they serve K of their tile and, a tile later, V.
+      uint4 kd[4], vd[4];
+      float ks[4], vs[4];  // the scale of the lane's group, by row
+      auto take = [&](int t) {
+        wait(mb_r_full, t & 1);
+        const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
+        const uint32_t raw = base + SM_RAW + 4 * w * 656;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          d[x] = ldg_nc16(fp8_row(p.kv, code[x]) + 16 * lane);
+        for (int x = 0; x < 4; ++x) {
+          kd[x] = lds16(raw + 656 * x + 16 * lane);
+          ks[x] = lds4(raw + 656 * x + 512 + 4 * (lane >> 3));
         }
-        sc = __ldg(reinterpret_cast<const float*>(fp8_row(p.kv, ts) + 512) + (lane & 3));
-        tail[0] = ldg_nc16(fp8_row(p.kv, t0) + 528 + 16 * (lane & 7));
-        tail[1] = ldg_nc16(fp8_row(p.kv, t1) + 528 + 16 * (lane & 7));
-      };
-      const uint32_t at = base + SM_K + (lane >> 2) * kBlk + sw128_off(8 * w, 2 * (lane & 3) + odd);
-      const uint32_t tail_at = base + SM_K + 8 * kBlk + sw128_off(8 * w + (lane >> 3), lane & 7);
-      auto put = [&](auto how) {
+        if ((valid & 15u) != 15u || !ok) {  // the others read as zeros
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          put16(how, (at ^ (16 * x)) + 128 * x, d[x], __shfl_sync(0xffffffffu, sc, 4 * x + (lane >> 3)));
+          for (int x = 0; x < 4; ++x)
+            if (!((valid >> x) & 1)) {
+              kd[x] = make_uint4(0, 0, 0, 0);
+              ks[x] = 1.f;
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_r_free);
       };
-      if (total > 0) load(0);
-#pragma unroll 1
-      for (int t = 0; t < total; ++t) {
+      // A lane's 16 columns are chunks 2 (lane & 3) and the next of 64-column block
+      // lane / 4; lanes of odd blocks store the second chunk first, so that the eight
+      // lanes of a store cover all banks. Row x further on moves the swizzle by x.
+      // (Formed anew for each use: kept, the addresses would not fit the registers.)
+      const bool odd = (lane >> 2) & 1;
+      auto k_row = [&]() {
+        const int l = (int)pinned(lane);
+        return base + SM_K + (l >> 2) * kBlk + sw128_off(4 * w, 2 * (l & 3) + ((l >> 2) & 1));
+      };
+      // V: columns below 256 are CTA 0's, the others CTA 1's
+      const bool mine = (lane >> 4) == rank;
+      auto v_row = [&]() {
+        const int l = (int)pinned(lane);
+        const uint32_t at =
+            base + SM_V + ((l >> 2) & 3) * kVBlk + sw128_off(64 * rank + 4 * w, 2 * (l & 3) + ((l >> 2) & 1));
+        return mine ? at : cluster_map(at, rank ^ 1);
+      };
+      auto expand = [&](auto how, const uint4& v, float scale, uint4& first, uint4& second) {
+        constexpr int HOW = decltype(how)::value;
+        const uint4 d = make_uint4(pinned(v.x), pinned(v.y), pinned(v.z), pinned(v.w));
+        const Scale s(scale);
+        first = dequant8<HOW>(odd ? make_uint2(d.z, d.w) : make_uint2(d.x, d.y), s);
+        second = dequant8<HOW>(odd ? make_uint2(d.x, d.y) : make_uint2(d.z, d.w), s);
+      };
+      auto put_k = [&](auto how) {
+        const uint32_t k_at = k_row();
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint4 first, second;
+          expand(how, kd[x], ks[x], first, second);
+          const uint32_t at = (k_at ^ (16 * x)) + 128 * x;
+          sts16(at, first);
+          sts16(at ^ 16, second);
+        }
+      };
+      auto put_v = [&](auto how) {
+        const uint32_t v_at = v_row();
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint4 first, second;
+          expand(how, vd[x], vs[x], first, second);
+          const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
+          if (mine) {
+            sts16(at, first);
+            sts16(at ^ 16, second);
+          } else {
+            sts16_cluster(at, first);
+            sts16_cluster(at ^ 16, second);
+          }
+        }
+      };
+      auto all_fast = [](const float (&f)[4]) {
+        return __all_sync(0xffffffffu, fast_scale(f[0]) && fast_scale(f[1]) && fast_scale(f[2]) && fast_scale(f[3]));
+      };
+      auto store_k = [&]() {
         if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
         enter();
         if (ok) {
           // two passes: the first rounds in f32, the second stores its remainder
-          if (!two && all_fast(sc))
-            put(std::integral_constant<int, kFast>());
+          if (!two && all_fast(ks))
+            put_k(std::integral_constant<int, kFast>());
           else
-            put(std::integral_constant<int, kWide>());
-          sts16(tail_at, tail[0]);
-          sts16((tail_at ^ 64) + 512, tail[1]);
+            put_k(std::integral_constant<int, kWide>());
         }
-        announce(k_full0);
+        fence_proxy_async();
+        fence_before_sync();  // Q's tensor-memory stores
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(k_full0);
         ++kc;
         if (two) {
           wait(mb_k_free, (kc - 1) & 1);
           if (ok) {
-            put(std::integral_constant<int, kRest>());
-            sts16(tail_at, make_uint4(0, 0, 0, 0));
-            sts16((tail_at ^ 64) + 512, make_uint4(0, 0, 0, 0));
+            put_k(std::integral_constant<int, kRest>());
           }
-          announce(k_full0);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(k_full0);
           ++kc;
         }
         --left;
-        if (t + 1 < total) load(t + 1);
+      };
+      auto pass_on = [&]() {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          vd[x] = kd[x];
+          vs[x] = ks[x];
+        }
+      };
+      if (total > 0) {
+        take(0);
+        store_k();
+        pass_on();
+        if (total > 1) take(1);
       }
-    } else {
-      const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
-        wait_rows(t);
-        int code[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) code[i] = ok ? rows_of(t)[64 * rank + 8 * w + 4 * i + r4] : -1;
-        free_rows(t);
+        if (t + 1 < total) store_k();
+        if (t > 0) wait(mb_v_free, (t - 1) & 1);
+        if (ok) {
+          if (all_fast(vs))
+            put_v(std::integral_constant<int, kFast>());
+          else
+            put_v(std::integral_constant<int, kWide>());
+        }
+        fence_proxy_async_all();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_release(v_full0);
+        if (t + 1 < total) pass_on();
+        if (t + 2 < total) take(t + 2);
+      }
+    } else {
+      // rows of tile t, from the row warp: each reader of a slot frees it
+      const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
+      auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
+      auto store_k = [&](int t) {
+        wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
+        const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
         if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
+        enter();
+        if (ok) {
+          const uint8_t* row = p.kv + (int64_t)max(code, 0) * kRowBytes + 16 * l8;
+#pragma unroll
+          for (int x = 0; x < 9; ++x)
+            cp_async16_zfill(base + SM_K + x * kBlk + sw128_off(4 * w + r4, l8), row + 128 * x, code >= 0);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(k_full0);
+        ++kc;
+        --left;
+      };
+      if (total > 0) store_k(0);
+#pragma unroll 1
+      for (int t = 0; t < total; ++t) {
+        if (t + 1 < total) store_k(t + 1);
+        int code[2];
+        code[0] = ok ? rows_of(t)[8 * w + r4] : -1;
+        code[1] = ok ? rows_of(t)[8 * w + r4 + 4] : -1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
+        if (t > 0) wait(mb_v_free, (t - 1) & 1);
         if (ok) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint8_t* row = p.kv + (int64_t)max(code[i], 0) * kRowBytes + 16 * l8;
-#pragma unroll
-            for (int x = 0; x < 9; ++x)
-              cp_async16_zfill(base + SM_K + x * kBlk + sw128_off(8 * w + 4 * i + r4, l8), row + 128 * x, code[i] >= 0);
-          }
-        }
-        cp_async_commit();
-        enter();
-        cp_async_wait<0>();
-        announce(k_full0);
-        ++kc;
-        --left;
-      }
-    }
-  } else if (warp < kKWarps + kVWarps) {
-    // -------------------------------------------------------------------- V
-    // This CTA's 256 columns of all 128 keys; V(t) is stored under QK(t+1).
-    const int w = warp - kKWarps;
-    const uint32_t v_full0 = cluster_map(mb_v_full, 0);
-    if constexpr (kFp8) {
-      uint4 d[8];      // rows 16w + 2x + lane / 16
-      float sc = 1.f;  // of row 16w + lane / 2, group 2 rank + (lane & 1)
-      auto load = [&](int t) {
-        wait_rows(t);
-        if (!ok) return;
-        const int* rows = rows_of(t) + 16 * w;
-        int code[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) code[x] = rows[2 * x + (lane >> 4)];
-        const int ts = rows[lane >> 1];
-        free_rows(t);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) d[x] = ldg_nc16(fp8_row(p.kv, code[x]) + 256 * rank + 16 * (lane & 15));
-        sc = __ldg(reinterpret_cast<const float*>(fp8_row(p.kv, ts) + 512) + 2 * rank + (lane & 1));
-      };
-      const uint32_t at =
-          base + SM_V + ((lane >> 2) & 3) * kVBlk + sw128_off(16 * w + (lane >> 4), 2 * (lane & 3) + odd);
-      auto put = [&](auto how) {
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-          put16(how, (at ^ (32 * (x & 3))) + 256 * (x & 3) + 1024 * (x >> 2), d[x],
-                __shfl_sync(0xffffffffu, sc, 4 * x + 2 * (lane >> 4) + ((lane >> 3) & 1)));
-      };
-      if (total > 0) load(0);
-#pragma unroll 1
-      for (int t = 0; t < total; ++t) {
-        if (t > 0) wait(mb_v_free, (t - 1) & 1);
-        if (ok) {
-          if (all_fast(sc))
-            put(std::integral_constant<int, kFast>());
-          else
-            put(std::integral_constant<int, kWide>());
-        }
-        announce(v_full0);
-        if (t + 1 < total) load(t + 1);
-      }
-    } else {
-      const int r4 = lane >> 3, l8 = lane & 7;
-#pragma unroll 1
-      for (int t = 0; t < total; ++t) {
-        wait_rows(t);
-        int code[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) code[i] = ok ? rows_of(t)[16 * w + 4 * i + r4] : -1;
-        free_rows(t);
-        if (t > 0) wait(mb_v_free, (t - 1) & 1);
-        if (ok) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
             const uint8_t* row = p.kv + (int64_t)max(code[i], 0) * kRowBytes + 512 * rank + 16 * l8;
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              cp_async16_zfill(base + SM_V + x * kVBlk + sw128_off(16 * w + 4 * i + r4, l8), row + 128 * x, code[i] >= 0);
+              cp_async16_zfill(base + SM_V + x * kVBlk + sw128_off(8 * w + 4 * i + r4, l8), row + 128 * x, code[i] >= 0);
           }
         }
         cp_async_commit();
         cp_async_wait<0>();
-        announce(v_full0);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(v_full0);
       }
     }
   } else if (warp == kRowWarp) {
     // ------------------------------------------------------ rows of the tiles
-    // Block table -> cache row of each key, kRing tiles ahead.
+    // Block table -> cache rows: for 16-bit caches of all keys into the ring, kRing
+    // tiles ahead; for fp8 of this CTA's keys, which are copied into the raw buffer
+    // when the tile before has been taken, and fetched into L2 before that.
     uint64_t seen = 0;
     int seg = 0;
 #pragma unroll 1
     for (int t = 0; t < total; ++t) {
       if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
-      int code[4];
-      row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
+      constexpr int kParts = kFp8 ? 2 : 4;
+      int code[kParts];
+      row_codes<kParts>(p, c.b, c.r, seen, c.tile * kKeys + (kFp8 ? 64 * rank : 0), lane, code);
+      bool run[kParts];  // 32 neighbouring rows: one copy
       if constexpr (kFp8) {
-        // this CTA's half into L2: neighbouring rows as one run
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int mine = rank ? code[2 + k] : code[k];
-          const int head = __shfl_sync(0xffffffffu, mine, 0);
-          if (__all_sync(0xffffffffu, mine >= 0 && mine == head + lane)) {
-            if (lane == 0) prefetch_l2(p.kv + (int64_t)mine * kRowBytes, 32 * kRowBytes);
-          } else if (mine >= 0) {
-            prefetch_l2(p.kv + (int64_t)mine * kRowBytes, kRowBytes);
-          }
+        for (int k = 0; k < kParts; ++k) {
+          const int head = __shfl_sync(0xffffffffu, code[k], 0);
+          run[k] = __all_sync(0xffffffffu, code[k] >= 0 && code[k] == head + lane);
         }
       }
-      if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
-      if (ok) {
+      const int slot = kFp8 ? 0 : t % kRing, turn = kFp8 ? t : t / kRing;
+      if (turn > 0) wait(mb_r_free + 8 * slot, (turn - 1) & 1);
+      if (ok && c.first && lane == 0) {
+        Segment sg;
+        sg.b = c.b;
+        sg.rt = c.rt;
+        sg.n = min(c.r.nt - c.tile, c.left);
+        sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
+        sg.nd = c.r.nd;
+        sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
+        segs[seg % kSegs] = sg;
+      }
+      if constexpr (kFp8) {
+        uint32_t bytes = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
-        if (c.first && lane == 0) {
-          Segment sg;
-          sg.b = c.b;
-          sg.rt = c.rt;
-          sg.n = min(c.r.nt - c.tile, c.left);
-          sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
-          sg.nd = c.r.nd;
-          sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
-          segs[seg % kSegs] = sg;
+        for (int k = 0; k < kParts; ++k) {
+          const uint32_t valid = __ballot_sync(0xffffffffu, code[k] >= 0);
+          bytes += __popc(valid) * kRowBytes;
+          if (ok && lane == 0) raw_valid[k] = valid;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(mb_r_full, ok ? bytes : 0u);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < kParts; ++k)
+          if (ok && (run[k] ? lane == 0 : code[k] >= 0))
+            bulk_load(base + SM_RAW + (32 * k + lane) * kRowBytes, p.kv + (int64_t)code[k] * kRowBytes,
+                      (run[k] ? 32 : 1) * kRowBytes, mb_r_full);
+      } else {
+        if (ok) {
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) ring[slot * kKeys + 32 * k + lane] = code[k];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_r_full + 8 * slot);
       }
       if (c.first) ++seg;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(mb_r_full + 8 * (t % kRing));
       c.next(p);
     }
-  } else if (!kFp8 && warp >= kFetch0) {
-    // 16-bit rows go to shared memory when their buffer is free, without a stop in
-    // registers: these warps bring this CTA's half of the tile's keys into L2 (the
-    // other CTA brings the rest of V's).
+  } else if (warp >= kTail0) {
+    const int w = warp - kTail0;
+    if constexpr (kFp8) {
+      // ------------------------------------------------- rotary part of K
+      // Rows 32w + 4x + lane / 8, 16 bytes a lane: copied, they are 16-bit in the cache.
+      const uint32_t k_full0 = cluster_map(mb_k_full, 0);
+      int kc = 0, seg = 0, left = 0;
+      bool two = false;
 #pragma unroll 1
-    for (int t = 0; t < total; ++t) {
-      wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
-      const int code = ok ? ring[(t % kRing) * kKeys + 64 * rank + 32 * (warp - kFetch0) + lane] : -1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
-      if (code >= 0) prefetch_l2(p.kv + (int64_t)code * kRowBytes, kRowBytes);
+      for (int t = 0; t < total; ++t) {
+        wait(mb_r_full, t & 1);
+        uint4 d[8];
+        const uint32_t raw = base + SM_RAW + (32 * w + (lane >> 3)) * 656 + 528 + 16 * (lane & 7);
+        const uint32_t valid = raw_valid[w] >> (lane >> 3);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          d[x] = lds16(raw + 4 * 656 * x);
+          if (!((valid >> (4 * x)) & 1)) d[x] = make_uint4(0, 0, 0, 0);
+        }
+        if (left == 0 && ok) {
+          left = segs[seg % kSegs].n;
+          two = (segs[seg % kSegs].flags & kTwo) != 0;
+          ++seg;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_r_free);
+#pragma unroll 1
+        for (int s = 0; s < (two ? 2 : 1); ++s) {
+          if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
+          // Q passes through the K buffer's other blocks only
+          if (ok) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              sts16(base + SM_K + 8 * kBlk + sw128_off(32 * w + 4 * x + (lane >> 3), lane & 7),
+                    s > 0 ? make_uint4(0, 0, 0, 0) : d[x]);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(k_full0);
+          ++kc;
+        }
+        --left;
+      }
+    } else {
+      // 16-bit rows go to shared memory when their buffer is free, without a stop in
+      // registers: these warps bring this CTA's half of the tile's keys into L2 (the
+      // other CTA brings the rest of V's).
+#pragma unroll 1
+      for (int t = 0; t < total; ++t) {
+        wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
+        const int code = ok ? ring[(t % kRing) * kKeys + 64 * rank + 32 * w + lane] : -1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
+        if (code >= 0) prefetch_l2(p.kv + (int64_t)code * kRowBytes, kRowBytes);
+      }
     }
   } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------- MMA issue
@@ -711,18 +825,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
             passes = segs[qseg % kSegs].flags & kTwo ? 2 : 1;
             ++qseg;
           }
+          if (s == 0 && gq > 0) {  // the softmax has read S(gq - 1)
+            ok = ok && mbar_wait_lazy(mb_s_free, (gq - 1) & 1, abort_flag, err, kWaitNs);
+            if (!ok) return;
+          }
           fence_after_sync();
           const uint64_t dq = desc(SM_Q, 16), dk = desc(SM_K, 16);
 #pragma unroll
           for (int kb = 0; kb < 9; ++kb)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_f16_ss_pair(tmem + S_COL + 64 * (gq & 1), dq + ((kb * kBlk + 32 * k) >> 4),
-                              dk + ((kb * kBlk + 32 * k) >> 4), IDESC_QK, (kb | k) != 0 || s > 0);
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t b = dk + ((kb * kBlk + 32 * k) >> 4);
+              if (kb < kQtBlks)
+                mma_f16_ts_pair(tmem + S_COL, tmem + Q_COL + 32 * kb + 8 * k, b, IDESC_QK, (kb | k) != 0 || s > 0);
+              else
+                mma_f16_ss_pair(tmem + S_COL, dq + (((kb - kQtBlks) * kBlk + 32 * k) >> 4), b, IDESC_QK, 1);
+            }
           mma_commit_pair(mb_k_free);
           ++kc;
         }
-        mma_commit_pair(mb_s_full + 8 * (gq & 1));
+        mma_commit_pair(mb_s_full);
         --qleft;
         ++gq;
       };
@@ -732,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       for (int g = 0; g < total && ok; ++g) {
         if (g + 1 < total) qk();
         const bool first = pleft == 0;
-        ok = ok && mbar_wait_lazy(mb_v_full, g & 1, abort_flag, err, kWaitNs) &&
+        ok = ok && mbar_wait_lazy<true>(mb_v_full, g & 1, abort_flag, err, kWaitNs) &&
              mbar_wait_lazy(mb_p_full, g & 1, abort_flag, err, kWaitNs);
         if (first) {
           // the accumulator of the segment before has been read
@@ -764,7 +886,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     const int q4 = 2 * (sp >> 1) + hh;          // this thread's quarter of the row's keys
     const int kofs = 64 * (sp >> 1) + 32 * hh;  // its first key
     const uint32_t t_sp = tmem + ((uint32_t)(32 * sp) << 16);
-    const uint32_t p_full0 = cluster_map(mb_p_full, 0), o_free0 = cluster_map(mb_o_free, 0);
+    const uint32_t p_full0 = cluster_map(mb_p_full, 0), o_free0 = cluster_map(mb_o_free, 0),
+                   s_free0 = cluster_map(mb_s_free, 0);
     uint8_t* prow = sm + SM_P + (sp >> 1) * kBlk;
     int g = 0;
 #pragma unroll 1
@@ -790,16 +913,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           allow |= (uint32_t)(d >= 0 ? bits << d : bits >> -d);
         }
         d = max(d - kKeys, -64);
-        wait(mb_s_full + 8 * (g & 1), (g >> 1) & 1);
+        wait(mb_s_full, g & 1);
         fence_after_sync();
         uint32_t s[32];
         if (ok) {
-          tmem_ld32(t_sp + S_COL + 64 * (g & 1) + 32 * hh, s);
+          tmem_ld32(t_sp + S_COL + 32 * hh, s);
           tmem_wait_ld();
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) s[j] = 0u;
         }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(s_free0);
         if (allow != 0xffffffffu) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;  // -inf
