@@ -320,32 +320,13 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mbar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
-// The same with a cluster-scope release: for writes into the other CTA's shared memory.
-__device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t mbar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
-}
-// Order this thread's generic-proxy writes, to whatever memory, before later async-proxy reads.
-__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t mbar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred P1;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, P1;\n\t}"
-      : "=r"(ok)
-      : "r"(mbar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // mbar_wait that reads the clock only once a wait has become long: the first
 // test of globaltimer costs about a microsecond, more than most waits here.
-// kCluster: acquires what the other CTA released.
-template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait_lazy(uint32_t mbar, uint32_t parity, volatile int* abort, int32_t* err,
                                                uint64_t timeout_ns) {
   uint64_t t0 = 0;
   for (uint32_t it = 1;; ++it) {
-    if (kCluster ? mbar_try_wait_cluster(mbar, parity) : mbar_try_wait(mbar, parity)) return true;
+    if (mbar_try_wait(mbar, parity)) return true;
     if ((it & 63u) == 0) {
       if (*abort) return false;
       const uint64_t t = globaltimer_ns();

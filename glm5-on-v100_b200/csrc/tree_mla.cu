@@ -65,7 +65,7 @@ constexpr int kProducers = 16;  // warps 0-15
 constexpr int kSoftmax0 = 16, kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 24, kRowWarp = 25;
 constexpr int kTail0 = 26, kTailWarps = 2;  // fp8: the rotary part of K; 16-bit: L2 prefetch
-constexpr int kRing = 3;        // 16-bit caches: tiles whose cache rows are known ahead
+constexpr int kRing = 3;        // tiles whose cache rows are known ahead
 constexpr int kThreads = 28 * 32;
 constexpr uint32_t kBlk = 64 * 128;    // 64 rows x 64 16-bit values: 8 KB
 constexpr uint32_t kVBlk = 128 * 128;  // 128 keys x 64 columns: 16 KB
@@ -75,7 +75,7 @@ constexpr uint32_t SM_K = SM_Q + (9 - kQtBlks) * kBlk;
 constexpr uint32_t SM_V = SM_K + 9 * kBlk;
 constexpr uint32_t SM_P = SM_V + 4 * kVBlk;
 constexpr uint32_t SM_RAW = SM_P + 2 * kBlk;       // fp8: this CTA's 64 cache rows as they lie in the cache
-constexpr uint32_t SM_RING = SM_RAW + 64 * 656;    // 16-bit: rows[kRing][128]
+constexpr uint32_t SM_RING = SM_RAW + 64 * 656;    // rows[kRing][128]
 constexpr uint32_t SM_MISC = SM_RING + kRing * kKeys * 4;
 constexpr int kSegs = 6;        // segment descriptors kept: the row warp is at most five tiles ahead of an epilogue
 constexpr int kQeSegs = 3;      // Q is at most two segments ahead of the softmax
@@ -297,9 +297,16 @@ __device__ __forceinline__ float lds4(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ void sts16_cluster(uint32_t addr, const uint4& v) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-               : "memory");
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ uint2 ldg_nc8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
 }
 
 // Bytes of global memory (both 16-byte aligned, a multiple of 16) into this CTA's shared memory.
@@ -326,21 +333,20 @@ __device__ __forceinline__ uint64_t seen_columns(const TreeArgs& p, int b, int n
   return ((uint64_t)hi << 32) | lo;
 }
 
-// Cache rows of positions pos0 + 32k + lane, k < N, or -1 (reads as zeros); the
+// Cache rows of positions pos0 + 32k + lane, k < 4, or -1 (reads as zeros); the
 // block-table loads are in flight together.
-template <int N>
 __device__ __forceinline__ void row_codes(const TreeArgs& p, int b, const Req& r, uint64_t seen, int pos0, int lane,
-                                          int (&code)[N]) {
+                                          int (&code)[4]) {
   const int32_t* bt = p.bt + (int64_t)b * p.bt_stride;
-  int blk[N], page_row[N];
+  int blk[4], page_row[4];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
+  for (int k = 0; k < 4; ++k) {
     const int pos = pos0 + 32 * k + lane;
     blk[k] = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page;
     page_row[k] = p.max_blocks > 0 ? __ldg(bt + min(blk[k], p.max_blocks - 1)) : -1;
   }
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
+  for (int k = 0; k < 4; ++k) {
     const int pos = pos0 + 32 * k + lane;
     const int j = pos - (r.seq - r.nd);
     const int64_t row = (int64_t)page_row[k] * p.page + (pos - blk[k] * p.page);
@@ -385,17 +391,17 @@ __device__ __forceinline__ void load_q(const TreeArgs& p, uint32_t base, uint32_
   // four warps a sub-partition: blocks w / 4 and w / 4 + 4
   const int sp = w & 3, trow = (32 * sp + lane) & 63;
 #pragma unroll 1
-  for (int c = w >> 2; c < kQtBlks; c += 4) {
-    uint32_t r[32];
+  for (int c = 2 * (w >> 2); c < 2 * kQtBlks; c += (c & 1) ? 7 : 1) {  // half blocks: 32 columns of Q
+    uint32_t r[16];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint4 v = lds16(base + SM_K + c * kBlk + sw128_off(trow, k));
+    for (int k = 0; k < 4; ++k) {
+      const uint4 v = lds16(base + SM_K + (c >> 1) * kBlk + sw128_off(trow, 4 * (c & 1) + k));
       r[4 * k] = v.x;
       r[4 * k + 1] = v.y;
       r[4 * k + 2] = v.z;
       r[4 * k + 3] = v.w;
     }
-    tmem_st32(tmem + ((uint32_t)(32 * sp) << 16) + Q_COL + 32 * c, r);
+    tmem_st16(tmem + ((uint32_t)(32 * sp) << 16) + Q_COL + 16 * c, r);
   }
   tmem_wait_st();
   named_bar(2, kProducers * 32);  // the K buffer has been read
@@ -419,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   const uint32_t mb = smem_u32(misc) + kBarAt;
   const uint32_t mb_k_full = mb, mb_k_free = mb + 8, mb_v_full = mb + 16, mb_v_free = mb + 24, mb_p_full = mb + 32,
                  mb_o_free = mb + 40, mb_done = mb + 48, mb_s_full = mb + 56, mb_s_free = mb + 64,
-                 mb_q_full = mb + 72 /* [3] */, mb_r_full = mb + 96 /* [3] */, mb_r_free = mb + 120 /* [3] */;
+                 mb_q_full = mb + 72 /* [3] */, mb_r_full = mb + 96 /* [3] */, mb_r_free = mb + 120 /* [3] */,
+                 mb_raw_full = mb + 144, mb_raw_free = mb + 152;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + kWordsAt);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + kWordsAt + 4);
   int* run_tiles = reinterpret_cast<int*>(misc + kWordsAt + 8);
@@ -448,8 +455,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       for (int x = 0; x < kQeSegs; ++x) mbar_init(mb_q_full + 8 * x, kProducers);
       for (int x = 0; x < kRing; ++x) {
         mbar_init(mb_r_full + 8 * x, 1);
-        mbar_init(mb_r_free + 8 * x, kProducers + kTailWarps);
+        mbar_init(mb_r_free + 8 * x, kProducers + (kFp8 ? 0 : kTailWarps));
       }
+      mbar_init(mb_raw_full, 1);
+      mbar_init(mb_raw_free, kProducers + kTailWarps);
       mbar_init_fence();
       *abort_flag = 0;
     }
@@ -466,13 +475,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   const uint32_t tmem = *tmem_slot;
   const int total = *run_tiles;
 
-  // 16 x 80 + 8 x 64 + 4 x 56 registers a lane: what the block's 28 warps of 72 were launched with
-  if (warp < kProducers)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
-  else if (warp < kMmaWarp)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   bool ok = true;
   // By a whole warp: `ok` stays uniform.
   auto wait = [&](uint32_t mbar, uint32_t parity) {
@@ -502,93 +504,86 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (lane == 0) mbar_arrive(mb_q_full + 8 * (seg % kQeSegs));
       ++seg;
     };
+    auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
+    auto free_rows = [&](int t) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
+    };
     if constexpr (kFp8) {
-      // This CTA's 64 keys land in shared memory as they lie in the cache (bulk
-      // copies of the row warp: loads would pass through an L1 of 28 KB and hold up
-      // the other accesses). Rows 4w + x are this warp's, 16 codes a lane; in
-      // registers they serve K of their tile and, a tile later, V.
-      uint4 kd[4], vd[4];
-      float ks[4], vs[4];  // the scale of the lane's group, by row
+      // This CTA's 64 keys land in shared memory as they lie in the cache, by bulk
+      // copies: loads would go through an L1 of 28 KB, whose lines they fill faster
+      // than they arrive. Rows 4w + x are this warp's. A lane takes 8 codes of each
+      // half row, which is one 16-byte chunk of f16, so a store writes whole 128-byte
+      // rows of four 64-column blocks. In registers a tile's codes serve K and, a tile
+      // later, the half of V that is this CTA's columns of its own keys; those of the
+      // other CTA's keys (V: 64 x 256 codes) are loaded a tile ahead.
+      uint2 kd[4][2], vd[4], pd[4];  // [row][half] | own rows | the other CTA's rows
+      // scales: lane 4x + g < 16 holds row x, group g; of the other CTA's rows lane
+      // 2x + g < 8, of this CTA's columns
+      float ks = 1.f, vs = 1.f, ps = 1.f;
       auto take = [&](int t) {
-        wait(mb_r_full, t & 1);
+        wait(mb_raw_full, t & 1);
         const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
         const uint32_t raw = base + SM_RAW + 4 * w * 656;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          kd[x] = lds16(raw + 656 * x + 16 * lane);
-          ks[x] = lds4(raw + 656 * x + 512 + 4 * (lane >> 3));
-        }
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) kd[x][h] = lds8(raw + 656 * x + 256 * h + 8 * lane);
+        ks = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
         if ((valid & 15u) != 15u || !ok) {  // the others read as zeros
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            if (!((valid >> x) & 1)) {
-              kd[x] = make_uint4(0, 0, 0, 0);
-              ks[x] = 1.f;
-            }
+            if (!((valid >> x) & 1)) kd[x][0] = kd[x][1] = make_uint2(0, 0);
+          if (!((valid >> ((lane >> 2) & 3)) & 1)) ks = 1.f;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(mb_r_free);
+        if (lane == 0) mbar_arrive(mb_raw_free);
       };
-      // A lane's 16 columns are chunks 2 (lane & 3) and the next of 64-column block
-      // lane / 4; lanes of odd blocks store the second chunk first, so that the eight
-      // lanes of a store cover all banks. Row x further on moves the swizzle by x.
-      // (Formed anew for each use: kept, the addresses would not fit the registers.)
-      const bool odd = (lane >> 2) & 1;
-      auto k_row = [&]() {
-        const int l = (int)pinned(lane);
-        return base + SM_K + (l >> 2) * kBlk + sw128_off(4 * w, 2 * (l & 3) + ((l >> 2) & 1));
-      };
-      // V: columns below 256 are CTA 0's, the others CTA 1's
-      const bool mine = (lane >> 4) == rank;
-      auto v_row = [&]() {
-        const int l = (int)pinned(lane);
-        const uint32_t at =
-            base + SM_V + ((l >> 2) & 3) * kVBlk + sw128_off(64 * rank + 4 * w, 2 * (l & 3) + ((l >> 2) & 1));
-        return mine ? at : cluster_map(at, rank ^ 1);
-      };
-      auto expand = [&](auto how, const uint4& v, float scale, uint4& first, uint4& second) {
-        constexpr int HOW = decltype(how)::value;
-        const uint4 d = make_uint4(pinned(v.x), pinned(v.y), pinned(v.z), pinned(v.w));
-        const Scale s(scale);
-        first = dequant8<HOW>(odd ? make_uint2(d.z, d.w) : make_uint2(d.x, d.y), s);
-        second = dequant8<HOW>(odd ? make_uint2(d.x, d.y) : make_uint2(d.z, d.w), s);
-      };
-      auto put_k = [&](auto how) {
-        const uint32_t k_at = k_row();
+      auto load_others = [&](int t) {
+        wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
+        if (!ok) return;
+        const int* rows = rows_of(t) + 64 * (rank ^ 1) + 4 * w;
+        const int4 c = *reinterpret_cast<const int4*>(rows);
+        const int cs = rows[(lane >> 1) & 3];
+        free_rows(t);
+        const int code[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          uint4 first, second;
-          expand(how, kd[x], ks[x], first, second);
-          const uint32_t at = (k_at ^ (16 * x)) + 128 * x;
-          sts16(at, first);
-          sts16(at ^ 16, second);
+          pd[x] = make_uint2(0, 0);
+          if (code[x] >= 0) pd[x] = ldg_nc8(p.kv + (int64_t)code[x] * kRowBytes + 256 * rank + 8 * lane);
         }
+        ps = 1.f;
+        if (lane < 8 && cs >= 0)
+          ps = __ldg(reinterpret_cast<const float*>(p.kv + (int64_t)cs * kRowBytes + 512) + 2 * rank + (lane & 1));
+      };
+      auto expand = [&](auto how, const uint2& v, float scale) {
+        return dequant8<decltype(how)::value>(make_uint2(pinned(v.x), pinned(v.y)), Scale(scale));
+      };
+      // chunk lane & 7 of block lane / 8, row 4w: row x further on moves the swizzle by x
+      const uint32_t k_at = base + SM_K + (lane >> 3) * kBlk + sw128_off(4 * w, lane & 7);
+      const uint32_t v_at = base + SM_V + (lane >> 3) * kVBlk + sw128_off(4 * w, lane & 7);
+      auto put_k = [&](auto how) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            sts16((k_at ^ (16 * x)) + 128 * x + 4 * h * kBlk,
+                  expand(how, kd[x][h], __shfl_sync(0xffffffffu, ks, 4 * x + 2 * h + (lane >> 4))));
       };
       auto put_v = [&](auto how) {
-        const uint32_t v_at = v_row();
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          uint4 first, second;
-          expand(how, vd[x], vs[x], first, second);
           const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
-          if (mine) {
-            sts16(at, first);
-            sts16(at ^ 16, second);
-          } else {
-            sts16_cluster(at, first);
-            sts16_cluster(at ^ 16, second);
-          }
+          sts16(at + 8192 * rank, expand(how, vd[x], __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4))));
+          sts16(at + 8192 * (rank ^ 1), expand(how, pd[x], __shfl_sync(0xffffffffu, ps, 2 * x + (lane >> 4))));
         }
-      };
-      auto all_fast = [](const float (&f)[4]) {
-        return __all_sync(0xffffffffu, fast_scale(f[0]) && fast_scale(f[1]) && fast_scale(f[2]) && fast_scale(f[3]));
       };
       auto store_k = [&]() {
         if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
         enter();
         if (ok) {
           // two passes: the first rounds in f32, the second stores its remainder
-          if (!two && all_fast(ks))
+          if (!two && __all_sync(0xffffffffu, fast_scale(ks)))
             put_k(std::integral_constant<int, kFast>());
           else
             put_k(std::integral_constant<int, kWide>());
@@ -600,9 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         ++kc;
         if (two) {
           wait(mb_k_free, (kc - 1) & 1);
-          if (ok) {
-            put_k(std::integral_constant<int, kRest>());
-          }
+          if (ok) put_k(std::integral_constant<int, kRest>());
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(k_full0);
@@ -612,13 +605,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       };
       auto pass_on = [&]() {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          vd[x] = kd[x];
-          vs[x] = ks[x];
-        }
+        for (int x = 0; x < 4; ++x) vd[x] = rank ? kd[x][1] : kd[x][0];
+        vs = ks;
       };
       if (total > 0) {
         take(0);
+        load_others(0);
         store_k();
         pass_on();
         if (total > 1) take(1);
@@ -628,21 +620,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (t + 1 < total) store_k();
         if (t > 0) wait(mb_v_free, (t - 1) & 1);
         if (ok) {
-          if (all_fast(vs))
+          if (__all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps)))
             put_v(std::integral_constant<int, kFast>());
           else
             put_v(std::integral_constant<int, kWide>());
         }
-        fence_proxy_async_all();
+        fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_release(v_full0);
-        if (t + 1 < total) pass_on();
+        if (lane == 0) mbar_arrive_cluster(v_full0);
+        if (t + 1 < total) {
+          pass_on();
+          load_others(t + 1);
+        }
         if (t + 2 < total) take(t + 2);
       }
     } else {
-      // rows of tile t, from the row warp: each reader of a slot frees it
       const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
-      auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
       auto store_k = [&](int t) {
         wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
         const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
@@ -670,8 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         int code[2];
         code[0] = ok ? rows_of(t)[8 * w + r4] : -1;
         code[1] = ok ? rows_of(t)[8 * w + r4 + 4] : -1;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
+        free_rows(t);
         if (t > 0) wait(mb_v_free, (t - 1) & 1);
         if (ok) {
 #pragma unroll
@@ -691,60 +683,52 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     }
   } else if (warp == kRowWarp) {
     // ------------------------------------------------------ rows of the tiles
-    // Block table -> cache rows: for 16-bit caches of all keys into the ring, kRing
-    // tiles ahead; for fp8 of this CTA's keys, which are copied into the raw buffer
-    // when the tile before has been taken, and fetched into L2 before that.
+    // Block table -> cache rows into the ring, kRing tiles ahead; fp8: this CTA's keys
+    // are copied into the raw buffer when the tile before has been taken.
     uint64_t seen = 0;
     int seg = 0;
 #pragma unroll 1
     for (int t = 0; t < total; ++t) {
       if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
-      constexpr int kParts = kFp8 ? 2 : 4;
-      int code[kParts];
-      row_codes<kParts>(p, c.b, c.r, seen, c.tile * kKeys + (kFp8 ? 64 * rank : 0), lane, code);
-      bool run[kParts];  // 32 neighbouring rows: one copy
-      if constexpr (kFp8) {
+      int code[4];
+      row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
+      if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
+      if (ok) {
 #pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-          const int head = __shfl_sync(0xffffffffu, code[k], 0);
-          run[k] = __all_sync(0xffffffffu, code[k] >= 0 && code[k] == head + lane);
+        for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
+        if (c.first && lane == 0) {
+          Segment sg;
+          sg.b = c.b;
+          sg.rt = c.rt;
+          sg.n = min(c.r.nt - c.tile, c.left);
+          sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
+          sg.nd = c.r.nd;
+          sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
+          segs[seg % kSegs] = sg;
         }
       }
-      const int slot = kFp8 ? 0 : t % kRing, turn = kFp8 ? t : t / kRing;
-      if (turn > 0) wait(mb_r_free + 8 * slot, (turn - 1) & 1);
-      if (ok && c.first && lane == 0) {
-        Segment sg;
-        sg.b = c.b;
-        sg.rt = c.rt;
-        sg.n = min(c.r.nt - c.tile, c.left);
-        sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
-        sg.nd = c.r.nd;
-        sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
-        segs[seg % kSegs] = sg;
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb_r_full + 8 * (t % kRing));
       if constexpr (kFp8) {
-        uint32_t bytes = 0;
+        if (t > 0) wait(mb_raw_free, (t - 1) & 1);
+        uint32_t valid[2];
 #pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-          const uint32_t valid = __ballot_sync(0xffffffffu, code[k] >= 0);
-          bytes += __popc(valid) * kRowBytes;
-          if (ok && lane == 0) raw_valid[k] = valid;
+        for (int k = 0; k < 2; ++k) {
+          valid[k] = __ballot_sync(0xffffffffu, (rank ? code[2 + k] : code[k]) >= 0);
+          if (ok && lane == 0) raw_valid[k] = valid[k];
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(mb_r_full, ok ? bytes : 0u);
+        if (lane == 0) mbar_arrive_expect_tx(mb_raw_full, ok ? (__popc(valid[0]) + __popc(valid[1])) * kRowBytes : 0);
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < kParts; ++k)
-          if (ok && (run[k] ? lane == 0 : code[k] >= 0))
-            bulk_load(base + SM_RAW + (32 * k + lane) * kRowBytes, p.kv + (int64_t)code[k] * kRowBytes,
-                      (run[k] ? 32 : 1) * kRowBytes, mb_r_full);
-      } else {
-        if (ok) {
-#pragma unroll
-          for (int k = 0; k < kParts; ++k) ring[slot * kKeys + 32 * k + lane] = code[k];
+        for (int k = 0; k < 2; ++k) {
+          const int mine = rank ? code[2 + k] : code[k];
+          // 32 neighbouring rows are one copy
+          const int head = __shfl_sync(0xffffffffu, mine, 0);
+          const bool run = __all_sync(0xffffffffu, mine >= 0 && mine == head + lane);
+          if (ok && (run ? lane == 0 : mine >= 0))
+            bulk_load(base + SM_RAW + (32 * k + lane) * kRowBytes, p.kv + (int64_t)mine * kRowBytes,
+                      (run ? 32 : 1) * kRowBytes, mb_raw_full);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mb_r_full + 8 * slot);
       }
       if (c.first) ++seg;
       c.next(p);
@@ -759,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       bool two = false;
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
-        wait(mb_r_full, t & 1);
+        wait(mb_raw_full, t & 1);
         uint4 d[8];
         const uint32_t raw = base + SM_RAW + (32 * w + (lane >> 3)) * 656 + 528 + 16 * (lane & 7);
         const uint32_t valid = raw_valid[w] >> (lane >> 3);
@@ -774,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           ++seg;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(mb_r_free);
+        if (lane == 0) mbar_arrive(mb_raw_free);
 #pragma unroll 1
         for (int s = 0; s < (two ? 2 : 1); ++s) {
           if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
@@ -854,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       for (int g = 0; g < total && ok; ++g) {
         if (g + 1 < total) qk();
         const bool first = pleft == 0;
-        ok = ok && mbar_wait_lazy<true>(mb_v_full, g & 1, abort_flag, err, kWaitNs) &&
+        ok = ok && mbar_wait_lazy(mb_v_full, g & 1, abort_flag, err, kWaitNs) &&
              mbar_wait_lazy(mb_p_full, g & 1, abort_flag, err, kWaitNs);
         if (first) {
           // the accumulator of the segment before has been read
