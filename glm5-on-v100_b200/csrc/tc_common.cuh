@@ -278,30 +278,48 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // offsets in both CTAs. D of N columns takes N / 2 TMEM columns per CTA: lanes
 // 0-63 hold the CTA's 64 rows at columns [0, N/2), lanes 64-127 the same rows
 // at columns [N/2, N). Issued by one thread of the cluster's CTA 0.
-__device__ __forceinline__ void mma_f16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                                uint32_t accumulate) {
+// These are executed by a whole warp of CTA 0 in uniform control flow, so that
+// descriptors stay in uniform registers (a branch to one lane costs a move per
+// operand and MMA, and the issue rate); `leader` is non-zero in the lane that issues
+// (elect_one).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ void mma_f16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader));
 }
 // The same with A in tensor memory: each CTA's 64 rows in lanes 0-63 and again in
 // lanes 64-127 (both halves of D read their own copy), two 16-bit elements of K a
 // column, the lower index in the low half.
 __device__ __forceinline__ void mma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                                uint32_t accumulate) {
+                                                uint32_t accumulate, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader));
 }
 // Arrive (once) on this mbarrier offset in both CTAs when the pair MMAs issued so far complete.
-__device__ __forceinline__ void mma_commit_pair(uint32_t mbar) {
+__device__ __forceinline__ void mma_commit_pair(uint32_t mbar, uint32_t leader) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(mbar),
-      "h"((uint16_t)3)
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %2, 0;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+          mbar),
+      "h"((uint16_t)3), "r"(leader)
       : "memory");
 }
 // Executed by one warp of each CTA of the pair.

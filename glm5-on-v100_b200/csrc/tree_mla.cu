@@ -236,50 +236,38 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // How codes are expanded to f16: the product code * scale rounded once, by f16
-// arithmetic where the scale's parts and the products stay in f16's range
-// (kFast), by f32 elsewhere (kWide), or what that rounding left (kRest).
-enum { kFast, kWide, kRest };
+// arithmetic where the scale's parts and the products stay in f16's range, by f32
+// elsewhere.
 __device__ __forceinline__ bool fast_scale(float sc) { return sc >= 0x1p-10f && sc <= 128.0f; }
 
-// Volatile: else the expansions that the three ways share are formed before the
-// choice between them and held for all 64 codes of a lane.
-__device__ __forceinline__ uint32_t pinned(uint32_t v) {
-  asm volatile("" : "+r"(v));
-  return v;
+// Eight codes -> eight f16 values. The scale is cut in two, hi with 7 significant
+// bits: a code (4 bits) times hi is exact in f16's 11 bits, so fma(code, lo, code *
+// hi) rounds the whole product once (lo keeps the scale to 2^-15 of it or better).
+__device__ __forceinline__ uint4 dequant8(uint2 v, float sc) {
+  const float h = __uint_as_float(__float_as_uint(sc) & 0xFFFE0000u);
+  const __half2 hi = __float2half2_rn(h), lo = __float2half2_rn(sc - h);
+  __half2 x[4];
+  e4m3x4_to_half2x2(v.x, x[0], x[1]);
+  e4m3x4_to_half2x2(v.y, x[2], x[3]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = __hfma2(x[e], lo, __hmul2(x[e], hi));
+  return *reinterpret_cast<const uint4*>(x);
 }
 
-// A scale for kFast: hi cut to 7 significant bits, so that a code (4 bits) times
-// hi is exact in f16's 11 bits and fma(code, lo, code * hi) rounds the whole
-// product once (lo = scale - hi keeps the scale to 2^-15 of it or better).
-struct Scale {
-  float f;
-  __half2 hi, lo;
-  __device__ __forceinline__ explicit Scale(float sc) : f(sc) {
-    const float h = __uint_as_float(__float_as_uint(sc) & 0xFFFE0000u);
-    hi = __float2half2_rn(h);
-    lo = __float2half2_rn(sc - h);
-  }
-};
-
-// Eight codes -> eight f16 values.
-template <int HOW>
-__device__ __forceinline__ uint4 dequant8(uint2 v, const Scale& sc) {
+// The same for any scale, or with `rest` what that rounding left, itself rounded.
+// Rare: kept out of the loops' code, which has to fit the instruction cache.
+__device__ __noinline__ uint4 dequant8_any(uint2 v, float sc, bool rest) {
   __half2 x[4];
   e4m3x4_to_half2x2(v.x, x[0], x[1]);
   e4m3x4_to_half2x2(v.y, x[2], x[3]);
   uint32_t q[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if constexpr (HOW == kFast) {
-      const __half2 y = __hfma2(x[e], sc.lo, __hmul2(x[e], sc.hi));
-      q[e] = *reinterpret_cast<const uint32_t*>(&y);
-    } else {
-      const float2 f = __half22float2(x[e]);
-      q[e] = pack_half2(f.x * sc.f, f.y * sc.f);
-      if constexpr (HOW == kRest) {
-        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&q[e]));
-        q[e] = pack_half2(fmaf(f.x, sc.f, -y.x), fmaf(f.y, sc.f, -y.y));
-      }
+    const float2 f = __half22float2(x[e]);
+    q[e] = pack_half2(f.x * sc, f.y * sc);
+    if (rest) {
+      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&q[e]));
+      q[e] = pack_half2(fmaf(f.x, sc, -y.x), fmaf(f.y, sc, -y.y));
     }
   }
   return make_uint4(q[0], q[1], q[2], q[3]);
@@ -484,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   // executes its role's barriers and arrivals, and later waits return at once.
   if (warp < kProducers) {
     // ------------------------------------------------------------- producers
-    // Per tile t: store K(t+1) (under PV(t-1)), store V(t) (under QK(t+1)), take tile t+2.
+    // K(t+1) is stored under PV(t-1), V(t) under QK(t+1).
     const int w = warp;
     const uint32_t k_full0 = cluster_map(mb_k_full, 0), v_full0 = cluster_map(mb_v_full, 0);
     int kc = 0;             // K stores so far (two per tile in two-pass segments)
@@ -556,47 +544,66 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (lane < 8 && cs >= 0)
           ps = __ldg(reinterpret_cast<const float*>(p.kv + (int64_t)cs * kRowBytes + 512) + 2 * rank + (lane & 1));
       };
-      auto expand = [&](auto how, const uint2& v, float scale) {
-        return dequant8<decltype(how)::value>(make_uint2(pinned(v.x), pinned(v.y)), Scale(scale));
-      };
       // chunk lane & 7 of block lane / 8, row 4w: row x further on moves the swizzle by x
       const uint32_t k_at = base + SM_K + (lane >> 3) * kBlk + sw128_off(4 * w, lane & 7);
       const uint32_t v_at = base + SM_V + (lane >> 3) * kVBlk + sw128_off(4 * w, lane & 7);
-      auto put_k = [&](auto how) {
+      auto k_scale = [&](int x, int h) { return __shfl_sync(0xffffffffu, ks, 4 * x + 2 * h + (lane >> 4)); };
+      auto put_k = [&]() {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            sts16((k_at ^ (16 * x)) + 128 * x + 4 * h * kBlk,
-                  expand(how, kd[x][h], __shfl_sync(0xffffffffu, ks, 4 * x + 2 * h + (lane >> 4))));
+            sts16((k_at ^ (16 * x)) + 128 * x + 4 * h * kBlk, dequant8(kd[x][h], k_scale(x, h)));
       };
-      auto put_v = [&](auto how) {
+      // any scale; the registers go round, so that one piece of code serves all of them
+      auto put_k_any = [&](bool rest) {
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const int x = i >> 1, h = i & 1;
+          sts16((k_at ^ (16 * x)) + 128 * x + 4 * h * kBlk, dequant8_any(kd[0][0], k_scale(x, h), rest));
+          const uint2 d = kd[0][0];
+#pragma unroll
+          for (int k = 0; k < 7; ++k) kd[k >> 1][k & 1] = kd[(k + 1) >> 1][(k + 1) & 1];
+          kd[3][1] = d;
+        }
+      };
+      auto put_v = [&]() {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
-          sts16(at + 8192 * rank, expand(how, vd[x], __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4))));
-          sts16(at + 8192 * (rank ^ 1), expand(how, pd[x], __shfl_sync(0xffffffffu, ps, 2 * x + (lane >> 4))));
+          sts16(at + 8192 * rank, dequant8(vd[x], __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4))));
+          sts16(at + 8192 * (rank ^ 1), dequant8(pd[x], __shfl_sync(0xffffffffu, ps, 2 * x + (lane >> 4))));
+        }
+      };
+      auto put_v_any = [&]() {
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
+          const float s0 = __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4));
+          const float s1 = __shfl_sync(0xffffffffu, ps, 2 * x + (lane >> 4));
+          sts16(at + 8192 * rank, dequant8_any(vd[0], s0, false));
+          sts16(at + 8192 * (rank ^ 1), dequant8_any(pd[0], s1, false));
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            vd[k] = vd[k + 1];
+            pd[k] = pd[k + 1];
+          }
         }
       };
       auto store_k = [&]() {
-        if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
-        enter();
-        if (ok) {
-          // two passes: the first rounds in f32, the second stores its remainder
-          if (!two && __all_sync(0xffffffffu, fast_scale(ks)))
-            put_k(std::integral_constant<int, kFast>());
-          else
-            put_k(std::integral_constant<int, kWide>());
-        }
-        fence_proxy_async();
-        fence_before_sync();  // Q's tensor-memory stores
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(k_full0);
-        ++kc;
-        if (two) {
-          wait(mb_k_free, (kc - 1) & 1);
-          if (ok) put_k(std::integral_constant<int, kRest>());
+#pragma unroll 1
+        for (int s = 0; s == 0 || (s == 1 && two); ++s) {
+          if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
+          if (s == 0) enter();
+          if (ok) {
+            // two passes: the first rounds in f32, the second stores its remainder
+            if (!two && __all_sync(0xffffffffu, fast_scale(ks)))
+              put_k();
+            else
+              put_k_any(s == 1);
+          }
           fence_proxy_async();
+          fence_before_sync();  // Q's tensor-memory stores
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(k_full0);
           ++kc;
@@ -608,31 +615,27 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         for (int x = 0; x < 4; ++x) vd[x] = rank ? kd[x][1] : kd[x][0];
         vs = ks;
       };
-      if (total > 0) {
-        take(0);
-        load_others(0);
-        store_k();
-        pass_on();
-        if (total > 1) take(1);
-      }
 #pragma unroll 1
-      for (int t = 0; t < total; ++t) {
-        if (t + 1 < total) store_k();
-        if (t > 0) wait(mb_v_free, (t - 1) & 1);
-        if (ok) {
-          if (__all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps)))
-            put_v(std::integral_constant<int, kFast>());
-          else
-            put_v(std::integral_constant<int, kWide>());
+      for (int t = -1; t <= total; ++t) {
+        // K of tile t + 1 (in registers since the iteration before), V of tile t
+        if (t >= 0 && t < total) store_k();
+        if (t >= 1) {
+          if (t >= 2) wait(mb_v_free, t & 1);
+          if (ok) {
+            if (__all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps)))
+              put_v();
+            else
+              put_v_any();
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(v_full0);
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(v_full0);
-        if (t + 1 < total) {
+        if (t >= 0 && t < total) {
           pass_on();
-          load_others(t + 1);
+          load_others(t);
         }
-        if (t + 2 < total) take(t + 2);
+        if (t + 1 < total) take(t + 1);
       }
     } else {
       const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
@@ -656,10 +659,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         ++kc;
         --left;
       };
-      if (total > 0) store_k(0);
 #pragma unroll 1
-      for (int t = 0; t < total; ++t) {
+      for (int t = -1; t < total; ++t) {
         if (t + 1 < total) store_k(t + 1);
+        if (t < 0) continue;
         int code[2];
         code[0] = ok ? rows_of(t)[8 * w + r4] : -1;
         code[1] = ok ? rows_of(t)[8 * w + r4 + 4] : -1;
@@ -791,18 +794,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     }
   } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------- MMA issue
-    if (rank == 0 && lane == 0) {
-      // made anew for each tile: kept across the loop, the 104 advanced descriptors would take all registers
-      auto desc = [&](uint32_t at, uint32_t lbo) {
-        asm volatile("" : "+r"(at));
-        return sw128_desc(base + at, lbo, 1024);
-      };
+    if (rank == 0) {
+      const uint32_t leader = elect_one();
+      const uint32_t tm = __reduce_or_sync(0xffffffffu, tmem);  // in a uniform register
+      const uint64_t dq = sw128_desc(base + SM_Q, 16, 1024), dk = sw128_desc(base + SM_K, 16, 1024);
+      const uint64_t dp = sw128_desc(base + SM_P, 16, 1024), dv = sw128_desc(base + SM_V, kVBlk, 1024);
       int kc = 0, gq = 0;
       int qseg = 0, qleft = 0, passes = 1;  // segment of the next QK
       auto qk = [&]() {
 #pragma unroll 1
         for (int s = 0; s < passes || s == 0; ++s) {
-          ok = ok && mbar_wait_lazy(mb_k_full, kc & 1, abort_flag, err, kWaitNs);
+          wait(mb_k_full, kc & 1);
           if (!ok) return;
           if (qleft == 0) {  // its first tile is stored, so its descriptor is visible
             qleft = segs[qseg % kSegs].n;
@@ -810,56 +812,54 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
             ++qseg;
           }
           if (s == 0 && gq > 0) {  // the softmax has read S(gq - 1)
-            ok = ok && mbar_wait_lazy(mb_s_free, (gq - 1) & 1, abort_flag, err, kWaitNs);
+            wait(mb_s_free, (gq - 1) & 1);
             if (!ok) return;
           }
           fence_after_sync();
-          const uint64_t dq = desc(SM_Q, 16), dk = desc(SM_K, 16);
+          uint64_t a = dq, b = dk;
+#pragma unroll 1
+          for (int kb = 0; kb < kQtBlks; ++kb, b += kBlk >> 4)
 #pragma unroll
-          for (int kb = 0; kb < 9; ++kb)
+            for (int k = 0; k < 4; ++k)
+              mma_f16_ts_pair(tm + S_COL, tm + Q_COL + 32 * kb + 8 * k, b + 2 * k, IDESC_QK, (kb | k) != 0 || s > 0, leader);
+#pragma unroll 1
+          for (int kb = kQtBlks; kb < 9; ++kb, a += kBlk >> 4, b += kBlk >> 4)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint64_t b = dk + ((kb * kBlk + 32 * k) >> 4);
-              if (kb < kQtBlks)
-                mma_f16_ts_pair(tmem + S_COL, tmem + Q_COL + 32 * kb + 8 * k, b, IDESC_QK, (kb | k) != 0 || s > 0);
-              else
-                mma_f16_ss_pair(tmem + S_COL, dq + (((kb - kQtBlks) * kBlk + 32 * k) >> 4), b, IDESC_QK, 1);
-            }
-          mma_commit_pair(mb_k_free);
+            for (int k = 0; k < 4; ++k) mma_f16_ss_pair(tm + S_COL, a + 2 * k, b + 2 * k, IDESC_QK, 1, leader);
+          mma_commit_pair(mb_k_free, leader);
           ++kc;
         }
-        mma_commit_pair(mb_s_full);
+        mma_commit_pair(mb_s_full, leader);
         --qleft;
         ++gq;
       };
-      if (total > 0) qk();
       int pseg = 0, pleft = 0;
 #pragma unroll 1
-      for (int g = 0; g < total && ok; ++g) {
+      for (int g = -1; g < total && ok; ++g) {
         if (g + 1 < total) qk();
+        if (g < 0) continue;
         const bool first = pleft == 0;
-        ok = ok && mbar_wait_lazy(mb_v_full, g & 1, abort_flag, err, kWaitNs) &&
-             mbar_wait_lazy(mb_p_full, g & 1, abort_flag, err, kWaitNs);
+        wait(mb_v_full, g & 1);
+        wait(mb_p_full, g & 1);
         if (first) {
           // the accumulator of the segment before has been read
-          if (pseg > 0) ok = ok && mbar_wait_lazy(mb_o_free, (pseg - 1) & 1, abort_flag, err, kWaitNs);
+          if (pseg > 0) wait(mb_o_free, (pseg - 1) & 1);
           if (ok) pleft = segs[pseg % kSegs].n;
           ++pseg;
         }
         if (ok) {
           fence_after_sync();
-          const uint64_t dp = desc(SM_P, 16), dv = desc(SM_V, kVBlk);
-#pragma unroll
+#pragma unroll 1
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int s = 0; s < kKeys / 16; ++s)
-              mma_f16_ss_pair(tmem + 128 * h, dp + (((s >> 2) * kBlk + 32 * (s & 3)) >> 4),
-                              dv + ((2 * h * kVBlk + 2048 * s) >> 4), IDESC_PV, !first || s > 0);
-          mma_commit_pair(mb_v_free);
+              mma_f16_ss_pair(tm + 128 * h, dp + (((s >> 2) * kBlk + 32 * (s & 3)) >> 4),
+                              dv + h * (2 * kVBlk >> 4) + (2048 * s >> 4), IDESC_PV, !first || s > 0, leader);
+          mma_commit_pair(mb_v_free, leader);
         }
         --pleft;
       }
-      mma_commit_pair(mb_done);  // every MMA of this thread
+      mma_commit_pair(mb_done, leader);  // every MMA of this thread
     }
     __syncwarp();
   } else if (warp >= kSoftmax0 && warp < kSoftmax0 + kSoftmaxWarps) {
