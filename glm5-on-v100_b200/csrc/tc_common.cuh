@@ -338,24 +338,27 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mbar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
-// mbar_wait that reads the clock only once a wait has become long: the first
-// test of globaltimer costs about a microsecond, more than most waits here.
-__device__ __forceinline__ bool mbar_wait_lazy(uint32_t mbar, uint32_t parity, volatile int* abort, int32_t* err,
-                                               uint64_t timeout_ns) {
-  uint64_t t0 = 0;
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait(mbar, parity)) return true;
-    if ((it & 63u) == 0) {
-      if (*abort) return false;
-      const uint64_t t = globaltimer_ns();
-      if (t0 == 0) t0 = t;
-      if (t - t0 > timeout_ns) {
-        *abort = 1;
-        if (err) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
-        return false;
-      }
-    }
-  }
+// Bounded wait in few instructions, for loops whose code has to fit the
+// instruction cache: up to 2^20 tries, each suspended for at most about 2 us.
+// False when they ran out; the caller records it.
+__device__ __forceinline__ bool mbar_wait_tries(uint32_t mbar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      ".reg .u32 n;\n\t"
+      "mov.u32 n, 1048576;\n"
+      "WAIT_%=:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "@p bra DONE_%=;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, n, 0;\n\t"
+      "@q bra WAIT_%=;\n"
+      "DONE_%=:\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(mbar), "r"(parity), "r"(2000u)
+      : "memory");
+  return ok != 0;
 }
 // Named barrier that also ORs a predicate over its threads.
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool pred) {

@@ -79,7 +79,7 @@ constexpr uint32_t SM_RING = SM_RAW + 64 * 656;    // rows[kRing][128]
 constexpr uint32_t SM_MISC = SM_RING + kRing * kKeys * 4;
 constexpr int kSegs = 6;        // segment descriptors kept: the row warp is at most five tiles ahead of an epilogue
 constexpr int kQeSegs = 3;      // Q is at most two segments ahead of the softmax
-// the misc block: mbarriers | TMEM base, abort flag, tiles of the run, valid rows | qe | row maxima / sums | segments
+// the misc block: mbarriers | TMEM base, tiles of the run, valid rows | qe | row maxima / sums | segments
 constexpr uint32_t kBarAt = 0, kWordsAt = 192, kQeAt = 224, kRowxAt = kQeAt + kQeSegs * 64, kSegAt = kRowxAt + 4 * 64 * 4;
 constexpr uint32_t S_COL = 256, Q_COL = 320;  // O half h at [128h, +128), S at [256, +64), Q at [320, +192)
 constexpr uint32_t TMEM_COLS = 512;
@@ -291,9 +291,15 @@ __device__ __forceinline__ uint2 lds8(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ uint2 ldg_nc8(const void* p) {
+__device__ __forceinline__ uint2 ldg_nc8_or_zero(const void* p, bool on) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %3, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
+      "@q ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y)
+      : "l"(p), "r"((uint32_t)on));
   return v;
 }
 
@@ -416,7 +422,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
                  mb_q_full = mb + 72 /* [3] */, mb_r_full = mb + 96 /* [3] */, mb_r_free = mb + 120 /* [3] */,
                  mb_raw_full = mb + 144, mb_raw_free = mb + 152;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + kWordsAt);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + kWordsAt + 4);
   int* run_tiles = reinterpret_cast<int*>(misc + kWordsAt + 8);
   uint32_t* raw_valid = reinterpret_cast<uint32_t*>(misc + kWordsAt + 16);  // [2]: rows that lie in the raw buffer
   int8_t* qe = reinterpret_cast<int8_t*>(misc + kQeAt);         // [kQeSegs][64]
@@ -448,7 +453,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       mbar_init(mb_raw_full, 1);
       mbar_init(mb_raw_free, kProducers + kTailWarps);
       mbar_init_fence();
-      *abort_flag = 0;
     }
     __syncwarp();
     tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
@@ -466,9 +470,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   bool ok = true;
   // By a whole warp: `ok` stays uniform.
   auto wait = [&](uint32_t mbar, uint32_t parity) {
-    ok = __all_sync(0xffffffffu, ok && mbar_wait_lazy(mbar, parity, abort_flag, err, kWaitNs));
+    if (ok && !__all_sync(0xffffffffu, mbar_wait_tries(mbar, parity))) {
+      ok = false;
+      if (lane == 0) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
+    }
   };
-  // After a wait that ran out (`ok` false, abort flag set) every thread still
+  // After a wait that ran out (`ok` false) every thread of its warp still
   // executes its role's barriers and arrivals, and later waits return at once.
   if (warp < kProducers) {
     // ------------------------------------------------------------- producers
@@ -502,31 +509,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       // copies: loads would go through an L1 of 28 KB, whose lines they fill faster
       // than they arrive. Rows 4w + x are this warp's. A lane takes 8 codes of each
       // half row, which is one 16-byte chunk of f16, so a store writes whole 128-byte
-      // rows of four 64-column blocks. In registers a tile's codes serve K and, a tile
-      // later, the half of V that is this CTA's columns of its own keys; those of the
-      // other CTA's keys (V: 64 x 256 codes) are loaded a tile ahead.
-      uint2 kd[4][2], vd[4], pd[4];  // [row][half] | own rows | the other CTA's rows
-      // scales: lane 4x + g < 16 holds row x, group g; of the other CTA's rows lane
-      // 2x + g < 8, of this CTA's columns
-      float ks = 1.f, vs = 1.f, ps = 1.f;
-      auto take = [&](int t) {
-        wait(mb_raw_full, t & 1);
-        const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
-        const uint32_t raw = base + SM_RAW + 4 * w * 656;
+      // rows of four 64-column blocks. K is expanded from there; the half of V that is
+      // this CTA's columns of its own keys stays in registers as codes until its turn,
+      // a tile later, and that of the other CTA's keys is loaded a tile ahead.
+      uint2 vd[4], vn[4], pd[4];  // own rows: of the next V store | of the one after | the other CTA's rows
+      // their scales: lane 4x + g < 16 holds row x, group g; of the other CTA's rows
+      // lane 2x + g < 8, of this CTA's columns
+      float vs = 1.f, vns = 1.f, ps = 1.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) kd[x][h] = lds8(raw + 656 * x + 256 * h + 8 * lane);
-        ks = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
-        if ((valid & 15u) != 15u || !ok) {  // the others read as zeros
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (!((valid >> x) & 1)) kd[x][0] = kd[x][1] = make_uint2(0, 0);
-          if (!((valid >> ((lane >> 2) & 3)) & 1)) ks = 1.f;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mb_raw_free);
-      };
+      for (int x = 0; x < 4; ++x) vd[x] = vn[x] = pd[x] = make_uint2(0, 0);
       auto load_others = [&](int t) {
         wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
         if (!ok) return;
@@ -534,12 +525,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         const int4 c = *reinterpret_cast<const int4*>(rows);
         const int cs = rows[(lane >> 1) & 3];
         free_rows(t);
+        const uint8_t* at = p.kv + 256 * rank + 8 * lane;
         const int code[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          pd[x] = make_uint2(0, 0);
-          if (code[x] >= 0) pd[x] = ldg_nc8(p.kv + (int64_t)code[x] * kRowBytes + 256 * rank + 8 * lane);
-        }
+        for (int x = 0; x < 4; ++x) pd[x] = ldg_nc8_or_zero(at + (int64_t)code[x] * kRowBytes, code[x] >= 0);
         ps = 1.f;
         if (lane < 8 && cs >= 0)
           ps = __ldg(reinterpret_cast<const float*>(p.kv + (int64_t)cs * kRowBytes + 512) + 2 * rank + (lane & 1));
@@ -547,42 +536,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       // chunk lane & 7 of block lane / 8, row 4w: row x further on moves the swizzle by x
       const uint32_t k_at = base + SM_K + (lane >> 3) * kBlk + sw128_off(4 * w, lane & 7);
       const uint32_t v_at = base + SM_V + (lane >> 3) * kVBlk + sw128_off(4 * w, lane & 7);
-      auto k_scale = [&](int x, int h) { return __shfl_sync(0xffffffffu, ks, 4 * x + 2 * h + (lane >> 4)); };
-      auto put_k = [&]() {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            sts16((k_at ^ (16 * x)) + 128 * x + 4 * h * kBlk, dequant8(kd[x][h], k_scale(x, h)));
-      };
-      // any scale; the registers go round, so that one piece of code serves all of them
-      auto put_k_any = [&](bool rest) {
-#pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-          const int x = i >> 1, h = i & 1;
-          sts16((k_at ^ (16 * x)) + 128 * x + 4 * h * kBlk, dequant8_any(kd[0][0], k_scale(x, h), rest));
-          const uint2 d = kd[0][0];
-#pragma unroll
-          for (int k = 0; k < 7; ++k) kd[k >> 1][k & 1] = kd[(k + 1) >> 1][(k + 1) & 1];
-          kd[3][1] = d;
-        }
-      };
+      // Loops of one row, to stay in the instruction cache: register rows go round.
       auto put_v = [&]() {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
-          sts16(at + 8192 * rank, dequant8(vd[x], __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4))));
-          sts16(at + 8192 * (rank ^ 1), dequant8(pd[x], __shfl_sync(0xffffffffu, ps, 2 * x + (lane >> 4))));
-        }
-      };
-      auto put_v_any = [&]() {
+        const bool fast = __all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps));
 #pragma unroll 1
         for (int x = 0; x < 4; ++x) {
           const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
           const float s0 = __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4));
           const float s1 = __shfl_sync(0xffffffffu, ps, 2 * x + (lane >> 4));
-          sts16(at + 8192 * rank, dequant8_any(vd[0], s0, false));
-          sts16(at + 8192 * (rank ^ 1), dequant8_any(pd[0], s1, false));
+          uint4 v0, v1;
+          if (fast) {
+            v0 = dequant8(vd[0], s0);
+            v1 = dequant8(pd[0], s1);
+          } else {
+            v0 = dequant8_any(vd[0], s0, false);
+            v1 = dequant8_any(pd[0], s1, false);
+          }
+          sts16(at + 8192 * rank, v0);
+          sts16(at + 8192 * (rank ^ 1), v1);
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
             vd[k] = vd[k + 1];
@@ -590,52 +561,67 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           }
         }
       };
-      auto store_k = [&]() {
+      // K of tile t, from the raw buffer; `rest`: what the first of two passes rounded away
+      auto put_k = [&](bool rest) {
+        const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
+        const uint32_t raw = base + SM_RAW + 4 * w * 656;
+        vns = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
+        if (!((valid >> ((lane >> 2) & 3)) & 1)) vns = 1.f;
+        const bool fast = !two && __all_sync(0xffffffffu, fast_scale(vns));
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          uint2 k0 = lds8(raw + 656 * x + 8 * lane), k1 = lds8(raw + 656 * x + 256 + 8 * lane);
+          if (!((valid >> x) & 1)) k0 = k1 = make_uint2(0, 0);  // reads as zeros
+          const float s0 = __shfl_sync(0xffffffffu, vns, 4 * x + (lane >> 4));
+          const float s1 = __shfl_sync(0xffffffffu, vns, 4 * x + 2 + (lane >> 4));
+          uint4 v0, v1;
+          if (fast) {
+            v0 = dequant8(k0, s0);
+            v1 = dequant8(k1, s1);
+          } else {
+            v0 = dequant8_any(k0, s0, rest);
+            v1 = dequant8_any(k1, s1, rest);
+          }
+          const uint32_t at = (k_at ^ (16 * x)) + 128 * x;
+          sts16(at, v0);
+          sts16(at + 4 * kBlk, v1);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) vn[k] = vn[k + 1];
+          vn[3] = rank ? k1 : k0;
+        }
+      };
+      auto store_k = [&](int t) {
+        wait(mb_raw_full, t & 1);
 #pragma unroll 1
         for (int s = 0; s == 0 || (s == 1 && two); ++s) {
           if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
           if (s == 0) enter();
-          if (ok) {
-            // two passes: the first rounds in f32, the second stores its remainder
-            if (!two && __all_sync(0xffffffffu, fast_scale(ks)))
-              put_k();
-            else
-              put_k_any(s == 1);
-          }
+          if (ok) put_k(s == 1);
           fence_proxy_async();
           fence_before_sync();  // Q's tensor-memory stores
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(k_full0);
           ++kc;
         }
+        if (lane == 0) mbar_arrive(mb_raw_free);
         --left;
       };
-      auto pass_on = [&]() {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) vd[x] = rank ? kd[x][1] : kd[x][0];
-        vs = ks;
-      };
 #pragma unroll 1
-      for (int t = -1; t <= total; ++t) {
-        // K of tile t + 1 (in registers since the iteration before), V of tile t
-        if (t >= 0 && t < total) store_k();
-        if (t >= 1) {
-          if (t >= 2) wait(mb_v_free, t & 1);
-          if (ok) {
-            if (__all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps)))
-              put_v();
-            else
-              put_v_any();
-          }
+      for (int t = 0; t <= total; ++t) {
+        if (t < total) store_k(t);
+        if (t > 0) {  // V of tile t - 1
+          if (t > 1) wait(mb_v_free, t & 1);
+          if (ok) put_v();
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(v_full0);
         }
-        if (t >= 0 && t < total) {
-          pass_on();
+        if (t < total) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) vd[x] = vn[x];
+          vs = vns;
           load_others(t);
         }
-        if (t + 1 < total) take(t + 1);
       }
     } else {
       const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
@@ -747,36 +733,32 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
         wait(mb_raw_full, t & 1);
-        uint4 d[8];
-        const uint32_t raw = base + SM_RAW + (32 * w + (lane >> 3)) * 656 + 528 + 16 * (lane & 7);
-        const uint32_t valid = raw_valid[w] >> (lane >> 3);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          d[x] = lds16(raw + 4 * 656 * x);
-          if (!((valid >> (4 * x)) & 1)) d[x] = make_uint4(0, 0, 0, 0);
-        }
         if (left == 0 && ok) {
           left = segs[seg % kSegs].n;
           two = (segs[seg % kSegs].flags & kTwo) != 0;
           ++seg;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mb_raw_free);
+        const uint32_t raw = base + SM_RAW + (32 * w + (lane >> 3)) * 656 + 528 + 16 * (lane & 7);
+        const uint32_t at = base + SM_K + 8 * kBlk + sw128_off(32 * w + (lane >> 3), lane & 7);
+        const uint32_t valid = raw_valid[w] >> (lane >> 3);
 #pragma unroll 1
-        for (int s = 0; s < (two ? 2 : 1); ++s) {
+        for (int s = 0; s == 0 || (s == 1 && two); ++s) {
           if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
-          // Q passes through the K buffer's other blocks only
+          // (Q passes through the K buffer's other blocks only)
           if (ok) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              sts16(base + SM_K + 8 * kBlk + sw128_off(32 * w + 4 * x + (lane >> 3), lane & 7),
-                    s > 0 ? make_uint4(0, 0, 0, 0) : d[x]);
+#pragma unroll 2
+            for (int x = 0; x < 8; ++x) {  // four rows on: half a swizzle atom, chunks flip bit 2
+              uint4 d = lds16(raw + 4 * 656 * x);
+              if (s > 0 || !((valid >> (4 * x)) & 1)) d = make_uint4(0, 0, 0, 0);
+              sts16((at + 512 * x) ^ (64 * (x & 1)), d);
+            }
           }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(k_full0);
           ++kc;
         }
+        if (lane == 0) mbar_arrive(mb_raw_free);
         --left;
       }
     } else {
@@ -873,6 +855,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     const uint32_t p_full0 = cluster_map(mb_p_full, 0), o_free0 = cluster_map(mb_o_free, 0),
                    s_free0 = cluster_map(mb_s_free, 0);
     uint8_t* prow = sm + SM_P + (sp >> 1) * kBlk;
+    // 16 scores of this thread's row, hidden keys as -inf
+    auto read_s = [&](int col, uint32_t allow, uint32_t (&s)[16]) {
+      if (!ok) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = 0u;
+        return;
+      }
+      tmem_ld16(t_sp + S_COL + 32 * hh + col, s);
+      tmem_wait_ld();
+      if ((allow & 0xffffu) != 0xffffu) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;
+      }
+    };
     int g = 0;
 #pragma unroll 1
     for (int seg = 0; g < total; ++seg) {
@@ -899,24 +895,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         d = max(d - kKeys, -64);
         wait(mb_s_full, g & 1);
         fence_after_sync();
-        uint32_t s[32];
-        if (ok) {
-          tmem_ld32(t_sp + S_COL + 32 * hh, s);
-          tmem_wait_ld();
-        } else {
+        // twice through S, 16 columns at a time: the maximum, then the probabilities
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+          uint32_t s[16];
+          read_s(16 * x, allow >> (16 * x), s);
+          float y = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = 0u;
+          for (int j = 2; j < 16; j += 2) y = max3(y, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+          mx = fmaxf(mx, y);
         }
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(s_free0);
-        if (allow != 0xffffffffu) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;  // -inf
-        }
-        float mx = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-#pragma unroll
-        for (int j = 2; j < 32; j += 2) mx = max3(mx, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
         mx *= rs;  // rs >= 0
         float alpha = 1.f;
         const bool any = named_bar_or(1, kSoftmaxWarps * 32, mx > m + kRescale);
@@ -930,23 +919,36 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
             L *= alpha;
           }
         }
-        uint32_t pk[16];
+        uint4 pk[4];
         const uint64_t rs2 = pack64(rs, rs), nm2 = pack64(-m, -m);
         uint64_t sum2 = 0;
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+          uint32_t s[16];
+          read_s(16 * x, allow >> (16 * x), s);
+          pk[0] = pk[2];
+          pk[1] = pk[3];
+          uint32_t v[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float a, b;
-          unpack64(fma2(pack64(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), rs2, nm2), a, b);
-          a = ex2(a);
-          b = ex2(b);
-          sum2 = add2(sum2, pack64(a, b));
-          if (kBf16) {
-            const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-            pk[j] = *reinterpret_cast<const uint32_t*>(&v);
-          } else {
-            pk[j] = pack_half2(a, b);
+          for (int j = 0; j < 8; ++j) {
+            float a, b;
+            unpack64(fma2(pack64(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), rs2, nm2), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            sum2 = add2(sum2, pack64(a, b));
+            if (kBf16) {
+              const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+              v[j] = *reinterpret_cast<const uint32_t*>(&t);
+            } else {
+              v[j] = pack_half2(a, b);
+            }
           }
+          pk[2] = make_uint4(v[0], v[1], v[2], v[3]);
+          pk[3] = make_uint4(v[4], v[5], v[6], v[7]);
         }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(s_free0);
         {
           float a, b;
           unpack64(sum2, a, b);
@@ -957,19 +959,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (ok) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) =
-                make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
+            *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) = pk[k];
           if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
             fence_after_sync();
 #pragma unroll 1
-            for (int k = 0; k < 4; ++k) {
-              uint32_t o[32];
-              const uint32_t at = t_sp + 128 * hh + 32 * k;
-              tmem_ld32(at, o);
+            for (int k = 0; k < 8; ++k) {
+              uint32_t o[16];
+              const uint32_t at = t_sp + 128 * hh + 16 * k;
+              tmem_ld16(at, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-              tmem_st32(at, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              tmem_st16(at, o);
             }
             tmem_wait_st();
           }
