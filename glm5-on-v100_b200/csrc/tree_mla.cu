@@ -65,7 +65,7 @@ constexpr int kProducers = 16;  // warps 0-15
 constexpr int kSoftmax0 = 16, kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 24, kRowWarp = 25;
 constexpr int kTail0 = 26, kTailWarps = 2;  // fp8: the rotary part of K; 16-bit: L2 prefetch
-constexpr int kRing = 3;        // tiles whose cache rows are known ahead
+constexpr int kRing = 3;        // 16-bit caches: tiles whose rows are known ahead
 constexpr int kThreads = 28 * 32;
 constexpr uint32_t kBlk = 64 * 128;    // 64 rows x 64 16-bit values: 8 KB
 constexpr uint32_t kVBlk = 128 * 128;  // 128 keys x 64 columns: 16 KB
@@ -75,7 +75,7 @@ constexpr uint32_t SM_K = SM_Q + (9 - kQtBlks) * kBlk;
 constexpr uint32_t SM_V = SM_K + 9 * kBlk;
 constexpr uint32_t SM_P = SM_V + 4 * kVBlk;
 constexpr uint32_t SM_RAW = SM_P + 2 * kBlk;       // fp8: this CTA's 64 cache rows as they lie in the cache
-constexpr uint32_t SM_RING = SM_RAW + 64 * 656;    // rows[kRing][128]
+constexpr uint32_t SM_RING = SM_RAW + 64 * 656;    // 16-bit: rows[kRing][128]; fp8: rows[64] of the other CTA's keys
 constexpr uint32_t SM_MISC = SM_RING + kRing * kKeys * 4;
 constexpr int kSegs = 6;        // segment descriptors kept: the row warp is at most five tiles ahead of an epilogue
 constexpr int kQeSegs = 3;      // Q is at most two segments ahead of the softmax
@@ -499,11 +499,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (lane == 0) mbar_arrive(mb_q_full + 8 * (seg % kQeSegs));
       ++seg;
     };
-    auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
-    auto free_rows = [&](int t) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
-    };
     if constexpr (kFp8) {
       // This CTA's 64 keys land in shared memory as they lie in the cache, by bulk
       // copies: loads would go through an L1 of 28 KB, whose lines they fill faster
@@ -518,20 +513,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       float vs = 1.f, vns = 1.f, ps = 1.f;
 #pragma unroll
       for (int x = 0; x < 4; ++x) vd[x] = vn[x] = pd[x] = make_uint2(0, 0);
-      auto load_others = [&](int t) {
-        wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
-        if (!ok) return;
-        const int* rows = rows_of(t) + 64 * (rank ^ 1) + 4 * w;
-        const int4 c = *reinterpret_cast<const int4*>(rows);
-        const int cs = rows[(lane >> 1) & 3];
-        free_rows(t);
+      int4 oc = make_int4(-1, -1, -1, -1);  // the other CTA's rows of the tile last stored as K
+      int os = -1;
+      auto load_others = [&]() {
         const uint8_t* at = p.kv + 256 * rank + 8 * lane;
-        const int code[4] = {c.x, c.y, c.z, c.w};
+        const int code[4] = {oc.x, oc.y, oc.z, oc.w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) pd[x] = ldg_nc8_or_zero(at + (int64_t)code[x] * kRowBytes, code[x] >= 0);
         ps = 1.f;
-        if (lane < 8 && cs >= 0)
-          ps = __ldg(reinterpret_cast<const float*>(p.kv + (int64_t)cs * kRowBytes + 512) + 2 * rank + (lane & 1));
+        if (lane < 8 && os >= 0)
+          ps = __ldg(reinterpret_cast<const float*>(p.kv + (int64_t)os * kRowBytes + 512) + 2 * rank + (lane & 1));
       };
       // chunk lane & 7 of block lane / 8, row 4w: row x further on moves the swizzle by x
       const uint32_t k_at = base + SM_K + (lane >> 3) * kBlk + sw128_off(4 * w, lane & 7);
@@ -539,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       // Loops of one row, to stay in the instruction cache: register rows go round.
       auto put_v = [&]() {
         const bool fast = __all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps));
-#pragma unroll 1
+#pragma unroll 4
         for (int x = 0; x < 4; ++x) {
           const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
           const float s0 = __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4));
@@ -568,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         vns = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
         if (!((valid >> ((lane >> 2) & 3)) & 1)) vns = 1.f;
         const bool fast = !two && __all_sync(0xffffffffu, fast_scale(vns));
-#pragma unroll 1
+#pragma unroll 4
         for (int x = 0; x < 4; ++x) {
           uint2 k0 = lds8(raw + 656 * x + 8 * lane), k1 = lds8(raw + 656 * x + 256 + 8 * lane);
           if (!((valid >> x) & 1)) k0 = k1 = make_uint2(0, 0);  // reads as zeros
@@ -603,6 +594,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           if (lane == 0) mbar_arrive_cluster(k_full0);
           ++kc;
         }
+        if (ok) {
+          oc = *reinterpret_cast<const int4*>(ring + 4 * w);
+          os = ring[4 * w + ((lane >> 1) & 3)];
+        }
+        __syncwarp();
         if (lane == 0) mbar_arrive(mb_raw_free);
         --left;
       };
@@ -620,11 +616,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll
           for (int x = 0; x < 4; ++x) vd[x] = vn[x];
           vs = vns;
-          load_others(t);
+          if (ok) load_others();
         }
       }
     } else {
       const int r4 = lane >> 3, l8 = lane & 7;  // eight lanes a row, 16 bytes each
+      auto rows_of = [&](int t) { return ring + (t % kRing) * kKeys; };
+      auto free_rows = [&](int t) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
+      };
       auto store_k = [&](int t) {
         wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
         const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
@@ -672,8 +673,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     }
   } else if (warp == kRowWarp) {
     // ------------------------------------------------------ rows of the tiles
-    // Block table -> cache rows into the ring, kRing tiles ahead; fp8: this CTA's keys
-    // are copied into the raw buffer when the tile before has been taken.
+    // Block table -> cache rows. 16-bit: into the ring, kRing tiles ahead. fp8: this
+    // CTA's keys are copied into the raw buffer as soon as the tile before has been
+    // read, with the rows of the other CTA's keys beside it.
     uint64_t seen = 0;
     int seg = 0;
 #pragma unroll 1
@@ -681,43 +683,53 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
       int code[4];
       row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
-      if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
-      if (ok) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
-        if (c.first && lane == 0) {
-          Segment sg;
-          sg.b = c.b;
-          sg.rt = c.rt;
-          sg.n = min(c.r.nt - c.tile, c.left);
-          sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
-          sg.nd = c.r.nd;
-          sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
-          segs[seg % kSegs] = sg;
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(mb_r_full + 8 * (t % kRing));
       if constexpr (kFp8) {
         if (t > 0) wait(mb_raw_free, (t - 1) & 1);
-        uint32_t valid[2];
+      } else {
+        if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
+      }
+      if (ok && c.first && lane == 0) {
+        Segment sg;
+        sg.b = c.b;
+        sg.rt = c.rt;
+        sg.n = min(c.r.nt - c.tile, c.left);
+        sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
+        sg.nd = c.r.nd;
+        sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
+        segs[seg % kSegs] = sg;
+      }
+      if constexpr (kFp8) {
+        int mine[2];
+        uint32_t bytes = 0;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          valid[k] = __ballot_sync(0xffffffffu, (rank ? code[2 + k] : code[k]) >= 0);
-          if (ok && lane == 0) raw_valid[k] = valid[k];
+          mine[k] = rank ? code[2 + k] : code[k];
+          const uint32_t valid = __ballot_sync(0xffffffffu, mine[k] >= 0);
+          bytes += __popc(valid) * kRowBytes;
+          if (ok) {
+            ring[32 * k + lane] = rank ? code[k] : code[2 + k];  // the other CTA's keys
+            if (lane == 0) raw_valid[k] = valid;
+          }
         }
-        if (lane == 0) mbar_arrive_expect_tx(mb_raw_full, ok ? (__popc(valid[0]) + __popc(valid[1])) * kRowBytes : 0);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(mb_raw_full, ok ? bytes : 0);
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int mine = rank ? code[2 + k] : code[k];
           // 32 neighbouring rows are one copy
-          const int head = __shfl_sync(0xffffffffu, mine, 0);
-          const bool run = __all_sync(0xffffffffu, mine >= 0 && mine == head + lane);
-          if (ok && (run ? lane == 0 : mine >= 0))
-            bulk_load(base + SM_RAW + (32 * k + lane) * kRowBytes, p.kv + (int64_t)mine * kRowBytes,
+          const int head = __shfl_sync(0xffffffffu, mine[k], 0);
+          const bool run = __all_sync(0xffffffffu, mine[k] >= 0 && mine[k] == head + lane);
+          if (ok && (run ? lane == 0 : mine[k] >= 0))
+            bulk_load(base + SM_RAW + (32 * k + lane) * kRowBytes, p.kv + (int64_t)mine[k] * kRowBytes,
                       (run ? 32 : 1) * kRowBytes, mb_raw_full);
         }
+      } else {
+        if (ok) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_r_full + 8 * (t % kRing));
       }
       if (c.first) ++seg;
       c.next(p);
