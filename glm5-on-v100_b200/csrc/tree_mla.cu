@@ -240,12 +240,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // elsewhere.
 __device__ __forceinline__ bool fast_scale(float sc) { return sc >= 0x1p-10f && sc <= 128.0f; }
 
-// Eight codes -> eight f16 values. The scale is cut in two, hi with 7 significant
-// bits: a code (4 bits) times hi is exact in f16's 11 bits, so fma(code, lo, code *
+// A scale cut in two f16 parts, hi (low half word) with 7 significant bits and lo the
+// rest: a code (4 bits) times hi is exact in f16's 11 bits, so fma(code, lo, code *
 // hi) rounds the whole product once (lo keeps the scale to 2^-15 of it or better).
-__device__ __forceinline__ uint4 dequant8(uint2 v, float sc) {
+__device__ __forceinline__ uint32_t cut_scale(float sc) {
   const float h = __uint_as_float(__float_as_uint(sc) & 0xFFFE0000u);
-  const __half2 hi = __float2half2_rn(h), lo = __float2half2_rn(sc - h);
+  return pack_half2(h, sc - h);
+}
+
+// Eight codes -> eight f16 values.
+__device__ __forceinline__ uint4 dequant8(uint2 v, uint32_t cut) {
+  const __half2 c = *reinterpret_cast<const __half2*>(&cut);
+  const __half2 hi = __low2half2(c), lo = __high2half2(c);
   __half2 x[4];
   e4m3x4_to_half2x2(v.x, x[0], x[1]);
   e4m3x4_to_half2x2(v.y, x[2], x[3]);
@@ -504,15 +510,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       // copies: loads would go through an L1 of 28 KB, whose lines they fill faster
       // than they arrive. Rows 4w + x are this warp's. A lane takes 8 codes of each
       // half row, which is one 16-byte chunk of f16, so a store writes whole 128-byte
-      // rows of four 64-column blocks. K is expanded from there; the half of V that is
-      // this CTA's columns of its own keys stays in registers as codes until its turn,
-      // a tile later, and that of the other CTA's keys is loaded a tile ahead.
-      uint2 vd[4], vn[4], pd[4];  // own rows: of the next V store | of the one after | the other CTA's rows
+      // rows of four 64-column blocks. In registers the codes serve K and, the half that
+      // is this CTA's columns, V a tile later; V of the other CTA's keys is loaded a
+      // tile ahead.
+      uint2 kd[4][2], vd[4], pd[4];  // K: [row][half] | V: own rows | the other CTA's rows
       // their scales: lane 4x + g < 16 holds row x, group g; of the other CTA's rows
       // lane 2x + g < 8, of this CTA's columns
-      float vs = 1.f, vns = 1.f, ps = 1.f;
+      float ks = 1.f, vs = 1.f, ps = 1.f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) vd[x] = vn[x] = pd[x] = make_uint2(0, 0);
+      for (int x = 0; x < 4; ++x) kd[x][0] = kd[x][1] = vd[x] = pd[x] = make_uint2(0, 0);
       int4 oc = make_int4(-1, -1, -1, -1);  // the other CTA's rows of the tile last stored as K
       int os = -1;
       auto load_others = [&]() {
@@ -527,62 +533,59 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       // chunk lane & 7 of block lane / 8, row 4w: row x further on moves the swizzle by x
       const uint32_t k_at = base + SM_K + (lane >> 3) * kBlk + sw128_off(4 * w, lane & 7);
       const uint32_t v_at = base + SM_V + (lane >> 3) * kVBlk + sw128_off(4 * w, lane & 7);
-      // Loops of one row, to stay in the instruction cache: register rows go round.
+      // scale: as cut_scale gives it (fast), or as it is
+      auto expand = [](const uint2& v, uint32_t scale, bool fast, bool rest) {
+        return fast ? dequant8(v, scale) : dequant8_any(v, __uint_as_float(scale), rest);
+      };
       auto put_v = [&]() {
         const bool fast = __all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps));
-#pragma unroll 4
+        const uint32_t v0 = fast ? cut_scale(vs) : __float_as_uint(vs), p0 = fast ? cut_scale(ps) : __float_as_uint(ps);
+#pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
-          const float s0 = __shfl_sync(0xffffffffu, vs, 4 * x + 2 * rank + (lane >> 4));
-          const float s1 = __shfl_sync(0xffffffffu, ps, 2 * x + (lane >> 4));
-          uint4 v0, v1;
-          if (fast) {
-            v0 = dequant8(vd[0], s0);
-            v1 = dequant8(pd[0], s1);
-          } else {
-            v0 = dequant8_any(vd[0], s0, false);
-            v1 = dequant8_any(pd[0], s1, false);
-          }
-          sts16(at + 8192 * rank, v0);
-          sts16(at + 8192 * (rank ^ 1), v1);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            vd[k] = vd[k + 1];
-            pd[k] = pd[k + 1];
-          }
+          const uint32_t s0 = __shfl_sync(0xffffffffu, v0, 4 * x + 2 * rank + (lane >> 4));
+          const uint32_t s1 = __shfl_sync(0xffffffffu, p0, 2 * x + (lane >> 4));
+          sts16(at + 8192 * rank, expand(vd[x], s0, fast, false));
+          sts16(at + 8192 * (rank ^ 1), expand(pd[x], s1, fast, false));
         }
       };
-      // K of tile t, from the raw buffer; `rest`: what the first of two passes rounded away
-      auto put_k = [&](bool rest) {
-        const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
-        const uint32_t raw = base + SM_RAW + 4 * w * 656;
-        vns = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
-        if (!((valid >> ((lane >> 2) & 3)) & 1)) vns = 1.f;
-        const bool fast = !two && __all_sync(0xffffffffu, fast_scale(vns));
-#pragma unroll 4
-        for (int x = 0; x < 4; ++x) {
-          uint2 k0 = lds8(raw + 656 * x + 8 * lane), k1 = lds8(raw + 656 * x + 256 + 8 * lane);
-          if (!((valid >> x) & 1)) k0 = k1 = make_uint2(0, 0);  // reads as zeros
-          const float s0 = __shfl_sync(0xffffffffu, vns, 4 * x + (lane >> 4));
-          const float s1 = __shfl_sync(0xffffffffu, vns, 4 * x + 2 + (lane >> 4));
-          uint4 v0, v1;
-          if (fast) {
-            v0 = dequant8(k0, s0);
-            v1 = dequant8(k1, s1);
-          } else {
-            v0 = dequant8_any(k0, s0, rest);
-            v1 = dequant8_any(k1, s1, rest);
-          }
-          const uint32_t at = (k_at ^ (16 * x)) + 128 * x;
-          sts16(at, v0);
-          sts16(at + 4 * kBlk, v1);
+      auto take = [&](int t) {
+        wait(mb_raw_full, t & 1);
+        if (ok) {
+          const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
+          const uint32_t raw = base + SM_RAW + 4 * w * 656;
 #pragma unroll
-          for (int k = 0; k < 3; ++k) vn[k] = vn[k + 1];
-          vn[3] = rank ? k1 : k0;
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) kd[x][h] = lds8(raw + 656 * x + 256 * h + 8 * lane);
+          ks = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
+          oc = *reinterpret_cast<const int4*>(ring + 4 * w);
+          os = ring[4 * w + ((lane >> 1) & 3)];
+          if ((valid & 15u) != 15u) {  // the others read as zeros
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (!((valid >> x) & 1)) kd[x][0] = kd[x][1] = make_uint2(0, 0);
+            if (!((valid >> ((lane >> 2) & 3)) & 1)) ks = 1.f;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb_raw_free);
+      };
+      // `rest`: what the first of two passes rounded away
+      auto put_k = [&](bool rest) {
+        const bool fast = !two && __all_sync(0xffffffffu, fast_scale(ks));
+        const uint32_t k0 = fast ? cut_scale(ks) : __float_as_uint(ks);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t at = (k_at ^ (16 * x)) + 128 * x;
+          const uint32_t s0 = __shfl_sync(0xffffffffu, k0, 4 * x + (lane >> 4));
+          const uint32_t s1 = __shfl_sync(0xffffffffu, k0, 4 * x + 2 + (lane >> 4));
+          sts16(at, expand(kd[x][0], s0, fast, rest));
+          sts16(at + 4 * kBlk, expand(kd[x][1], s1, fast, rest));
         }
       };
       auto store_k = [&](int t) {
-        wait(mb_raw_full, t & 1);
+        take(t);
 #pragma unroll 1
         for (int s = 0; s == 0 || (s == 1 && two); ++s) {
           if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
@@ -594,12 +597,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           if (lane == 0) mbar_arrive_cluster(k_full0);
           ++kc;
         }
-        if (ok) {
-          oc = *reinterpret_cast<const int4*>(ring + 4 * w);
-          os = ring[4 * w + ((lane >> 1) & 3)];
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mb_raw_free);
         --left;
       };
 #pragma unroll 1
@@ -614,8 +611,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         }
         if (t < total) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) vd[x] = vn[x];
-          vs = vns;
+          for (int x = 0; x < 4; ++x) vd[x] = rank ? kd[x][1] : kd[x][0];
+          vs = ks;
           if (ok) load_others();
         }
       }
