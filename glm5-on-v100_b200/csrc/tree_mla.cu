@@ -533,20 +533,28 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       // chunk lane & 7 of block lane / 8, row 4w: row x further on moves the swizzle by x
       const uint32_t k_at = base + SM_K + (lane >> 3) * kBlk + sw128_off(4 * w, lane & 7);
       const uint32_t v_at = base + SM_V + (lane >> 3) * kVBlk + sw128_off(4 * w, lane & 7);
-      // scale: as cut_scale gives it (fast), or as it is
-      auto expand = [](const uint2& v, uint32_t scale, bool fast, bool rest) {
-        return fast ? dequant8(v, scale) : dequant8_any(v, __uint_as_float(scale), rest);
-      };
+      // The loops below for any scales are rolled, with row 0's registers taken and the
+      // others moved down, so that they cost little code.
       auto put_v = [&]() {
-        const bool fast = __all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps));
-        const uint32_t v0 = fast ? cut_scale(vs) : __float_as_uint(vs), p0 = fast ? cut_scale(ps) : __float_as_uint(ps);
+        if (__all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps))) {
+          const uint32_t vcut = cut_scale(vs), pcut = cut_scale(ps);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
-          const uint32_t s0 = __shfl_sync(0xffffffffu, v0, 4 * x + 2 * rank + (lane >> 4));
-          const uint32_t s1 = __shfl_sync(0xffffffffu, p0, 2 * x + (lane >> 4));
-          sts16(at + 8192 * rank, expand(vd[x], s0, fast, false));
-          sts16(at + 8192 * (rank ^ 1), expand(pd[x], s1, fast, false));
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t at = (v_at ^ (16 * x)) + 128 * x;
+            const uint32_t s0 = __shfl_sync(0xffffffffu, vcut, 4 * x + 2 * rank + (lane >> 4));
+            const uint32_t s1 = __shfl_sync(0xffffffffu, pcut, 2 * x + (lane >> 4));
+            sts16(at + 8192 * rank, dequant8(vd[x], s0));
+            sts16(at + 8192 * (rank ^ 1), dequant8(pd[x], s1));
+          }
+          return;
+        }
+#pragma unroll 1
+        for (int x = 0; x < 8; ++x) {  // own rows, then the other CTA's
+          const bool own = x < 4;
+          const float sc = __shfl_sync(0xffffffffu, own ? vs : ps, (own ? 4 * x + 2 * rank : 2 * (x - 4)) + (lane >> 4));
+          sts16((v_at ^ (16 * (x & 3))) + 128 * (x & 3) + 8192 * (own ? rank : rank ^ 1), dequant8_any(vd[0], sc, false));
+          vd[0] = vd[1], vd[1] = vd[2], vd[2] = vd[3], vd[3] = pd[0];
+          pd[0] = pd[1], pd[1] = pd[2], pd[2] = pd[3];
         }
       };
       auto take = [&](int t) {
@@ -573,15 +581,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       };
       // `rest`: what the first of two passes rounded away
       auto put_k = [&](bool rest) {
-        const bool fast = !two && __all_sync(0xffffffffu, fast_scale(ks));
-        const uint32_t k0 = fast ? cut_scale(ks) : __float_as_uint(ks);
+        if (!two && __all_sync(0xffffffffu, fast_scale(ks))) {
+          const uint32_t cut = cut_scale(ks);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t at = (k_at ^ (16 * x)) + 128 * x;
-          const uint32_t s0 = __shfl_sync(0xffffffffu, k0, 4 * x + (lane >> 4));
-          const uint32_t s1 = __shfl_sync(0xffffffffu, k0, 4 * x + 2 + (lane >> 4));
-          sts16(at, expand(kd[x][0], s0, fast, rest));
-          sts16(at + 4 * kBlk, expand(kd[x][1], s1, fast, rest));
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
+                    dequant8(kd[x][h], __shfl_sync(0xffffffffu, cut, 4 * x + 2 * h + (lane >> 4))));
+          return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const int x = i >> 1, h = i & 1;
+          const float sc = __shfl_sync(0xffffffffu, ks, 4 * x + 2 * h + (lane >> 4));
+          sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h, dequant8_any(kd[0][0], sc, rest));
+          const uint2 first = kd[0][0];
+          kd[0][0] = kd[0][1], kd[0][1] = kd[1][0], kd[1][0] = kd[1][1], kd[1][1] = kd[2][0];
+          kd[2][0] = kd[2][1], kd[2][1] = kd[3][0], kd[3][0] = kd[3][1], kd[3][1] = first;
         }
       };
       auto store_k = [&](int t) {
