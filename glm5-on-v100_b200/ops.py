@@ -484,16 +484,44 @@ def _indexer_qk_store_impl(q_out, weights_out, kv_cache, q, kw, slot_mapping, ln
                float(weight_scale), _vp(slot_mapping.contiguous()), T, H, _stream(q.device))
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        _check(t is None or (t.is_cuda and t.device == dev), f"{name} must be on {dev}")
+# The operators from here on are called every decode step on small batches, where
+# the host's time per call is the call's: messages are put together only when a
+# check fails, the device is entered only when it is not the current one, and the
+# stream is read without a Stream object.
+def _same_device(index, names, *tensors):
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"{names.split()[i]} must be on cuda:{index}")
 
 
-def _paged(block_table, lens, name, B):
+def _launch(index, fn, *args):
+    """The entry point `fn` on device `index` and its current stream (the last argument)."""
+    if torch.cuda.current_device() == index:
+        L.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            L.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _vector(t, n, name, shape="[B]"):
+    """An int32 vector of at least n elements, contiguous."""
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < n:
+        raise RuntimeError(f"{name} must be int32 {shape}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _pages(block_table, B):
+    """(pointer, row stride, blocks a row) of a block table of at least B rows."""
     _int32(block_table, "block_table")
-    _int32(lens, name)
     _rowmajor(block_table, "block_table")
-    _check(block_table.size(0) >= B, f"block_table has fewer than {B} rows")
+    n, width = block_table.shape
+    if n < B:
+        raise RuntimeError(f"block_table has fewer than {B} rows")
+    return block_table.data_ptr(), max(block_table.stride(0), width), width
 
 
 def _latent_format(kv_cache):
@@ -509,35 +537,36 @@ def _latent_format(kv_cache):
 
 def _tree_mla_decode_impl(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, draft_lens, scale):
     _check(q.is_cuda, "q must be a CUDA tensor")
-    _same_device(q.device, o=o, lse=lse, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens,
-                 tree_mask=tree_mask, draft_lens=draft_lens)
+    index = q.get_device()
+    _same_device(index, "o lse kv_cache block_table seq_lens tree_mask draft_lens", o, lse, kv_cache, block_table,
+                 seq_lens, tree_mask, draft_lens)
     _check(q.dtype in (torch.float16, torch.bfloat16), "q must be fp16 or bf16")
     _check(o.dtype in (torch.float16, torch.bfloat16), "o must be fp16 or bf16")
     _check(lse.dtype == torch.float32, "lse must be fp32")
     fmt, row = _latent_format(kv_cache)
     _check(q.dim() == 4 and q.size(3) == 576, "q must be [B, T, n_head, 576]")
-    B, T, H = q.size(0), q.size(1), q.size(2)
-    _check(tuple(o.shape) == (B, T, H, 512) and tuple(lse.shape) == (B, T, H), "o/lse shape mismatch with q")
+    B, T, H, _ = q.shape
+    _check(o.shape == (B, T, H, 512) and lse.shape == (B, T, H), "o/lse shape mismatch with q")
     _check(q.is_contiguous() and o.is_contiguous() and lse.is_contiguous() and kv_cache.is_contiguous(),
            "q, o, lse and kv_cache must be contiguous")
-    _paged(block_table, seq_lens, "seq_lens", B)
-    _check(seq_lens.dim() == 1 and seq_lens.numel() >= B, "seq_lens must be [B]")
+    pages = _pages(block_table, B)
+    seq_lens = _vector(seq_lens, B, "seq_lens")
     _check(tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.size(0) >= B and
            tree_mask.size(1) == T and (T <= 1 or tree_mask.stride(1) == 1),
            "tree_mask must be int64 [B, T] with unit inner stride")
     if draft_lens is not None:
-        _int32(draft_lens, "draft_lens")
-        _check(draft_lens.dim() == 1 and draft_lens.numel() >= B, "draft_lens must be [B]")
-        draft_lens = draft_lens.contiguous()
+        draft_lens = _vector(draft_lens, B, "draft_lens")
     page = kv_cache.size(-2)
     _check(page > 0, "kv_cache has no rows in a page")
-    with torch.cuda.device(q.device):
+    if torch.cuda.current_device() == index:
         ws_bytes = int(L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        L.call("dsa_tree_mla_decode", _vp(o), _DTYPE[o.dtype], _vp(lse), _vp(q), _DTYPE[q.dtype], _vp(kv_cache), fmt,
-               kv_cache.numel() // row, page, _vp(block_table), max(block_table.stride(0), block_table.size(1)),
-               block_table.size(1), _vp(seq_lens.contiguous()), _vp(draft_lens), _vp(tree_mask),
-               max(tree_mask.stride(0), T), B, T, H, float(scale), _vp(ws), ws_bytes, _stream(q.device))
+    else:
+        with torch.cuda.device(index):
+            ws_bytes = int(L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _launch(index, "dsa_tree_mla_decode", o.data_ptr(), _DTYPE[o.dtype], lse.data_ptr(), q.data_ptr(), _DTYPE[q.dtype],
+            kv_cache.data_ptr(), fmt, kv_cache.numel() // row, page, *pages, seq_lens.data_ptr(), _ptr(draft_lens),
+            tree_mask.data_ptr(), max(tree_mask.stride(0), T), B, T, H, float(scale), _ptr(ws), ws_bytes)
 
 
 def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens):
@@ -545,77 +574,76 @@ def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens)
         return
     c0 = caches[0]
     _check(c0.is_cuda and c0.dim() >= 2, "caches must be CUDA tensors [.., page, row]")
-    _same_device(c0.device, block_table=block_table, seq_lens=seq_lens, accepted=accepted, draft_lens=draft_lens)
+    index = c0.get_device()
+    _same_device(index, "block_table seq_lens accepted draft_lens", block_table, seq_lens, accepted, draft_lens)
+    shape, dtype = c0.shape, c0.dtype
     for i, c in enumerate(caches):
-        _check(c.device == c0.device and c.shape == c0.shape and c.dtype == c0.dtype and c.is_contiguous(),
-               f"cache {i} must be contiguous with the shape, dtype and device of the first")
-    _check(len({c.data_ptr() for c in caches}) == len(caches), "the same cache twice in the list")
+        if c.shape != shape or c.dtype != dtype or c.get_device() != index or not c.is_contiguous():
+            raise RuntimeError(f"cache {i} must be contiguous with the shape, dtype and device of the first")
+    ptrs = [c.data_ptr() for c in caches]
+    _check(len(set(ptrs)) == len(ptrs), "the same cache twice in the list")
     _check(accepted.dim() == 2, "accepted must be [B, n_accept]")
     _int32(accepted, "accepted")
     B, A = accepted.shape
     _check(A <= 1 or accepted.stride(1) == 1, "accepted must have unit inner stride")
-    _paged(block_table, seq_lens, "seq_lens", B)
-    _check(seq_lens.dim() == 1 and seq_lens.numel() >= B, "seq_lens must be [B]")
-    _int32(draft_lens, "draft_lens")
-    _check(draft_lens.dim() == 1 and draft_lens.numel() >= B, "draft_lens must be [B]")
-    page, row_bytes = c0.size(-2), c0.size(-1) * c0.element_size()
-    if c0.numel() == 0:
+    pages = _pages(block_table, B)
+    seq_lens = _vector(seq_lens, B, "seq_lens")
+    draft_lens = _vector(draft_lens, B, "draft_lens")
+    width, n = shape[-1], c0.numel()
+    if n == 0:
         return
-    ptrs = (ctypes.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
-    with torch.cuda.device(c0.device):
-        L.call("dsa_commit_draft_rows", ptrs, len(caches), c0.numel() // c0.size(-1), page, row_bytes,
-               _vp(block_table), max(block_table.stride(0), block_table.size(1)), block_table.size(1),
-               _vp(seq_lens.contiguous()), _vp(draft_lens.contiguous()), 64, _vp(accepted),
-               max(accepted.stride(0), A), A, B, _stream(c0.device))
+    _launch(index, "dsa_commit_draft_rows", (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), n // width, shape[-2],
+            width * c0.element_size(), *pages, seq_lens.data_ptr(), draft_lens.data_ptr(), 64, accepted.data_ptr(),
+            max(accepted.stride(0), A), A, B)
 
 
 def _gather_cache_impl(out, cache, block_table, cu_seq_lens, seq_starts):
     _check(out.is_cuda, "out must be a CUDA tensor")
-    _same_device(out.device, cache=cache, block_table=block_table, cu_seq_lens=cu_seq_lens, seq_starts=seq_starts)
+    index = out.get_device()
+    _same_device(index, "cache block_table cu_seq_lens seq_starts", cache, block_table, cu_seq_lens, seq_starts)
     _check(out.dtype in (torch.float16, torch.bfloat16), "out must be fp16 or bf16")
     _check(cache.dim() >= 2 and cache.is_contiguous(), "cache must be contiguous [.., page, row]")
+    elems = cache.size(-1)
     if cache.dtype == torch.uint8:
-        _check(cache.size(-1) in (DSMLA_ROW_BYTES, IDXK_FP8_ROW_BYTES), "uint8 cache rows must be 656 or 132 bytes")
-        fmt, width = ((L.DSA_FP8_DS_MLA, 576) if cache.size(-1) == DSMLA_ROW_BYTES else (L.DSA_FP8_IDXK, 128))
+        _check(elems in (DSMLA_ROW_BYTES, IDXK_FP8_ROW_BYTES), "uint8 cache rows must be 656 or 132 bytes")
+        fmt, width = (L.DSA_FP8_DS_MLA, 576) if elems == DSMLA_ROW_BYTES else (L.DSA_FP8_IDXK, 128)
     else:
         _check(cache.dtype in (torch.float16, torch.bfloat16), "cache must be fp16, bf16 or uint8 (fp8)")
-        fmt, width = _DTYPE[cache.dtype], cache.size(-1)
-    _check(out.dim() == 2 and out.size(1) == width and out.stride(1) == 1, f"out must be [N, {width}], unit inner stride")
-    _check(cu_seq_lens.dim() == 1 and cu_seq_lens.numel() >= 1, "cu_seq_lens must be [B + 1]")
+        fmt, width = _DTYPE[cache.dtype], elems
+    if out.dim() != 2 or out.size(1) != width or out.stride(1) != 1:
+        raise RuntimeError(f"out must be [N, {width}], unit inner stride")
     B = cu_seq_lens.numel() - 1
-    _paged(block_table, cu_seq_lens, "cu_seq_lens", B)
+    cu_seq_lens = _vector(cu_seq_lens, 1, "cu_seq_lens", "[B + 1]")
+    pages = _pages(block_table, B)
     if seq_starts is not None:
-        _int32(seq_starts, "seq_starts")
-        _check(seq_starts.dim() == 1 and seq_starts.numel() >= B, "seq_starts must be [B]")
-        seq_starts = seq_starts.contiguous()
+        seq_starts = _vector(seq_starts, B, "seq_starts")
     _check(cache.size(-2) > 0, "cache has no rows in a page")
     n = out.size(0)
     if n == 0:
         return
-    with torch.cuda.device(out.device):
-        L.call("dsa_gather_cache", _vp(out), _DTYPE[out.dtype], max(out.stride(0), width) if n == 1 else out.stride(0),
-               n, _vp(cache), fmt, cache.numel() // cache.size(-1), cache.size(-2), width, _vp(block_table),
-               max(block_table.stride(0), block_table.size(1)), block_table.size(1), _vp(cu_seq_lens.contiguous()),
-               _vp(seq_starts), B, _stream(out.device))
+    _launch(index, "dsa_gather_cache", out.data_ptr(), _DTYPE[out.dtype],
+            max(out.stride(0), width) if n == 1 else out.stride(0), n, cache.data_ptr(), fmt, cache.numel() // elems,
+            cache.size(-2), width, *pages, cu_seq_lens.data_ptr(), _ptr(seq_starts), B)
 
 
 def _rotary_embedding_impl(out, x, positions, cos_sin_cache, is_neox, rope_offset):
     _check(x.is_cuda, "x must be a CUDA tensor")
-    _same_device(x.device, out=out, positions=positions, cos_sin_cache=cos_sin_cache)
+    index = x.get_device()
+    _same_device(index, "out positions cos_sin_cache", out, positions, cos_sin_cache)
     _check(x.dtype in _DTYPE and out.dtype == x.dtype, "x and out must be fp16, bf16 or fp32, the same dtype")
-    _check(x.dim() == 3 and tuple(out.shape) == tuple(x.shape), "x and out must be [T, n_head, width]")
+    _check(x.dim() == 3 and out.shape == x.shape, "x and out must be [T, n_head, width]")
     T, H, W = x.shape
-    _check(W <= 1 or (x.stride(2) == 1 and out.stride(2) == 1), "x and out must have unit inner stride")
+    xs, ys = x.stride(), out.stride()
+    _check(W <= 1 or (xs[2] == 1 and ys[2] == 1), "x and out must have unit inner stride")
     _check(positions.dtype == torch.int64 and positions.dim() == 1 and positions.numel() == T and
            positions.is_contiguous(), "positions must be contiguous int64 [T]")
     _check(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.dim() == 2 and cos_sin_cache.is_contiguous() and
            cos_sin_cache.size(0) > 0, "cos_sin_cache must be contiguous f32 [max_pos, rotary_dim]")
-    if x.numel() == 0:
+    if T * H * W == 0:
         return
-    with torch.cuda.device(x.device):
-        L.call("dsa_rotary_embedding", _vp(out), out.stride(0), out.stride(1), _vp(x), x.stride(0), x.stride(1),
-               _DTYPE[x.dtype], _vp(positions), _vp(cos_sin_cache), cos_sin_cache.size(0), cos_sin_cache.size(1),
-               int(rope_offset), int(bool(is_neox)), T, H, W, _stream(x.device))
+    max_pos, rot = cos_sin_cache.shape
+    _launch(index, "dsa_rotary_embedding", out.data_ptr(), ys[0], ys[1], x.data_ptr(), xs[0], xs[1], _DTYPE[x.dtype],
+            positions.data_ptr(), cos_sin_cache.data_ptr(), max_pos, rot, int(rope_offset), int(bool(is_neox)), T, H, W)
 
 
 # ------------------------------------------------------ torch registration
@@ -680,8 +708,11 @@ for _name in ("sm70_sparse_mla_decode", "sm70_indexer_logits", "sm70_indexer_log
     torch.library.register_fake(f"{NAMESPACE}::{_name}")(_noop_fake)
 
 
+_OVERLOADS = {name: getattr(getattr(torch.ops, NAMESPACE), name).default for name in _SCHEMAS}
+
+
 def _op(name):
-    return getattr(getattr(torch.ops, NAMESPACE), name)
+    return _OVERLOADS[name]
 
 
 # ---------------------------------------- reference-compatible wrappers
