@@ -91,6 +91,13 @@ constexpr int kTwoPassKeys = 512;      // fp8: the remainder of the rounding is 
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kSlotF = DV + 2;         // f32 of a row's partial state: o, then m and l
 
+// Where a pair's run starts: key tile `tile` of `nt` in a row tile (0 also for an
+// empty run); the other pairs' runs follow at distances of `chunk`.
+struct Cut {
+  int b, rt, tile, nt;
+  int chunk, pad[3];
+};
+
 struct TreeArgs {
   const void* q;
   const uint8_t* kv;
@@ -102,6 +109,7 @@ struct TreeArgs {
   float* lse;
   float* part_o;   // [2 * pairs][slot_rows][512]
   float* part_ml;  // [2 * pairs][slot_rows][2]
+  Cut* cuts;       // [pairs]
   int64_t n_kv_rows, bt_stride, mask_stride;
   int page, page_shift, max_blocks, B, T, H, pairs, slot_rows;  // page_shift < 0: no power of two
   int q_bf16, o_bf16;
@@ -150,6 +158,7 @@ static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 
 // One pair's walk over its run of tiles.
 struct Cursor {
+  int chunk;       // tiles of a full run
   int left;        // tiles left, this one included
   int b, rt, tile;
   bool first;      // first tile of a segment
@@ -176,6 +185,7 @@ __device__ __forceinline__ Cursor find_run(const TreeArgs& p, int pair, int lane
   const long long chunk = chunk_of(work, p.pairs);
   const long long w0 = chunk * pair;
   Cursor c{};
+  c.chunk = (int)min(chunk, 0x7fffffffll);
   c.left = (int)max(min(chunk, work - w0), 0ll);
   c.first = true;
   if (c.left == 0) return c;
@@ -464,7 +474,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
   } else if (warp == kRowWarp) {
     c = find_run(p, pair, lane);
-    if (lane == 0) *run_tiles = c.left;
+    if (lane == 0) {
+      *run_tiles = c.left;
+      if (rank == 0) p.cuts[pair] = Cut{c.b, c.rt, c.tile, c.r.nt, c.chunk, {0, 0, 0}};
+    }
   }
   fence_before_sync();
   __syncthreads();
@@ -1079,67 +1092,92 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   }
 }
 
-// Rows whose key tiles lie in several segments: o = sum_s w_s o_s / sum_s w_s l_s
-// with w_s = 2^(m_s - max m); rows of no segment: o = 0, lse = -inf. One block
-// per 8 rows, a warp a row, 16 columns a lane; the segments are found as the
-// main kernel cut them.
-constexpr int kMergeRows = 8;
-__global__ void __launch_bounds__(32 * kMergeRows) tree_merge_kernel(const TreeArgs p) {
-  const int lane = threadIdx.x & 31;
-  const int rt = blockIdx.y / (kPairRows / kMergeRows);
-  const int row = (blockIdx.y % (kPairRows / kMergeRows)) * kMergeRows + (threadIdx.x >> 5);  // of the row tile
-  const int b = blockIdx.x;
-  const int64_t r = (int64_t)rt * kPairRows + row;
-  if (r >= (int64_t)p.T * p.H) return;
-  const int64_t grow = (int64_t)b * p.T * p.H + r;
-  const Req q = load_req(p, b);
-  float acc[16];
+// Row tiles whose key tiles lie in several segments: o = sum_s w_s o_s / sum_s w_s
+// l_s with w_s = 2^(m_s - max m), four warps a row, 128 columns each. Such a tile is
+// cut where a pair's run starts inside it; kMergeBlocks blocks belong to each of
+// these starts, and those of a tile's first one merge it. The last B * tiles
+// blocks write the row tiles that no segment holds: o = 0, lse = -inf.
+constexpr int kMergeRows = 2;
+constexpr int kMergeBlocks = kPairRows / kMergeRows;
+__device__ __forceinline__ void store_merged(const TreeArgs& p, int64_t at, float4 v) {
+  uint2 x;
+  if (p.o_bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    x = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    x = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+  }
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.o) + at * 2) = x;
+}
+
+__global__ void __launch_bounds__(128 * kMergeRows) tree_merge_kernel(const TreeArgs p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = p.T * p.H;
+  const int cuts = (p.pairs - 1) * kMergeBlocks;
+  cudaGridDependencySynchronize();  // the main kernel's results
+  if ((int64_t)blockIdx.x >= cuts) {
+    const int tiles = (rows + kPairRows - 1) / kPairRows;
+    const int64_t i = (int64_t)blockIdx.x - cuts;
+    const int b = (int)(i / tiles), rt = (int)(i % tiles);
+    const Req q = load_req(p, b);
+    if (q.nt > 0 && rt < q.nrt) return;
+    const int end = min(rows, (rt + 1) * kPairRows);
+    for (int r = rt * kPairRows + warp; r < end; r += 4 * kMergeRows) {
+      const int64_t grow = (int64_t)b * rows + r;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  float M = -INFINITY, L = 0.f;
-  if (q.nt > 0 && rt < q.nrt) {
-    const long long chunk = chunk_of(warp_work(p, p.B, lane), p.pairs);
-    const long long w0 = warp_work(p, b, lane) + (long long)rt * q.nt;
-    const int p0 = (int)(w0 / chunk), p1 = (int)((w0 + q.nt - 1) / chunk);
-    if (p0 == p1) return;  // one segment: the main kernel wrote the row
-    for (int s = p0; s <= p1; ++s) {
-      // the segment that starts a row tile inside its pair's run is the run's last: slot 1
-      const int64_t at = (int64_t)(2 * s + (s == p0 && w0 > s * chunk ? 1 : 0)) * p.slot_rows + row;
-      const float l = p.part_ml[at * 2 + 1];
-      if (!(l > 0.f)) {
-        if (l != l) L = l;  // NaN scores stay NaN
-        continue;
-      }
-      const float m = p.part_ml[at * 2];
-      const float Mn = fmaxf(M, m);
-      const float a = M == -INFINITY ? 0.f : exp2f(M - Mn), w = exp2f(m - Mn);
-      M = Mn;
-      L = L * a + l * w;
+      for (int c = 0; c < 4; ++c) store_merged(p, grow * DV + 128 * c + 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (lane == 0) p.lse[grow] = -INFINITY;
+    }
+    return;
+  }
+  const int pair = 1 + blockIdx.x / kMergeBlocks;
+  const Cut cut = p.cuts[pair];
+  if (cut.tile == 0 || cut.tile > cut.chunk) return;  // no cut, or not the tile's first
+  const int row = (int)(blockIdx.x % kMergeBlocks) * kMergeRows + (warp >> 2);  // of the row tile
+  if (cut.rt * kPairRows + row >= rows) return;
+  const int64_t grow = (int64_t)cut.b * rows + cut.rt * kPairRows + row;
+  const int n = 1 + (cut.nt - cut.tile + cut.chunk - 1) / cut.chunk;  // segments
+  // the first one is slot 0 if the tile starts where its pair's run does, else slot 1
+  auto state = [&](int i) {
+    return (int64_t)(2 * (pair - 1 + i) + (i == 0 && cut.tile < cut.chunk ? 1 : 0)) * p.slot_rows + row;
+  };
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) {
+    const float2 x = ml[state(i)];
+    if (x.y > 0.f) M = fmaxf(M, x.x);
+  }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * DV + 128 * c + 4 * lane);
-        acc[4 * c] = acc[4 * c] * a + v.x * w;
-        acc[4 * c + 1] = acc[4 * c + 1] * a + v.y * w;
-        acc[4 * c + 2] = acc[4 * c + 2] * a + v.z * w;
-        acc[4 * c + 3] = acc[4 * c + 3] * a + v.w * w;
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float* po = p.part_o + 128 * (warp & 3) + 4 * lane;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float w = 0.f;
+    if (i0 + lane < n) {
+      const float2 x = ml[state(i0 + lane)];
+      if (x.y > 0.f) w = exp2f(x.x - M);
+      L += x.y == 0.f ? 0.f : x.y * (x.y > 0.f ? w : 1.f);  // a NaN stays one
+    }
+    const int m = min(32, n - i0);
+#pragma unroll 4
+    for (int j = 0; j < m; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const float4 v = *reinterpret_cast<const float4*>(po + state(i0 + j) * DV);
+      if (wj != 0.f) {
+        acc.x = fmaf(v.x, wj, acc.x);
+        acc.y = fmaf(v.y, wj, acc.y);
+        acc.z = fmaf(v.z, wj, acc.z);
+        acc.w = fmaf(v.w, wj, acc.w);
       }
     }
   }
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint2 v;
-    if (p.o_bf16) {
-      const __nv_bfloat162 x = __floats2bfloat162_rn(acc[4 * c] * inv, acc[4 * c + 1] * inv);
-      const __nv_bfloat162 y = __floats2bfloat162_rn(acc[4 * c + 2] * inv, acc[4 * c + 3] * inv);
-      v = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-    } else {
-      v = make_uint2(pack_half2(acc[4 * c] * inv, acc[4 * c + 1] * inv),
-                     pack_half2(acc[4 * c + 2] * inv, acc[4 * c + 3] * inv));
-    }
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.o) + (grow * DV + 128 * c + 4 * lane) * 2) = v;
-  }
-  if (lane == 0) p.lse[grow] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  const float inv = L > 0.f ? 1.f / L : L;
+  store_merged(p, grow * DV + 128 * (warp & 3) + 4 * lane,
+               make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  if (lane == 0 && (warp & 3) == 0) p.lse[grow] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 std::once_flag g_once[kMaxDevices];
@@ -1209,7 +1247,7 @@ using namespace dsa;
 // Two partial states per pair, of the rows that a pair can hold.
 static size_t tree_workspace(int T, int n_head, int pairs) {
   const int64_t rows = std::min<int64_t>(kPairRows, (int64_t)T * n_head);
-  return (size_t)2 * pairs * rows * kSlotF * sizeof(float);
+  return (size_t)pairs * sizeof(Cut) + (size_t)2 * pairs * rows * kSlotF * sizeof(float);
 }
 
 extern "C" size_t dsa_tree_mla_decode_workspace_bytes(int B, int T, int n_head) {
@@ -1279,7 +1317,8 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
   DSA_REQUIRE(workspace != nullptr && workspace_bytes >= need, DSA_ERR_WORKSPACE,
               "tree_mla_decode: workspace needs %zu bytes, got %zu", need, workspace_bytes);
   DSA_REQUIRE(((uintptr_t)workspace & 15) == 0, DSA_ERR_INVALID, "tree_mla_decode: workspace must be 16-byte aligned");
-  p.part_o = reinterpret_cast<float*>(workspace);
+  p.cuts = reinterpret_cast<Cut*>(workspace);
+  p.part_o = reinterpret_cast<float*>(p.cuts + p.pairs);
   p.part_ml = p.part_o + (size_t)2 * p.pairs * p.slot_rows * DV;
   cudaStream_t s = as_stream(stream);
   const cudaError_t e = kv_format == DSA_FP8_DS_MLA ? launch_main<DSA_FP8_DS_MLA>(p, dev, s)
@@ -1290,6 +1329,20 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
     return DSA_ERR_CUDA;
   }
   const int rt = (T * n_head + kPairRows - 1) / kPairRows;
-  tree_merge_kernel<<<dim3(B, rt * (kPairRows / kMergeRows)), 32 * kMergeRows, 0, s>>>(p);
+  // launched while the main kernel's last blocks run
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((int64_t)B * rt + (int64_t)(p.pairs - 1) * kMergeBlocks));
+  cfg.blockDim = dim3(128 * kMergeRows);
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const cudaError_t em = cudaLaunchKernelEx(&cfg, tree_merge_kernel, p);
+  if (em != cudaSuccess) {
+    set_error("tree_merge_kernel launch: %s", cudaGetErrorString(em));
+    return DSA_ERR_CUDA;
+  }
   return check_launch("tree_merge_kernel");
 }

@@ -99,13 +99,15 @@ def forward_mqa_tree(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch
     """
     B, T = tree_mask.shape
     lead = q.shape[:-1]
-    q4 = q.reshape(B, T, q.shape[-2], q.shape[-1])
-    out_dtype = q.dtype if q.dtype in (torch.float16, torch.bfloat16) else torch.float16
-    qk = q4 if q4.dtype == out_dtype and q4.is_contiguous() else q4.to(out_dtype).contiguous()
-    o = torch.empty(*qk.shape[:3], kv_lora_rank, dtype=out_dtype, device=q.device)
-    lse = torch.empty(qk.shape[:3], dtype=torch.float32, device=q.device)
-    ops.tree_mla_decode(o, lse, qk, kv_cache, block_table, seq_lens, tree_mask, float(scale), draft_lens)
-    return o.view(*lead, kv_lora_rank), lse.view(lead)
+    if q.dim() != 4:
+        q = q.reshape(B, T, q.shape[-2], q.shape[-1])
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        q = q.to(torch.float16)
+    q = q.contiguous()
+    o = q.new_empty((*q.shape[:3], kv_lora_rank))
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32)
+    ops.tree_mla_decode(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, float(scale), draft_lens)
+    return (o, lse) if len(lead) == 3 else (o.view(*lead, kv_lora_rank), lse.view(lead))
 
 
 def per_token_metadata(chunks, nd0: int, q_len: int, query_start_loc: torch.Tensor, block_table: torch.Tensor):
