@@ -10,13 +10,13 @@
 // writers' rotation. The table holds whatever scaling of the frequencies the
 // model uses (rope.rope_cos_sin_cache).
 //
-// Bound by HBM: each element is read and written once; the table row of a token
-// stays in L1 over its heads. A block takes whole tokens, or a range of one
-// token's heads, as "units" of one 16-byte vector (GPT-J: whole pairs in it;
-// NeoX: the two vectors of its pairs), so every load and store is 16 bytes wide
-// and in-place rotation reads both halves of a pair before it writes either.
-// Rows whose strides, offset or widths are not multiples of 16 bytes take units
-// of one pair (or one copied element) instead.
+// Bound by HBM: each element is read and written once. A thread owns one "unit" of
+// the head, a 16-byte vector (GPT-J: whole pairs in it; NeoX: the two vectors of
+// its pairs), of several heads of a token: the angles are loaded once and stay in
+// registers, the heads' loads are in flight together with them, and in-place
+// rotation reads both halves of a pair before it writes either. Rows whose
+// strides, offset or widths are not multiples of 16 bytes take units of one pair
+// (or one copied element) instead.
 #include <algorithm>
 
 #include "common.cuh"
@@ -24,9 +24,7 @@
 namespace dsa {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kUnroll = 4;      // units whose loads are in flight at once
-constexpr int kMaxUnits = 2048; // units per block: 8 per thread
+constexpr int kThreads = 256;  // at most, of a block: units x heads x tokens
 
 struct RotaryArgs {
   void* out;
@@ -38,9 +36,6 @@ struct RotaryArgs {
   int r, off, width;
   int n_tok, n_head;
   int units_rot, units;    // units of the rotary part / of a whole head
-  int tokens_per_block, heads_per_block;
-  uint32_t mul_units;      // ceil(2^32 / units): exact quotients below 2^16
-  int copy;                // 0: in place, nothing to copy
 };
 
 template <typename T>
@@ -76,115 +71,97 @@ struct Chunk {
   }
 };
 
+// Heads of a thread whose loads are in flight at once (NeoX loads two words each).
+template <bool NEOX, bool VEC>
+constexpr int kHeads = NEOX && VEC ? 2 : 4;
+
 template <typename T, bool NEOX, bool VEC>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   using C = Chunk<T, VEC>;
   constexpr int E = C::E;
-  const int t0 = blockIdx.x * a.tokens_per_block;
-  const int h0 = blockIdx.y * a.heads_per_block;
-  const int nt = min(a.tokens_per_block, a.n_tok - t0);
-  const int nh = min(a.heads_per_block, a.n_head - h0);
+  constexpr int U = kHeads<NEOX, VEC>;
+  constexpr bool TWO = NEOX || !VEC;       // a pair's elements in two chunks
+  constexpr int P = TWO ? E : E / 2;       // pairs of a unit
+  const int t = blockIdx.x * blockDim.z + threadIdx.z;
+  if (t >= a.n_tok) return;
+  const int64_t pos = a.pos[t];
+  const float* cs = a.cos_sin + (pos < 0 ? 0 : (pos >= a.max_pos ? a.max_pos - 1 : pos)) * a.r;
   const int half = a.r >> 1;
-  const int per_token = nh * a.units;
-  const int n = nt * per_token;
-  for (int base = threadIdx.x; base < n; base += kThreads * kUnroll) {
-    C lo[kUnroll], hi[kUnroll];
-    int first[kUnroll], token[kUnroll], unit[kUnroll];
-    int64_t src[kUnroll], dst[kUnroll];
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      int j = base + k * kThreads;
-      token[k] = -1;
-      if (j >= n) continue;
-      int t = 0;
-      if (nt > 1) {
-        t = j / per_token;
-        j -= t * per_token;
-      }
-      const int h = a.mul_units ? (int)__umulhi((uint32_t)j, a.mul_units) : j;
-      const int u = j - h * a.units;
-      if (u >= a.units_rot && !a.copy) continue;
-      token[k] = t0 + t;
-      unit[k] = u;
-      src[k] = (int64_t)(t0 + t) * a.xt + (int64_t)(h0 + h) * a.xh;
-      dst[k] = (int64_t)(t0 + t) * a.ot + (int64_t)(h0 + h) * a.oh;
-      const T* x = reinterpret_cast<const T*>(a.x) + src[k];
-      if (u < a.units_rot) {
-        // the pair's two elements, or for GPT-J vectors the one word that holds E/2 pairs
-        first[k] = a.off + (NEOX ? u * E : u * (VEC ? E : 2));
-        lo[k].load(x + first[k]);
-        if (NEOX || !VEC) hi[k].load(x + first[k] + (NEOX ? half : 1));
-      } else {
-        const int c = (u - a.units_rot) * E;
-        first[k] = c < a.off ? c : c + a.r;
-        lo[k].load(x + first[k]);
-      }
+  const int h0 = blockIdx.y * (U * blockDim.y) + threadIdx.y;
+  for (int u = threadIdx.x; u < a.units; u += blockDim.x) {
+    const bool rot = u < a.units_rot;
+    int at;  // in the head: of the first chunk
+    if (rot) {
+      at = a.off + u * (NEOX ? E : VEC ? E : 2);
+    } else {
+      at = (u - a.units_rot) * E;
+      if (at >= a.off) at += a.r;
     }
+    const T* x = reinterpret_cast<const T*>(a.x) + (t * a.xt + h0 * a.xh + at);
+    T* o = reinterpret_cast<T*>(a.out) + (t * a.ot + h0 * a.oh + at);
+    const int64_t xs = a.xh * blockDim.y, os = a.oh * blockDim.y;
+    C lo[U], hi[U];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      if (token[k] < 0) continue;
-      T* o = reinterpret_cast<T*>(a.out) + dst[k] + first[k];
-      if (unit[k] >= a.units_rot) {
-        lo[k].store(o);
-        continue;
-      }
-      int64_t p = a.pos[token[k]];
-      p = p < 0 ? 0 : (p >= a.max_pos ? a.max_pos - 1 : p);
-      const float* cs = a.cos_sin + p * a.r;
-      if constexpr (VEC && !NEOX) {
-        constexpr int P = E / 2;  // pairs in the word
-        float c[P], s[P];
-        const float* q = cs + unit[k] * P;
-        if constexpr (P == 4) {
-          *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(q);
-          *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(q + half);
-        } else {
-          *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(q);
-          *reinterpret_cast<float2*>(s) = *reinterpret_cast<const float2*>(q + half);
+    for (int k = 0; k < U; ++k) {
+      if (h0 + k * (int)blockDim.y >= a.n_head) continue;
+      lo[k].load(x + k * xs);
+      if (TWO && rot) hi[k].load(x + k * xs + (NEOX ? half : 1));
+    }
+    if (rot) {
+      float c[P], s[P];
+      const float* q = cs + u * P;
+      if constexpr (P % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < P; e += 4) {
+          *reinterpret_cast<float4*>(c + e) = __ldg(reinterpret_cast<const float4*>(q + e));
+          *reinterpret_cast<float4*>(s + e) = __ldg(reinterpret_cast<const float4*>(q + half + e));
         }
+      } else if constexpr (P == 2) {
+        *reinterpret_cast<float2*>(c) = __ldg(reinterpret_cast<const float2*>(q));
+        *reinterpret_cast<float2*>(s) = __ldg(reinterpret_cast<const float2*>(q + half));
+      } else {
+        c[0] = __ldg(q);
+        s[0] = __ldg(q + half);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
 #pragma unroll
         for (int e = 0; e < P; ++e) {
+          T& x1 = TWO ? lo[k].v[e] : lo[k].v[(2 * e) % E];
+          T& x2 = TWO ? hi[k].v[e] : lo[k].v[(2 * e + 1) % E];
           float o1, o2;
-          rotate(to_f32(lo[k].v[2 * e]), to_f32(lo[k].v[2 * e + 1]), c[e], s[e], o1, o2);
-          lo[k].v[2 * e] = from_f32<T>(o1);
-          lo[k].v[2 * e + 1] = from_f32<T>(o2);
+          rotate(to_f32(x1), to_f32(x2), c[e], s[e], o1, o2);
+          x1 = from_f32<T>(o1);
+          x2 = from_f32<T>(o2);
         }
-        lo[k].store(o);
-      } else {
-        float c[E], s[E];
-        const float* q = cs + unit[k] * E;
-        if constexpr (VEC) {
+    }
 #pragma unroll
-          for (int e = 0; e < E; e += 4) {
-            *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(q + e);
-            *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(q + half + e);
-          }
-        } else {
-          c[0] = q[0];
-          s[0] = q[half];
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float o1, o2;
-          rotate(to_f32(lo[k].v[e]), to_f32(hi[k].v[e]), c[e], s[e], o1, o2);
-          lo[k].v[e] = from_f32<T>(o1);
-          hi[k].v[e] = from_f32<T>(o2);
-        }
-        lo[k].store(o);
-        hi[k].store(o + (NEOX ? half : 1));
-      }
+    for (int k = 0; k < U; ++k) {
+      if (h0 + k * (int)blockDim.y >= a.n_head) continue;
+      lo[k].store(o + k * os);
+      if (TWO && rot) hi[k].store(o + k * os + (NEOX ? half : 1));
     }
   }
 }
 
+template <typename T, bool NEOX, bool VEC>
+void launch(const RotaryArgs& a, cudaStream_t s) {
+  constexpr int U = kHeads<NEOX, VEC>;
+  // a block: the units of as many heads of a token as it takes, U a thread; where
+  // that leaves threads over, more tokens
+  const int x = std::min(a.units, kThreads);
+  const int y = std::min((a.n_head + U - 1) / U, kThreads / x);
+  const int z = std::min(std::min(kThreads / (x * y), 64), a.n_tok);
+  const dim3 grid((unsigned)((a.n_tok + z - 1) / z), (unsigned)((a.n_head + U * y - 1) / (U * y)));
+  rotary_kernel<T, NEOX, VEC><<<grid, dim3(x, y, z), 0, s>>>(a);
+}
+
 template <typename T>
-void launch(const RotaryArgs& a, bool neox, bool vec, dim3 grid, cudaStream_t s) {
+void launch(const RotaryArgs& a, bool neox, bool vec, cudaStream_t s) {
   if (neox)
-    vec ? rotary_kernel<T, true, true><<<grid, kThreads, 0, s>>>(a)
-        : rotary_kernel<T, true, false><<<grid, kThreads, 0, s>>>(a);
+    vec ? launch<T, true, true>(a, s) : launch<T, true, false>(a, s);
   else
-    vec ? rotary_kernel<T, false, true><<<grid, kThreads, 0, s>>>(a)
-        : rotary_kernel<T, false, false><<<grid, kThreads, 0, s>>>(a);
+    vec ? launch<T, false, true>(a, s) : launch<T, false, false>(a, s);
 }
 
 }  // namespace
@@ -230,26 +207,15 @@ extern "C" int dsa_rotary_embedding(void* out, int64_t out_tok_stride, int64_t o
   a.width = width;
   a.n_tok = n_tok;
   a.n_head = n_head;
-  a.copy = !(out == x && out_tok_stride == x_tok_stride && out_head_stride == x_head_stride);
+  const bool copy = !(out == x && out_tok_stride == x_tok_stride && out_head_stride == x_head_stride);
   a.units_rot = vec ? (rope_neox ? rotary_dim / 2 / e : rotary_dim / e) : rotary_dim / 2;
-  a.units = a.units_rot + (a.copy ? (width - rotary_dim) / (vec ? e : 1) : 0);
-  // units per block: 256 a pass, up to eight passes while the blocks still fill the GPU about four times
-  const int64_t total = (int64_t)n_tok * n_head * a.units;
-  const int nsm = sm_count(current_device());
-  const int64_t want = std::min<int64_t>(kMaxUnits, std::max<int64_t>(kThreads, total / ((int64_t)nsm * 4)));
-  a.heads_per_block = (int)std::min<int64_t>(n_head, std::max<int64_t>(1, want / a.units));
-  a.tokens_per_block = a.heads_per_block == n_head
-                           ? (int)std::min<int64_t>(n_tok, std::max<int64_t>(1, want / ((int64_t)n_head * a.units)))
-                           : 1;
-  a.mul_units = a.units == 1 ? 0u : (uint32_t)(((1ull << 32) + a.units - 1) / a.units);  // 0: the quotient is j
-  const dim3 grid((unsigned)((n_tok + a.tokens_per_block - 1) / a.tokens_per_block),
-                  (unsigned)((n_head + a.heads_per_block - 1) / a.heads_per_block));
+  a.units = a.units_rot + (copy ? (width - rotary_dim) / (vec ? e : 1) : 0);  // in place nothing is copied
   cudaStream_t s = as_stream(stream);
   if (dtype == DSA_F32)
-    launch<float>(a, rope_neox != 0, vec, grid, s);
+    launch<float>(a, rope_neox != 0, vec, s);
   else if (dtype == DSA_F16)
-    launch<__half>(a, rope_neox != 0, vec, grid, s);
+    launch<__half>(a, rope_neox != 0, vec, s);
   else
-    launch<__nv_bfloat16>(a, rope_neox != 0, vec, grid, s);
+    launch<__nv_bfloat16>(a, rope_neox != 0, vec, s);
   return check_launch("rotary_kernel");
 }
