@@ -107,7 +107,7 @@ struct TreeArgs {
   const int64_t* mask;
   void* o;
   float* lse;
-  float* part_o;   // [2 * pairs][slot_rows][512]
+  float* part_o;   // [2 * pairs][512 / 4][slot_rows][4]
   float* part_ml;  // [2 * pairs][slot_rows][2]
   Cut* cuts;       // [pairs]
   int64_t n_kv_rows, bt_stride, mask_stride;
@@ -178,6 +178,19 @@ struct Cursor {
     }
   }
 };
+
+// The segment that starts at c.
+template <bool FP8>
+__device__ __forceinline__ Segment segment_of(const Cursor& c) {
+  Segment sg;
+  sg.b = c.b;
+  sg.rt = c.rt;
+  sg.n = min(c.r.nt - c.tile, c.left);
+  sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
+  sg.nd = c.r.nd;
+  sg.flags = (FP8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
+  return sg;
+}
 
 // The start of a pair's run, by one warp.
 __device__ __forceinline__ Cursor find_run(const TreeArgs& p, int pair, int lane) {
@@ -267,6 +280,21 @@ __device__ __forceinline__ uint4 dequant8(uint2 v, uint32_t cut) {
   e4m3x4_to_half2x2(v.y, x[2], x[3]);
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = __hfma2(x[e], lo, __hmul2(x[e], hi));
+  return *reinterpret_cast<const uint4*>(x);
+}
+
+// What that rounding left, itself rounded: code * hi - x is exact.
+__device__ __forceinline__ uint4 rest8(uint2 v, uint32_t cut) {
+  const __half2 c = *reinterpret_cast<const __half2*>(&cut);
+  const __half2 hi = __low2half2(c), lo = __high2half2(c);
+  __half2 x[4];
+  e4m3x4_to_half2x2(v.x, x[0], x[1]);
+  e4m3x4_to_half2x2(v.y, x[2], x[3]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __half2 y = __hfma2(x[e], lo, __hmul2(x[e], hi));
+    x[e] = __hfma2(x[e], lo, __hfma2(x[e], hi, __hneg2(y)));
+  }
   return *reinterpret_cast<const uint4*>(x);
 }
 
@@ -365,11 +393,14 @@ __device__ __forceinline__ void row_codes(const TreeArgs& p, int b, const Req& r
   }
 }
 
+__device__ __forceinline__ void prefetch_line(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // This CTA's 64 query rows (f16, or bf16 as it is), by the producer warps: the last
 // three 64-column blocks into shared memory, the others by way of the K buffer,
 // which is free then, into tensor memory (twice, for its two lane halves). Warp w
 // loads rows 4w + lane / 8, eight lanes a row. qe[row]: the power of two that a
 // bf16 row was divided by.
+constexpr int kQLoads = 3;  // loads in flight, of 9
 template <int FMT>
 __device__ __forceinline__ void load_q(const TreeArgs& p, uint32_t base, uint32_t tmem, int8_t* qe, int b, int row0, int w,
                                        int lane) {
@@ -377,24 +408,36 @@ __device__ __forceinline__ void load_q(const TreeArgs& p, uint32_t base, uint32_
   const bool on = row0 + row < p.T * p.H;
   const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
                                                     ((int64_t)b * p.T * p.H + row0 + row) * DK * 2);
-  int e = 0;
-  if (FMT != DSA_BF16 && p.q_bf16) {
-    uint32_t bits = 0;
-    if (on) {
-#pragma unroll 3
-      for (int c = 0; c < 9; ++c) bits = max(bits, bf16x8_max_abs_bits(__ldg(src + l8 + 8 * c)));
+  auto at = [&](int c) {
+    return base + (c < kQtBlks ? SM_K + c * kBlk : SM_Q + (c - kQtBlks) * kBlk) + sw128_off(row, l8);
+  };
+  if (on) {  // the row's nine lines come from memory together
+    prefetch_line(src + 8 * l8);
+    if (l8 == 0) prefetch_line(src + 64);
+  }
+  const bool scaled = FMT != DSA_BF16 && p.q_bf16;
+  uint32_t bits = 0;
+#pragma unroll 1
+  for (int c0 = 0; c0 < 9; c0 += kQLoads) {
+    uint4 v[kQLoads];
+#pragma unroll
+    for (int k = 0; k < kQLoads; ++k)
+      v[k] = on && c0 + k < 9 ? __ldg(src + l8 + 8 * (c0 + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < kQLoads; ++k) {
+      if (scaled) bits = max(bits, bf16x8_max_abs_bits(v[k]));
+      v[k] = make_uint4(v[k].x ^ p.q_sign, v[k].y ^ p.q_sign, v[k].z ^ p.q_sign, v[k].w ^ p.q_sign);
+      if (c0 + k < 9) sts16(at(c0 + k), v[k]);
     }
+  }
+  int e = 0;
+  if (scaled) {
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
     e = bf16_fp16_shift(bits);
-  }
-#pragma unroll 3
-  for (int c = 0; c < 9; ++c) {
-    uint4 v = on ? __ldg(src + l8 + 8 * c) : make_uint4(0, 0, 0, 0);
-    if (FMT != DSA_BF16 && p.q_bf16) v = bf16x8_to_half8_scaled(v, e);
-    v = make_uint4(v.x ^ p.q_sign, v.y ^ p.q_sign, v.z ^ p.q_sign, v.w ^ p.q_sign);
-    sts16(base + (c < kQtBlks ? SM_K + c * kBlk : SM_Q + (c - kQtBlks) * kBlk) + sw128_off(row, l8), v);
+#pragma unroll 1
+    for (int c = 0; c < 9; ++c) sts16(at(c), bf16x8_to_half8_scaled(lds16(at(c)), e));
   }
   if (l8 == 0) qe[row] = (int8_t)e;
   named_bar(2, kProducers * 32);
@@ -476,6 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     c = find_run(p, pair, lane);
     if (lane == 0) {
       *run_tiles = c.left;
+      if (c.left > 0) segs[0] = segment_of<kFp8>(c);
       if (rank == 0) p.cuts[pair] = Cut{c.b, c.rt, c.tile, c.r.nt, c.chunk, {0, 0, 0}};
     }
   }
@@ -504,9 +548,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     int kc = 0;             // K stores so far (two per tile in two-pass segments)
     int seg = 0, left = 0;  // the segment of the next K store, and its tiles left
     bool two = false;
-    // before a K store: the next segment's Q, when its first tile is due
+    // the next segment's Q, through the K buffer
     auto enter = [&]() {
-      if (left > 0) return;
       const Segment& sg = segs[seg % kSegs];  // visible: the wait for this tile's rows
       const bool live = !named_bar_or(2, kProducers * 32, !ok);  // all take the same number of barriers
       left = live ? sg.n : 1 << 30;
@@ -594,14 +637,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       };
       // `rest`: what the first of two passes rounded away
       auto put_k = [&](bool rest) {
-        if (!two && __all_sync(0xffffffffu, fast_scale(ks))) {
+        if (__all_sync(0xffffffffu, fast_scale(ks))) {
           const uint32_t cut = cut_scale(ks);
+          if (!rest) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
-                    dequant8(kd[x][h], __shfl_sync(0xffffffffu, cut, 4 * x + 2 * h + (lane >> 4))));
+              for (int h = 0; h < 2; ++h)
+                sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
+                      dequant8(kd[x][h], __shfl_sync(0xffffffffu, cut, 4 * x + 2 * h + (lane >> 4))));
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
+                      rest8(kd[x][h], __shfl_sync(0xffffffffu, cut, 4 * x + 2 * h + (lane >> 4))));
+          }
           return;
         }
 #pragma unroll 1
@@ -615,11 +667,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         }
       };
       auto store_k = [&](int t) {
+        if (left <= 0) {
+          if (t > 0) {
+            wait(mb_raw_full, t & 1);  // the segment's descriptor is visible
+            wait(mb_k_free, (kc - 1) & 1);
+          }
+          enter();
+        }
         take(t);
 #pragma unroll 1
         for (int s = 0; s == 0 || (s == 1 && two); ++s) {
           if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
-          if (s == 0) enter();
           if (ok) put_k(s == 1);
           fence_proxy_async();
           fence_before_sync();  // Q's tensor-memory stores
@@ -654,10 +712,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
       };
       auto store_k = [&](int t) {
+        if (left <= 0 && t == 0) enter();
         wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
         const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
         if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
-        enter();
+        if (left <= 0) enter();
         if (ok) {
           const uint8_t* row = p.kv + (int64_t)max(code, 0) * kRowBytes + 16 * l8;
 #pragma unroll
@@ -715,16 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       } else {
         if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
       }
-      if (ok && c.first && lane == 0) {
-        Segment sg;
-        sg.b = c.b;
-        sg.rt = c.rt;
-        sg.n = min(c.r.nt - c.tile, c.left);
-        sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
-        sg.nd = c.r.nd;
-        sg.flags = (kFp8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
-        segs[seg % kSegs] = sg;
-      }
+      if (ok && c.first && t > 0 && lane == 0) segs[seg % kSegs] = segment_of<kFp8>(c);
       if constexpr (kFp8) {
         int mine[2];
         uint32_t bytes = 0;
@@ -1060,9 +1110,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
               dst[e] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           } else if (mine) {
-            uint4* dst = reinterpret_cast<uint4*>(p.part_o + prow_i * DV + col0 + 32 * k);
+            uint4* dst = reinterpret_cast<uint4*>(p.part_o) + ((int64_t)slot * (DV / 4) + (col0 + 32 * k) / 4) * p.slot_rows +
+                         kRows * rank + row;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 8; ++e)
+              dst[(int64_t)e * p.slot_rows] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
         if (mine && q4 == 0) {
@@ -1093,24 +1145,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 }
 
 // Row tiles whose key tiles lie in several segments: o = sum_s w_s o_s / sum_s w_s
-// l_s with w_s = 2^(m_s - max m), four warps a row, 128 columns each. Such a tile is
-// cut where a pair's run starts inside it; kMergeBlocks blocks belong to each of
-// these starts, and those of a tile's first one merge it. The last B * tiles
-// blocks write the row tiles that no segment holds: o = 0, lse = -inf.
-constexpr int kMergeRows = 2;
-constexpr int kMergeBlocks = kPairRows / kMergeRows;
-__device__ __forceinline__ void store_merged(const TreeArgs& p, int64_t at, float4 v) {
-  uint2 x;
-  if (p.o_bf16) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-    x = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-  } else {
-    x = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
-  }
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.o) + at * 2) = x;
+// l_s with w_s = 2^(m_s - max m). A lane takes a row and 16 columns of it, so that
+// a warp reads 32 rows' neighbouring vectors. Such a tile is cut where a pair's run
+// starts inside it; kMergeBlocks blocks belong to each of these starts, and those
+// of a tile's first one merge it. The last B * tiles blocks write the row tiles
+// that no segment holds: o = 0, lse = -inf.
+constexpr int kMergeWarps = 8;
+constexpr int kMergeCols = 16;                                                  // of a lane
+constexpr int kMergeBlocks = (kPairRows / 32) * (DV / kMergeCols) / kMergeWarps;
+__device__ __forceinline__ uint32_t pack_out(const TreeArgs& p, float a, float b) {
+  if (!p.o_bf16) return pack_half2(a, b);
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
 
-__global__ void __launch_bounds__(128 * kMergeRows) tree_merge_kernel(const TreeArgs p) {
+__global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const TreeArgs p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.T * p.H;
   const int cuts = (p.pairs - 1) * kMergeBlocks;
@@ -1122,10 +1171,11 @@ __global__ void __launch_bounds__(128 * kMergeRows) tree_merge_kernel(const Tree
     const Req q = load_req(p, b);
     if (q.nt > 0 && rt < q.nrt) return;
     const int end = min(rows, (rt + 1) * kPairRows);
-    for (int r = rt * kPairRows + warp; r < end; r += 4 * kMergeRows) {
+    for (int r = rt * kPairRows + warp; r < end; r += kMergeWarps) {
       const int64_t grow = (int64_t)b * rows + r;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) store_merged(p, grow * DV + 128 * c + 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
+      uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.o) + grow * DV * 2);
+      o[lane] = make_uint4(0, 0, 0, 0);
+      o[lane + 32] = make_uint4(0, 0, 0, 0);
       if (lane == 0) p.lse[grow] = -INFINITY;
     }
     return;
@@ -1133,51 +1183,54 @@ __global__ void __launch_bounds__(128 * kMergeRows) tree_merge_kernel(const Tree
   const int pair = 1 + blockIdx.x / kMergeBlocks;
   const Cut cut = p.cuts[pair];
   if (cut.tile == 0 || cut.tile > cut.chunk) return;  // no cut, or not the tile's first
-  const int row = (int)(blockIdx.x % kMergeBlocks) * kMergeRows + (warp >> 2);  // of the row tile
+  const int item = (int)(blockIdx.x % kMergeBlocks) * kMergeWarps + warp;
+  const int row = 32 * (item % (kPairRows / 32)) + lane;  // of the row tile
+  const int col = kMergeCols * (item / (kPairRows / 32));
   if (cut.rt * kPairRows + row >= rows) return;
-  const int64_t grow = (int64_t)cut.b * rows + cut.rt * kPairRows + row;
   const int n = 1 + (cut.nt - cut.tile + cut.chunk - 1) / cut.chunk;  // segments
   // the first one is slot 0 if the tile starts where its pair's run does, else slot 1
-  auto state = [&](int i) {
-    return (int64_t)(2 * (pair - 1 + i) + (i == 0 && cut.tile < cut.chunk ? 1 : 0)) * p.slot_rows + row;
-  };
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  auto slot = [&](int i) { return 2 * (pair - 1 + i) + (i == 0 && cut.tile < cut.chunk ? 1 : 0); };
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row;
   float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) {
-    const float2 x = ml[state(i)];
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float2 x = ml[(int64_t)slot(i) * p.slot_rows];
     if (x.y > 0.f) M = fmaxf(M, x.x);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float* po = p.part_o + 128 * (warp & 3) + 4 * lane;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    float w = 0.f;
-    if (i0 + lane < n) {
-      const float2 x = ml[state(i0 + lane)];
-      if (x.y > 0.f) w = exp2f(x.x - M);
-      L += x.y == 0.f ? 0.f : x.y * (x.y > 0.f ? w : 1.f);  // a NaN stays one
-    }
-    const int m = min(32, n - i0);
-#pragma unroll 4
-    for (int j = 0; j < m; ++j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const float4 v = *reinterpret_cast<const float4*>(po + state(i0 + j) * DV);
-      if (wj != 0.f) {
-        acc.x = fmaf(v.x, wj, acc.x);
-        acc.y = fmaf(v.y, wj, acc.y);
-        acc.z = fmaf(v.z, wj, acc.z);
-        acc.w = fmaf(v.w, wj, acc.w);
-      }
+  float acc[kMergeCols];
+#pragma unroll
+  for (int c = 0; c < kMergeCols; ++c) acc[c] = 0.f;
+  const float4* po = reinterpret_cast<const float4*>(p.part_o) + (int64_t)(col / 4) * p.slot_rows + row;
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const float2 x = ml[(int64_t)slot(i) * p.slot_rows];
+    const float4* at = po + (int64_t)slot(i) * (DV / 4) * p.slot_rows;
+    float4 v[kMergeCols / 4];
+#pragma unroll
+    for (int c = 0; c < kMergeCols / 4; ++c) v[c] = at[(int64_t)c * p.slot_rows];
+    if (x.y == 0.f) continue;  // saw nothing
+    const float w = x.y > 0.f ? exp2f(x.x - M) : 1.f;
+    L += x.y * w;  // a NaN stays one
+#pragma unroll
+    for (int c = 0; c < kMergeCols / 4; ++c) {
+      acc[4 * c] = fmaf(v[c].x, w, acc[4 * c]);
+      acc[4 * c + 1] = fmaf(v[c].y, w, acc[4 * c + 1]);
+      acc[4 * c + 2] = fmaf(v[c].z, w, acc[4 * c + 2]);
+      acc[4 * c + 3] = fmaf(v[c].w, w, acc[4 * c + 3]);
     }
   }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int64_t grow = (int64_t)cut.b * rows + cut.rt * kPairRows + row;
+  uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.o) + (grow * DV + col) * 2);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  const float inv = L > 0.f ? 1.f / L : L;
-  store_merged(p, grow * DV + 128 * (warp & 3) + 4 * lane,
-               make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-  if (lane == 0 && (warp & 3) == 0) p.lse[grow] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  for (int c = 0; c < kMergeCols / 8; ++c) {
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = pack_out(p, acc[8 * c + 2 * e] * inv, acc[8 * c + 2 * e + 1] * inv);
+    o[c] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  if (col == 0) p.lse[grow] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 std::once_flag g_once[kMaxDevices];
@@ -1335,7 +1388,7 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((int64_t)B * rt + (int64_t)(p.pairs - 1) * kMergeBlocks));
-  cfg.blockDim = dim3(128 * kMergeRows);
+  cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = s;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
