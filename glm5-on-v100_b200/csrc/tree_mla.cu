@@ -436,7 +436,7 @@ __device__ __forceinline__ void load_q(const TreeArgs& p, uint32_t base, uint32_
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
     e = bf16_fp16_shift(bits);
-#pragma unroll 1
+#pragma unroll 3
     for (int c = 0; c < 9; ++c) sts16(at(c), bf16x8_to_half8_scaled(lds16(at(c)), e));
   }
   if (l8 == 0) qe[row] = (int8_t)e;
@@ -1145,13 +1145,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 }
 
 // Row tiles whose key tiles lie in several segments: o = sum_s w_s o_s / sum_s w_s
-// l_s with w_s = 2^(m_s - max m). A lane takes a row and 16 columns of it, so that
+// l_s with w_s = 2^(m_s - max m). A lane takes a row and 8 columns of it, so that
 // a warp reads 32 rows' neighbouring vectors. Such a tile is cut where a pair's run
 // starts inside it; kMergeBlocks blocks belong to each of these starts, and those
 // of a tile's first one merge it. The last B * tiles blocks write the row tiles
 // that no segment holds: o = 0, lse = -inf.
 constexpr int kMergeWarps = 8;
-constexpr int kMergeCols = 16;                                                  // of a lane
+constexpr int kMergeCols = 8;                                                   // of a lane
 constexpr int kMergeBlocks = (kPairRows / 32) * (DV / kMergeCols) / kMergeWarps;
 __device__ __forceinline__ uint32_t pack_out(const TreeArgs& p, float a, float b) {
   if (!p.o_bf16) return pack_half2(a, b);
@@ -1202,22 +1202,22 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const Tree
 #pragma unroll
   for (int c = 0; c < kMergeCols; ++c) acc[c] = 0.f;
   const float4* po = reinterpret_cast<const float4*>(p.part_o) + (int64_t)(col / 4) * p.slot_rows + row;
-#pragma unroll 2
+#pragma unroll 4
   for (int i = 0; i < n; ++i) {
     const float2 x = ml[(int64_t)slot(i) * p.slot_rows];
     const float4* at = po + (int64_t)slot(i) * (DV / 4) * p.slot_rows;
     float4 v[kMergeCols / 4];
 #pragma unroll
     for (int c = 0; c < kMergeCols / 4; ++c) v[c] = at[(int64_t)c * p.slot_rows];
-    if (x.y == 0.f) continue;  // saw nothing
-    const float w = x.y > 0.f ? exp2f(x.x - M) : 1.f;
-    L += x.y * w;  // a NaN stays one
+    // 0: saw nothing; a NaN stays one
+    const float w = x.y == 0.f ? 0.f : x.y > 0.f ? exp2f(x.x - M) : 1.f;
+    L += x.y * w;
 #pragma unroll
     for (int c = 0; c < kMergeCols / 4; ++c) {
-      acc[4 * c] = fmaf(v[c].x, w, acc[4 * c]);
-      acc[4 * c + 1] = fmaf(v[c].y, w, acc[4 * c + 1]);
-      acc[4 * c + 2] = fmaf(v[c].z, w, acc[4 * c + 2]);
-      acc[4 * c + 3] = fmaf(v[c].w, w, acc[4 * c + 3]);
+      acc[4 * c] = x.y == 0.f ? acc[4 * c] : fmaf(v[c].x, w, acc[4 * c]);
+      acc[4 * c + 1] = x.y == 0.f ? acc[4 * c + 1] : fmaf(v[c].y, w, acc[4 * c + 1]);
+      acc[4 * c + 2] = x.y == 0.f ? acc[4 * c + 2] : fmaf(v[c].z, w, acc[4 * c + 2]);
+      acc[4 * c + 3] = x.y == 0.f ? acc[4 * c + 3] : fmaf(v[c].w, w, acc[4 * c + 3]);
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
