@@ -339,24 +339,24 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mbar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
 // Bounded wait in few instructions, for loops whose code has to fit the
-// instruction cache: up to 2^20 tries, each suspended for at most about 2 us.
-// False when they ran out; the caller records it.
-__device__ __forceinline__ bool mbar_wait_tries(uint32_t mbar, uint32_t parity) {
+// instruction cache: one try and up to `more` others, each suspended for at most
+// about 2 us. False when they ran out; the caller records it.
+__device__ __forceinline__ bool mbar_wait_tries(uint32_t mbar, uint32_t parity, uint32_t more) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       ".reg .u32 n;\n\t"
-      "mov.u32 n, 1048576;\n"
+      "mov.u32 n, %4;\n"
       "WAIT_%=:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "@p bra DONE_%=;\n\t"
-      "sub.u32 n, n, 1;\n\t"
       "setp.ne.u32 q, n, 0;\n\t"
+      "sub.u32 n, n, 1;\n\t"
       "@q bra WAIT_%=;\n"
       "DONE_%=:\n\t"
       "selp.b32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(mbar), "r"(parity), "r"(2000u)
+      : "r"(mbar), "r"(parity), "r"(2000u), "r"(more)
       : "memory");
   return ok != 0;
 }

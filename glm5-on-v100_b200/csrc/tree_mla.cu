@@ -227,6 +227,10 @@ __device__ __forceinline__ Cursor find_run(const TreeArgs& p, int pair, int lane
   }
 }
 
+// A value that a warp's lanes have in common, in a register of the warp: where branches
+// are known to be uniform, warp-wide instructions need no code to gather their lanes.
+__device__ __forceinline__ int uniform(uint32_t x) { return (int)__reduce_or_sync(0xffffffffu, x); }
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -488,8 +492,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   int* ring = reinterpret_cast<int*>(sm + SM_RING);             // [kRing][128]
   Segment* segs = reinterpret_cast<Segment*>(misc + kSegAt);    // [kSegs]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_rank();
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = uniform(cluster_rank());
   const int pair = blockIdx.x >> 1;
 
   Cursor c{};  // the row warp's
@@ -528,15 +532,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   cluster_sync();  // both CTAs' barriers exist and TMEM is allocated
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const int total = *run_tiles;
+  const int total = uniform(*run_tiles);
 
-  bool ok = true;
-  // By a whole warp: `ok` stays uniform.
+  uint32_t ok = 1;
+  // By a whole warp: `ok` stays uniform. The compiler is not to know that it is 0 after
+  // a wait that ran out: it would write the rest of the loop a second time for that.
   auto wait = [&](uint32_t mbar, uint32_t parity) {
-    if (ok && !__all_sync(0xffffffffu, mbar_wait_tries(mbar, parity))) {
-      ok = false;
-      if (lane == 0) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
-    }
+    const bool got = __all_sync(0xffffffffu, mbar_wait_tries(mbar, parity, ok << 20));
+    if (!got && ok && lane == 0) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
+    ok = got ? ok : 0;
+    asm volatile("" : "+r"(ok));
   };
   // After a wait that ran out (`ok` false) every thread of its warp still
   // executes its role's barriers and arrivals, and later waits return at once.
@@ -552,11 +557,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     auto enter = [&]() {
       const Segment& sg = segs[seg % kSegs];  // visible: the wait for this tile's rows
       const bool live = !named_bar_or(2, kProducers * 32, !ok);  // all take the same number of barriers
-      left = live ? sg.n : 1 << 30;
-      two = live && (sg.flags & kTwo) != 0;
+      left = live ? uniform(sg.n) : 1 << 30;
+      two = live && (uniform(sg.flags) & kTwo) != 0;
       if (live)
         load_q<FMT>(p, base, tmem, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
-      ok = ok && live;
+      ok = live ? ok : 0;
+      asm volatile("" : "+r"(ok));
       __syncwarp();
       if (lane == 0) mbar_arrive(mb_q_full + 8 * (seg % kQeSegs));
       ++seg;
@@ -823,8 +829,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       for (int t = 0; t < total; ++t) {
         wait(mb_raw_full, t & 1);
         if (left == 0 && ok) {
-          left = segs[seg % kSegs].n;
-          two = (segs[seg % kSegs].flags & kTwo) != 0;
+          left = uniform(segs[seg % kSegs].n);
+          two = (uniform(segs[seg % kSegs].flags) & kTwo) != 0;
           ++seg;
         }
         const uint32_t raw = base + SM_RAW + (32 * w + (lane >> 3)) * 656 + 528 + 16 * (lane & 7);
@@ -878,8 +884,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           wait(mb_k_full, kc & 1);
           if (!ok) return;
           if (qleft == 0) {  // its first tile is stored, so its descriptor is visible
-            qleft = segs[qseg % kSegs].n;
-            passes = segs[qseg % kSegs].flags & kTwo ? 2 : 1;
+            qleft = uniform(segs[qseg % kSegs].n);
+            passes = uniform(segs[qseg % kSegs].flags) & kTwo ? 2 : 1;
             ++qseg;
           }
           if (s == 0 && gq > 0) {  // the softmax has read S(gq - 1)
@@ -915,7 +921,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (first) {
           // the accumulator of the segment before has been read
           if (pseg > 0) wait(mb_o_free, (pseg - 1) & 1);
-          if (ok) pleft = segs[pseg % kSegs].n;
+          if (ok) pleft = uniform(segs[pseg % kSegs].n);
           ++pseg;
         }
         if (ok) {
@@ -962,9 +968,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll 1
     for (int seg = 0; g < total; ++seg) {
       wait(mb_q_full + 8 * (seg % kQeSegs), (seg / kQeSegs) & 1);
-      ok = !named_bar_or(1, kSoftmaxWarps * 32, !ok);  // all take the same number of barriers
+      ok = named_bar_or(1, kSoftmaxWarps * 32, !ok) ? 0 : 1;  // all take the same number of barriers
+      asm volatile("" : "+r"(ok));
       const Segment& sg = segs[seg % kSegs];
-      const int end = ok ? g + sg.n : total;
+      const int end = ok ? g + uniform(sg.n) : total;
       // positions before the drafts, from this thread's first key of the tile on
       int d = -64;
       if (ok && (sg.rt * kPairRows + kRows * rank + row) / p.H < sg.nd) d = max(sg.pre - kofs, -64);
