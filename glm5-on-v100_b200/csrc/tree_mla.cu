@@ -87,7 +87,8 @@ constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kNoMax = -1e30f;
 constexpr int kMaxSeq = 0x7fffff00;   // tile ends stay in 32 bits
 constexpr float kRescale = 8.0f;       // log2 units
-constexpr int kTwoPassKeys = 512;      // fp8: the remainder of the rounding is multiplied up to here
+constexpr int kTwoPassKeys = 32768;    // fp8: two products to a score up to here
+constexpr int kFineKeys = 1024;        // and up to here the second is the rounding's remainder
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kSlotF = DV + 2;         // f32 of a row's partial state: o, then m and l
 
@@ -150,9 +151,9 @@ struct Segment {
   int n;      // key tiles
   int pre;    // context positions less those before the first tile
   int nd;     // drafts of the request
-  int flags;  // kTwo: two-pass products | kFull: every key tile of the row tile
+  int flags;  // kTwo: two-pass products, kFine: of the rounding's remainder | kFull: every key tile of the row tile
 };
-enum { kTwo = 1, kFull = 2 };
+enum { kTwo = 1, kFull = 2, kFine = 4 };
 constexpr uint32_t SMEM_BYTES = SM_MISC + kSegAt + kSegs * (uint32_t)sizeof(Segment);
 static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 
@@ -188,7 +189,7 @@ __device__ __forceinline__ Segment segment_of(const Cursor& c) {
   sg.n = min(c.r.nt - c.tile, c.left);
   sg.pre = c.r.seq - c.r.nd - c.tile * kKeys;
   sg.nd = c.r.nd;
-  sg.flags = (FP8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (sg.n == c.r.nt ? kFull : 0);
+  sg.flags = (FP8 && c.r.seq <= kTwoPassKeys ? kTwo : 0) | (FP8 && c.r.seq <= kFineKeys ? kFine : 0) | (sg.n == c.r.nt ? kFull : 0);
   return sg;
 }
 
@@ -287,24 +288,45 @@ __device__ __forceinline__ uint4 dequant8(uint2 v, uint32_t cut) {
   return *reinterpret_cast<const uint4*>(x);
 }
 
-// What that rounding left, itself rounded: code * hi - x is exact.
-__device__ __forceinline__ uint4 rest8(uint2 v, uint32_t cut) {
-  const __half2 c = *reinterpret_cast<const __half2*>(&cut);
-  const __half2 hi = __low2half2(c), lo = __high2half2(c);
+// With one of the two parts, as f16 (hi: exact): the two products' sum keeps the scale
+// to 2^-18, or to 2^-25 of the largest value where f16 runs out of exponents.
+__device__ __forceinline__ uint4 dequant8_part(uint2 v, __half part) {
+  __half2 x[4];
+  e4m3x4_to_half2x2(v.x, x[0], x[1]);
+  e4m3x4_to_half2x2(v.y, x[2], x[3]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = __hmul2(x[e], __half2half2(part));
+  return *reinterpret_cast<const uint4*>(x);
+}
+
+// The scale's part after hi times 256, itself cut in two: 29 bits of the scale in all.
+__device__ __forceinline__ uint32_t cut_rest(float sc) {
+  const float lo = (sc - __uint_as_float(__float_as_uint(sc) & 0xFFFE0000u)) * 256.f;
+  const __half h = __float2half_rn(lo);
+  return pack_half2(__half2float(h), lo - __half2float(h));
+}
+
+// What dequant8's rounding left, itself rounded. Its value y lies so near code * hi
+// that the difference is exact; the small parts take code / 256.
+__device__ __forceinline__ uint4 rest8(uint2 v, uint32_t cut, uint32_t small) {
+  const __half2 c = *reinterpret_cast<const __half2*>(&cut), d = *reinterpret_cast<const __half2*>(&small);
+  const __half2 hi = __low2half2(c), lo = __high2half2(c), lo1 = __low2half2(d), lo2 = __high2half2(d);
   __half2 x[4];
   e4m3x4_to_half2x2(v.x, x[0], x[1]);
   e4m3x4_to_half2x2(v.y, x[2], x[3]);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const __half2 y = __hfma2(x[e], lo, __hmul2(x[e], hi));
-    x[e] = __hfma2(x[e], lo, __hfma2(x[e], hi, __hneg2(y)));
+    const __half2 z = __hmul2(x[e], __float2half2_rn(0x1p-8f));
+    x[e] = __hfma2(z, lo2, __hfma2(z, lo1, __hfma2(x[e], hi, __hneg2(y))));
   }
   return *reinterpret_cast<const uint4*>(x);
 }
 
 // The same for any scale, or with `rest` what that rounding left, itself rounded.
 // Rare: kept out of the loops' code, which has to fit the instruction cache.
-__device__ __noinline__ uint4 dequant8_any(uint2 v, float sc, bool rest) {
+__device__ __noinline__ uint4 dequant8_any(uint2 v, float sc, bool rest, bool fast) {
+  if (fast) return rest8(v, cut_scale(sc), cut_rest(sc));
   __half2 x[4];
   e4m3x4_to_half2x2(v.x, x[0], x[1]);
   e4m3x4_to_half2x2(v.y, x[2], x[3]);
@@ -483,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   const uint32_t mb_k_full = mb, mb_k_free = mb + 8, mb_v_full = mb + 16, mb_v_free = mb + 24, mb_p_full = mb + 32,
                  mb_o_free = mb + 40, mb_done = mb + 48, mb_s_full = mb + 56, mb_s_free = mb + 64,
                  mb_q_full = mb + 72 /* [3] */, mb_r_full = mb + 96 /* [3] */, mb_r_free = mb + 120 /* [3] */,
-                 mb_raw_full = mb + 144, mb_raw_free = mb + 152;
+                 mb_raw_full = mb + 144, mb_raw_free = mb + 152, mb_pv = mb + 160;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + kWordsAt);
   int* run_tiles = reinterpret_cast<int*>(misc + kWordsAt + 8);
   uint32_t* raw_valid = reinterpret_cast<uint32_t*>(misc + kWordsAt + 16);  // [2]: rows that lie in the raw buffer
@@ -513,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         mbar_init(mb_r_full + 8 * x, 1);
         mbar_init(mb_r_free + 8 * x, kProducers + (kFp8 ? 0 : kTailWarps));
       }
+      mbar_init(mb_pv, 1);
       mbar_init(mb_raw_full, 1);
       mbar_init(mb_raw_free, kProducers + kTailWarps);
       mbar_init_fence();
@@ -547,18 +570,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   // executes its role's barriers and arrivals, and later waits return at once.
   if (warp < kProducers) {
     // ------------------------------------------------------------- producers
-    // K(t+1) is stored under PV(t-1), V(t) under QK(t+1).
+    // K(t+1) is stored under PV(t-1), V(t) under QK(t+1); with two passes the first
+    // of K(t+1) under QK(t), the second under PV(t).
     const int w = warp;
     const uint32_t k_full0 = cluster_map(mb_k_full, 0), v_full0 = cluster_map(mb_v_full, 0);
-    int kc = 0;             // K stores so far (two per tile in two-pass segments)
     int seg = 0, left = 0;  // the segment of the next K store, and its tiles left
-    bool two = false;
+    // The flags of the next K's segment, those of the next V's three bits up, and the
+    // parities of the number of K and of V stores so far. A wait for the buffer's next
+    // release goes by the parity's complement: at once before the first.
+    constexpr int kVShift = 3, kKOdd = 64, kVOdd = 128;
+    int st = 0;
+    auto wait_k = [&]() { wait(mb_k_free, st & kKOdd ? 0 : 1); };
+    auto wait_v = [&]() { wait(mb_v_free, st & kVOdd ? 0 : 1); };
     // the next segment's Q, through the K buffer
     auto enter = [&]() {
       const Segment& sg = segs[seg % kSegs];  // visible: the wait for this tile's rows
       const bool live = !named_bar_or(2, kProducers * 32, !ok);  // all take the same number of barriers
       left = live ? uniform(sg.n) : 1 << 30;
-      two = live && (uniform(sg.flags) & kTwo) != 0;
+      st = (st & ~(kTwo | kFine | kFull)) | (live ? uniform(sg.flags) : 0);
       if (live)
         load_q<FMT>(p, base, tmem, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
       ok = live ? ok : 0;
@@ -597,8 +626,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       const uint32_t v_at = base + SM_V + (lane >> 3) * kVBlk + sw128_off(4 * w, lane & 7);
       // The loops below for any scales are rolled, with row 0's registers taken and the
       // others moved down, so that they cost little code.
-      auto put_v = [&]() {
-        if (__all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps))) {
+      auto put_v = [&](bool rest) {
+        const bool fast = __all_sync(0xffffffffu, fast_scale(vs) && fast_scale(ps));
+        if (fast && !rest) {
           const uint32_t vcut = cut_scale(vs), pcut = cut_scale(ps);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -614,9 +644,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         for (int x = 0; x < 8; ++x) {  // own rows, then the other CTA's
           const bool own = x < 4;
           const float sc = __shfl_sync(0xffffffffu, own ? vs : ps, (own ? 4 * x + 2 * rank : 2 * (x - 4)) + (lane >> 4));
-          sts16((v_at ^ (16 * (x & 3))) + 128 * (x & 3) + 8192 * (own ? rank : rank ^ 1), dequant8_any(vd[0], sc, false));
+          const uint4 v = dequant8_any(vd[0], sc, rest, fast);
+          sts16((v_at ^ (16 * (x & 3))) + 128 * (x & 3) + 8192 * (own ? rank : rank ^ 1), v);
+          const uint2 first = vd[0];
           vd[0] = vd[1], vd[1] = vd[2], vd[2] = vd[3], vd[3] = pd[0];
-          pd[0] = pd[1], pd[1] = pd[2], pd[2] = pd[3];
+          pd[0] = pd[1], pd[1] = pd[2], pd[2] = pd[3], pd[3] = first;
         }
       };
       auto take = [&](int t) {
@@ -641,72 +673,84 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         __syncwarp();
         if (lane == 0) mbar_arrive(mb_raw_free);
       };
-      // `rest`: what the first of two passes rounded away
+      // `rest`: what rounding takes away
       auto put_k = [&](bool rest) {
-        if (__all_sync(0xffffffffu, fast_scale(ks))) {
-          const uint32_t cut = cut_scale(ks);
-          if (!rest) {
+        const bool fast = __all_sync(0xffffffffu, fast_scale(ks));
+        const uint32_t cut = cut_scale(ks);
+        if (fast && (!(st & kTwo) || (!rest && (st & kFine)))) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 4; ++x)
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
-                      dequant8(kd[x][h], __shfl_sync(0xffffffffu, cut, 4 * x + 2 * h + (lane >> 4))));
-          } else {
+            for (int h = 0; h < 2; ++h)
+              sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
+                    dequant8(kd[x][h], __shfl_sync(0xffffffffu, cut, 4 * x + 2 * h + (lane >> 4))));
+          return;
+        }
+        if (fast && !(st & kFine)) {
+          const uint32_t part = rest ? cut >> 16 : cut;
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 4; ++x)
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
-                      rest8(kd[x][h], __shfl_sync(0xffffffffu, cut, 4 * x + 2 * h + (lane >> 4))));
-          }
+            for (int h = 0; h < 2; ++h)
+              sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h,
+                    dequant8_part(kd[x][h], __ushort_as_half((unsigned short)__shfl_sync(
+                                                0xffffffffu, part, 4 * x + 2 * h + (lane >> 4)))));
           return;
         }
 #pragma unroll 1
         for (int i = 0; i < 8; ++i) {
           const int x = i >> 1, h = i & 1;
           const float sc = __shfl_sync(0xffffffffu, ks, 4 * x + 2 * h + (lane >> 4));
-          sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h, dequant8_any(kd[0][0], sc, rest));
+          const uint4 v = dequant8_any(kd[0][0], sc, rest, fast);
+          sts16((k_at ^ (16 * x)) + 128 * x + 4 * kBlk * h, v);
           const uint2 first = kd[0][0];
           kd[0][0] = kd[0][1], kd[0][1] = kd[1][0], kd[1][0] = kd[1][1], kd[1][1] = kd[2][0];
           kd[2][0] = kd[2][1], kd[2][1] = kd[3][0], kd[3][0] = kd[3][1], kd[3][1] = first;
         }
       };
-      auto store_k = [&](int t) {
+      auto begin_k = [&](int t) {
         if (left <= 0) {
           if (t > 0) {
             wait(mb_raw_full, t & 1);  // the segment's descriptor is visible
-            wait(mb_k_free, (kc - 1) & 1);
+            wait_k();
           }
           enter();
         }
         take(t);
-#pragma unroll 1
-        for (int s = 0; s == 0 || (s == 1 && two); ++s) {
-          if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
-          if (ok) put_k(s == 1);
-          fence_proxy_async();
-          fence_before_sync();  // Q's tensor-memory stores
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(k_full0);
-          ++kc;
-        }
         --left;
       };
 #pragma unroll 1
       for (int t = 0; t <= total; ++t) {
-        if (t < total) store_k(t);
-        if (t > 0) {  // V of tile t - 1
-          if (t > 1) wait(mb_v_free, t & 1);
-          if (ok) put_v();
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(v_full0);
+        if (t < total) begin_k(t);
+        // K of tile t, or first what rounding takes from it; V of tile t - 1; then K
+#pragma unroll 1
+        for (int s = 0; s < 2; ++s) {
+          if (t < total && (s == 0 || (st & kTwo))) {
+            wait_k();
+            if (ok) put_k(s == 0 && (st & kTwo));
+            fence_proxy_async();
+            fence_before_sync();  // Q's tensor-memory stores
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(k_full0);
+            st ^= kKOdd;
+          }
+          if (s == 0 && t > 0) {
+#pragma unroll 1
+            for (int x = st & (kFine << kVShift) ? 0 : 1; x < 2; ++x) {
+              wait_v();
+              if (ok) put_v(x == 0);
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(v_full0);
+              st ^= kVOdd;
+            }
+          }
         }
         if (t < total) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) vd[x] = rank ? kd[x][1] : kd[x][0];
           vs = ks;
+          st = (st & ~(7 << kVShift)) | (st & 7) << kVShift;
           if (ok) load_others();
         }
       }
@@ -721,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (left <= 0 && t == 0) enter();
         wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
         const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
-        if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
+        wait_k();
         if (left <= 0) enter();
         if (ok) {
           const uint8_t* row = p.kv + (int64_t)max(code, 0) * kRowBytes + 16 * l8;
@@ -735,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(k_full0);
-        ++kc;
+        st ^= kKOdd;
         --left;
       };
 #pragma unroll 1
@@ -837,14 +881,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         const uint32_t at = base + SM_K + 8 * kBlk + sw128_off(32 * w + (lane >> 3), lane & 7);
         const uint32_t valid = raw_valid[w] >> (lane >> 3);
 #pragma unroll 1
-        for (int s = 0; s == 0 || (s == 1 && two); ++s) {
+        for (int s = two ? 0 : 1; s < 2; ++s) {
           if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
           // (Q passes through the K buffer's other blocks only)
           if (ok) {
 #pragma unroll 2
             for (int x = 0; x < 8; ++x) {  // four rows on: half a swizzle atom, chunks flip bit 2
               uint4 d = lds16(raw + 4 * 656 * x);
-              if (s > 0 || !((valid >> (4 * x)) & 1)) d = make_uint4(0, 0, 0, 0);
+              if (s == 0 || !((valid >> (4 * x)) & 1)) d = make_uint4(0, 0, 0, 0);
               sts16((at + 512 * x) ^ (64 * (x & 1)), d);
             }
           }
@@ -877,64 +921,74 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       const uint64_t dq = sw128_desc(base + SM_Q, 16, 1024), dk = sw128_desc(base + SM_K, 16, 1024);
       const uint64_t dp = sw128_desc(base + SM_P, 16, 1024), dv = sw128_desc(base + SM_V, kVBlk, 1024);
       int kc = 0, gq = 0;
-      int qseg = 0, qleft = 0, passes = 1;  // segment of the next QK
-      auto qk = [&]() {
-#pragma unroll 1
-        for (int s = 0; s < passes || s == 0; ++s) {
-          wait(mb_k_full, kc & 1);
-          if (!ok) return;
-          if (qleft == 0) {  // its first tile is stored, so its descriptor is visible
-            qleft = uniform(segs[qseg % kSegs].n);
-            passes = uniform(segs[qseg % kSegs].flags) & kTwo ? 2 : 1;
-            ++qseg;
-          }
-          if (s == 0 && gq > 0) {  // the softmax has read S(gq - 1)
-            wait(mb_s_free, (gq - 1) & 1);
-            if (!ok) return;
-          }
-          fence_after_sync();
-          uint64_t a = dq, b = dk;
-#pragma unroll 1
-          for (int kb = 0; kb < kQtBlks; ++kb, b += kBlk >> 4)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_f16_ts_pair(tm + S_COL, tm + Q_COL + 32 * kb + 8 * k, b + 2 * k, IDESC_QK, (kb | k) != 0 || s > 0, leader);
-#pragma unroll 1
-          for (int kb = kQtBlks; kb < 9; ++kb, a += kBlk >> 4, b += kBlk >> 4)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f16_ss_pair(tm + S_COL, a + 2 * k, b + 2 * k, IDESC_QK, 1, leader);
-          mma_commit_pair(mb_k_free, leader);
-          ++kc;
-        }
-        mma_commit_pair(mb_s_full, leader);
-        --qleft;
-        ++gq;
-      };
-      int pseg = 0, pleft = 0;
+      int qseg = 0, qleft = 0;  // segment of the next QK
+      bool two = false;
+      int pseg = 0, pleft = 0, vc = 0;  // of the next PV
+      bool fine = false;
 #pragma unroll 1
       for (int g = -1; g < total && ok; ++g) {
-        if (g + 1 < total) qk();
-        if (g < 0) continue;
-        const bool first = pleft == 0;
-        wait(mb_v_full, g & 1);
-        wait(mb_p_full, g & 1);
-        if (first) {
-          // the accumulator of the segment before has been read
-          if (pseg > 0) wait(mb_o_free, (pseg - 1) & 1);
-          if (ok) pleft = uniform(segs[pseg % kSegs].n);
-          ++pseg;
-        }
-        if (ok) {
-          fence_after_sync();
+        // QK of tile g + 1, or of two passes the first; PV of tile g; then the second
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h)
+        for (int s = 0; s < 2; ++s) {
+          if (g + 1 < total && (s == 0 || two)) {
+            wait(mb_k_full, kc & 1);
+            if (!ok) break;
+            if (s == 0) {
+              if (qleft == 0) {  // its first tile is stored, so its descriptor is visible
+                qleft = uniform(segs[qseg % kSegs].n);
+                two = (uniform(segs[qseg % kSegs].flags) & kTwo) != 0;
+                ++qseg;
+              }
+              --qleft;
+              if (gq > 0) wait(mb_s_free, (gq - 1) & 1);  // the softmax has read S(gq - 1)
+              if (!ok) break;
+              ++gq;
+            }
+            fence_after_sync();
+            uint64_t a = dq, b = dk;
+#pragma unroll 1
+            for (int kb = 0; kb < kQtBlks; ++kb, b += kBlk >> 4)
 #pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
-              mma_f16_ss_pair(tm + 128 * h, dp + (((s >> 2) * kBlk + 32 * (s & 3)) >> 4),
-                              dv + h * (2 * kVBlk >> 4) + (2048 * s >> 4), IDESC_PV, !first || s > 0, leader);
-          mma_commit_pair(mb_v_free, leader);
+              for (int k = 0; k < 4; ++k)
+                mma_f16_ts_pair(tm + S_COL, tm + Q_COL + 32 * kb + 8 * k, b + 2 * k, IDESC_QK, (kb | k) != 0 || s > 0,
+                                leader);
+#pragma unroll 1
+            for (int kb = kQtBlks; kb < 9; ++kb, a += kBlk >> 4, b += kBlk >> 4)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_f16_ss_pair(tm + S_COL, a + 2 * k, b + 2 * k, IDESC_QK, 1, leader);
+            mma_commit_pair(mb_k_free, leader);
+            ++kc;
+            if (s > 0 || !two) mma_commit_pair(mb_s_full, leader);
+          }
+          if (s == 0 && g >= 0) {
+            const bool first = pleft == 0;
+            wait(mb_p_full, g & 1);
+            if (first) {
+              // the accumulator of the segment before has been read
+              if (pseg > 0) wait(mb_o_free, (pseg - 1) & 1);
+              if (ok) pleft = uniform(segs[pseg % kSegs].n);
+              if (ok) fine = (uniform(segs[pseg % kSegs].flags) & kFine) != 0;
+              ++pseg;
+            }
+#pragma unroll 1
+            for (int y = fine ? 0 : 1; y < 2; ++y) {
+              wait(mb_v_full, vc & 1);
+              if (!ok) break;
+              fence_after_sync();
+              const uint32_t keep = !first || (fine && y > 0);
+#pragma unroll 1
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int x = 0; x < kKeys / 16; ++x)
+                  mma_f16_ss_pair(tm + 128 * h, dp + (((x >> 2) * kBlk + 32 * (x & 3)) >> 4),
+                                  dv + h * (2 * kVBlk >> 4) + (2048 * x >> 4), IDESC_PV, x > 0 ? 1 : keep, leader);
+              mma_commit_pair(mb_v_free, leader);
+              ++vc;
+            }
+            mma_commit_pair(mb_pv, leader);
+            --pleft;
+          }
         }
-        --pleft;
       }
       mma_commit_pair(mb_done, leader);  // every MMA of this thread
     }
@@ -1051,7 +1105,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           L += a + b;
         }
         // P's buffer and O are free once PV(t-1) has completed (the epilogue waited for a segment's last)
-        if (!first) wait(mb_v_free, (g - 1) & 1);
+        if (!first) wait(mb_pv, (g - 1) & 1);
         if (ok) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -1083,7 +1137,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       named_bar(1, kSoftmaxWarps * 32);
       L = (rowx[row] + rowx[64 + row]) + (rowx[128 + row] + rowx[192 + row]);
       named_bar(1, kSoftmaxWarps * 32);
-      wait(mb_v_free, (g - 1) & 1);
+      wait(mb_pv, (g - 1) & 1);
       if (ok) {
         fence_after_sync();
         const bool mine = sg.rt * kPairRows + kRows * rank + row < p.T * p.H;
