@@ -411,7 +411,8 @@ int dsa_shard_exchange_merge(int32_t* out, int64_t out_stride,
  * never read. A position that is seen resolves as in dsa_sparse_mla_decode; a
  * cache row outside [0, n_kv_rows), or past the block table, reads as zeros.
  * A position that some rows see must hold finite values: its NaN or infinity
- * reaches the other rows of the request too.
+ * reaches the other rows of the request too. Values of an fp8 cache enter the
+ * products as f16, so one beyond 65504 counts as infinite.
  *
  * q      [B, T, n_head, 576] f16 or bf16, contiguous (bf16 with a bf16 cache)
  * kv     f16/bf16 [.., page, 576] or u8 [.., page, 656] (DSA_FP8_DS_MLA)

@@ -683,3 +683,51 @@ def test_verify_a_tree_end_to_end(dsa):
     dsa.rotary_embedding(ctx, both, torch.arange(L + 3, device=DEV), table)
     # the writer rounds the rotated key to fp16, the operator to bf16
     assert bool(((back[:, 512:].double() - ctx[:, 0].double()).abs() <= 2.0 ** -7 * ctx[:, 0].double().abs() + 2.0 ** -20).all())
+
+
+def test_tree_lengths_of_every_kind_in_one_batch(dsa, oracle):
+    """Requests whose scores take one, two or two finer products follow one
+    another in a pair's run, with rows of empty requests between them."""
+    lens = [1000, 20000, 40000, 3, 1024, 1025, 0, 32768, 32769, 1, 700]
+    run_tree(dsa, oracle, "fp8", BF, BF, 2, 8, lens, None, seed=21)
+    run_tree(dsa, oracle, "fp8", HF, HF, 3, 64, lens[::-1], [3, 1, 2, 3, 0, 3, 3, 3, 2, 3, 3], seed=22)
+
+
+@pytest.mark.parametrize("lens", [[1, 2, 5, 40], [130, 600, 1024], [1025, 1500, 3001], [9000, 17001]])
+def test_tree_scores_keep_the_scale(dsa, oracle, lens):
+    """Up to 32768 positions an fp8 key enters the scores with 2^-16 of its value:
+    the scale's second part has 2^-6 of it and is rounded to f16, as its product
+    with the code is (2^-17 each). The errors are independent, so lse's, which
+    averages scores', has no larger deviation than 2^-16 / sqrt 3 of the score's
+    terms in the 2-norm; an f32 sum of the 2 * 576 terms adds sqrt(1152) 2^-24 of
+    partial sums that are at most about twice that norm."""
+    q, cache, bt, ln, mask, dl, o, lse = run_tree(dsa, oracle, "fp8", BF, BF, 3, 16, lens, None, seed=23)
+    ref = tree64(q, cache, bt, lens, mask, None, SCALE)[1]
+    fin = torch.isfinite(ref)
+    k2 = values64(cache).square().mean(0)
+    norm = (q.double().square() @ k2).sqrt()[fin].max() * SCALE
+    rms = (lse.double() - ref)[fin].square().mean().sqrt()
+    tol = (2.0 ** -16 / 3 ** 0.5 + 2 * 1152 ** 0.5 * 2.0 ** -24) * norm
+    assert float(rms) <= float(tol), (float(rms), float(tol))
+
+
+@pytest.mark.parametrize("lens", [[700, 3], [1500, 2100], [33000]])
+def test_tree_scales_of_every_size(dsa, oracle, lens):
+    """Groups' scales from 2^-24 to 2^2 side by side, and groups of scale zero; each
+    element of a key is off by at most half an f16 step of itself or 2^-25."""
+    bt, pages = tables(lens, 64, 31)
+    cache = make_cache("fp8", pages, 64, 32, oracle)
+    rows = cache.view(-1, 656)
+    scale = rows[:, 512:528].contiguous().view(F32)
+    power = torch.randint(-17, 2, scale.shape, generator=gen(33), device=DEV)
+    power[::5] = torch.randint(-17, 10, power[::5].shape, generator=gen(34), device=DEV)
+    scale = torch.ldexp(scale, power)
+    scale[7::11, 1] = 0.0
+    rows[:, 512:528] = scale.contiguous().view(torch.uint8)
+    B, T, H = len(lens), 2, 5
+    q = (torch.randn(B, T, H, 576, generator=gen(35), device=DEV) * 2.0 ** -8).to(BF)
+    mask = random_masks(dsa, B, T, 36)
+    ln = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o, lse = torch.empty(B, T, H, 512, dtype=BF, device=DEV), torch.empty(B, T, H, device=DEV)
+    dsa.tree_mla_decode(o, lse, q, cache, bt, ln, mask, SCALE)
+    check_tree(o, lse, tree64(q, cache, bt, lens, mask, None, SCALE), "fp8")
