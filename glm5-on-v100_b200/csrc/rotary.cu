@@ -18,6 +18,7 @@
 // strides, offset or widths are not multiples of 16 bytes take units of one pair
 // (or one copied element) instead.
 #include <algorithm>
+#include <cstdint>
 
 #include "common.cuh"
 
@@ -186,6 +187,13 @@ extern "C" int dsa_rotary_embedding(void* out, int64_t out_tok_stride, int64_t o
   DSA_REQUIRE(n_tok <= (1 << 28) && n_head <= 65535, DSA_ERR_UNSUPPORTED, "rotary_embedding: too many tokens or heads");
   if (n_tok == 0 || n_head == 0) return DSA_OK;
   DSA_REQUIRE(out && x && positions && cos_sin && max_pos > 0, DSA_ERR_INVALID, "rotary_embedding: null pointer");
+  // no two of out's heads share an element: the nearer of its strides spans a head,
+  // the other all the heads at the nearer one
+  const int64_t st = n_tok > 1 ? out_tok_stride : INT64_MAX, sh = n_head > 1 ? out_head_stride : INT64_MAX;
+  const int64_t near = std::min(st, sh), far = std::max(st, sh), n_near = st <= sh ? n_tok : n_head;
+  DSA_REQUIRE(near >= width && (far == INT64_MAX || (far - width) / (n_near - 1) >= near),
+              DSA_ERR_INVALID, "rotary_embedding: heads of out overlap (strides %lld, %lld)", (long long)out_tok_stride,
+              (long long)out_head_stride);
   const int item = dtype == DSA_F32 ? 4 : 2;
   const int e = 16 / item;
   auto is16 = [&](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };

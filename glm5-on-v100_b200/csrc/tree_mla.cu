@@ -1248,7 +1248,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) tree_merge_kernel(const Tree
   const int row = 32 * (item % (kPairRows / 32)) + lane;  // of the row tile
   const int col = kMergeCols * (item / (kPairRows / 32));
   if (cut.rt * kPairRows + row >= rows) return;
-  const int n = 1 + (cut.nt - cut.tile + cut.chunk - 1) / cut.chunk;  // segments
+  const int n = 1 + (int)(((long long)cut.nt - cut.tile + cut.chunk - 1) / cut.chunk);  // segments
   // the first one is slot 0 if the tile starts where its pair's run does, else slot 1
   auto slot = [&](int i) { return 2 * (pair - 1 + i) + (i == 0 && cut.tile < cut.chunk ? 1 : 0); };
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row;

@@ -507,6 +507,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _fits(*sizes):
+    """Sizes that the entry points take as 32-bit integers."""
+    if max(sizes) >= 1 << 31:
+        raise RuntimeError(f"sizes must be below 2^31 (got {max(sizes)})")
+
+
 def _vector(t, n, name, shape="[B]"):
     """An int32 vector of at least n elements, contiguous."""
     if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < n:
@@ -521,6 +527,7 @@ def _pages(block_table, B):
     n, width = block_table.shape
     if n < B:
         raise RuntimeError(f"block_table has fewer than {B} rows")
+    _fits(B, width)
     return block_table.data_ptr(), max(block_table.stride(0), width), width
 
 
@@ -558,6 +565,7 @@ def _tree_mla_decode_impl(o, lse, q, kv_cache, block_table, seq_lens, tree_mask,
         draft_lens = _vector(draft_lens, B, "draft_lens")
     page = kv_cache.size(-2)
     _check(page > 0, "kv_cache has no rows in a page")
+    _fits(T, H, page)
     if torch.cuda.current_device() == index:
         ws_bytes = int(L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H))
     else:
@@ -581,7 +589,9 @@ def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens)
         if c.shape != shape or c.dtype != dtype or c.get_device() != index or not c.is_contiguous():
             raise RuntimeError(f"cache {i} must be contiguous with the shape, dtype and device of the first")
     ptrs = [c.data_ptr() for c in caches]
-    _check(len(set(ptrs)) == len(ptrs), "the same cache twice in the list")
+    order, nbytes = sorted(ptrs), c0.numel() * c0.element_size()
+    _check(nbytes == 0 or all(b - a >= nbytes for a, b in zip(order, order[1:])),
+           "the same cache twice in the list, or caches that overlap")
     _check(accepted.dim() == 2, "accepted must be [B, n_accept]")
     _int32(accepted, "accepted")
     B, A = accepted.shape
@@ -592,6 +602,7 @@ def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens)
     width, n = shape[-1], c0.numel()
     if n == 0:
         return
+    _fits(shape[-2], width * c0.element_size(), A)
     _launch(index, "dsa_commit_draft_rows", (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), n // width, shape[-2],
             width * c0.element_size(), *pages, seq_lens.data_ptr(), draft_lens.data_ptr(), 64, accepted.data_ptr(),
             max(accepted.stride(0), A), A, B)
@@ -621,6 +632,7 @@ def _gather_cache_impl(out, cache, block_table, cu_seq_lens, seq_starts):
     n = out.size(0)
     if n == 0:
         return
+    _fits(n + 64, cache.size(-2), width)
     _launch(index, "dsa_gather_cache", out.data_ptr(), _DTYPE[out.dtype],
             max(out.stride(0), width) if n == 1 else out.stride(0), n, cache.data_ptr(), fmt, cache.numel() // elems,
             cache.size(-2), width, *pages, cu_seq_lens.data_ptr(), _ptr(seq_starts), B)
@@ -642,6 +654,7 @@ def _rotary_embedding_impl(out, x, positions, cos_sin_cache, is_neox, rope_offse
     if T * H * W == 0:
         return
     max_pos, rot = cos_sin_cache.shape
+    _fits(T, H, W, rot, rope_offset)
     _launch(index, "dsa_rotary_embedding", out.data_ptr(), ys[0], ys[1], x.data_ptr(), xs[0], xs[1], _DTYPE[x.dtype],
             positions.data_ptr(), cos_sin_cache.data_ptr(), max_pos, rot, int(rope_offset), int(bool(is_neox)), T, H, W)
 
@@ -822,6 +835,7 @@ def gather_cache(out, cache, block_table, cu_seq_lens, seq_starts=None) -> None:
 def rotary_embedding(out, x, positions, cos_sin_cache, is_neox: bool = False, rope_offset: int = 0) -> None:
     """out = x [T, n_head, width] with elements [rope_offset, rope_offset +
     cos_sin_cache.size(1)) of every head rotated; the rest is copied. out may
-    be x (in place) or a slice of another tensor, such as the rotary columns
-    of the attention's query rows. The table: rope.rope_cos_sin_cache."""
+    be x (in place), or lie in another tensor or in other columns of x's, such
+    as the rotary columns of the attention's query rows; other overlaps of the
+    two are not allowed. The table: rope.rope_cos_sin_cache."""
     _op("rotary_embedding")(out, x, positions, cos_sin_cache, bool(is_neox), int(rope_offset))

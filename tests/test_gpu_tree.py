@@ -731,3 +731,28 @@ def test_tree_scales_of_every_size(dsa, oracle, lens):
     o, lse = torch.empty(B, T, H, 512, dtype=BF, device=DEV), torch.empty(B, T, H, device=DEV)
     dsa.tree_mla_decode(o, lse, q, cache, bt, ln, mask, SCALE)
     check_tree(o, lse, tree64(q, cache, bt, lens, mask, None, SCALE), "fp8")
+
+
+def test_commit_refuses_caches_that_overlap(dsa):
+    pool = torch.zeros(5, 16, 132, dtype=torch.uint8, device=DEV)
+    bt = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    one = torch.ones(1, dtype=torch.int32, device=DEV)
+    acc = torch.full((1, 1), -1, dtype=torch.int32, device=DEV)
+    dsa.commit_draft_rows([pool[3:5], pool[0:2]], bt, one, acc, one)
+    with pytest.raises(RuntimeError, match="overlap"):
+        dsa.commit_draft_rows([pool[0:3], pool[4:5].expand(3, 16, 132).contiguous(), pool[1:4]], bt, one, acc, one)
+
+
+def test_rotary_out_in_other_columns_of_x(dsa):
+    """x and out interleaved in one buffer; in place with heads farther apart than tokens."""
+    table = dsa.rope.rope_cos_sin_cache(64, 100, device=DEV)
+    pos = torch.arange(7, device=DEV)
+    buf = torch.randn(7, 5, 192, generator=gen(2), device=DEV).to(BF)
+    want = buf.clone()
+    want[..., 128:] = rope_f32(buf[..., :64].contiguous(), table, pos, 0, False)
+    dsa.rotary_embedding(buf[..., 128:], buf[..., :64], pos, table)
+    assert torch.equal(buf, want)
+    x = torch.randn(5, 7, 64, generator=gen(3), device=DEV).to(BF)
+    want = rope_f32(x.transpose(0, 1).contiguous(), table, pos, 0, True)
+    dsa.rotary_embedding(x.transpose(0, 1), x.transpose(0, 1), pos, table, True)
+    assert torch.equal(x.transpose(0, 1), want)

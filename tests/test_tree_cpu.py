@@ -136,6 +136,25 @@ def test_rotary_entry_refuses_bad_arguments(dsa):
     assert call(n=0) == L.DSA_OK and call(h=0) == L.DSA_OK
 
 
+def test_rotary_entry_refuses_heads_that_overlap(dsa):
+    """Strides of out that give two heads the same element; x may repeat its heads."""
+    L, lib = dsa._lib, dsa._lib.lib()
+    P = ctypes.c_void_p
+
+    def call(n, h, ot, oh):
+        return lib.dsa_rotary_embedding(P(1024), ot, oh, P(1024), 0, 0, 1, P(1024), P(1024), 10, 64, 0, 0, n, h, 64, None)
+
+    for n, h, ot, oh in [(4, 1, 0, 64), (4, 1, 63, 0), (1, 3, 0, 0), (1, 3, 999, 56), (4, 3, 64, 64), (4, 3, 128, 64),
+                         (4, 3, 64, 192), (4, 3, 191, 64), (4, 3, -192, 64), (2, 2, 1 << 62, 1 << 62)]:
+        assert call(n, h, ot, oh) == L.DSA_ERR_INVALID, (n, h, ot, oh)
+
+
+def test_sizes_beyond_32_bits_are_refused(dsa):
+    dsa.ops._fits(1, (1 << 31) - 1)
+    with pytest.raises(RuntimeError, match="2.31"):
+        dsa.ops._fits(3, 1 << 31)
+
+
 def test_gather_and_commit_entries_refuse_bad_arguments(dsa):
     L, lib = dsa._lib, dsa._lib.lib()
     P = ctypes.c_void_p
