@@ -71,7 +71,6 @@
 #include <cfloat>
 #include <cmath>
 #include <mutex>
-#include <type_traits>
 
 #include "sparse_mla.cuh"
 #include "tc_common.cuh"

@@ -756,3 +756,53 @@ def test_rotary_out_in_other_columns_of_x(dsa):
     want = rope_f32(x.transpose(0, 1).contiguous(), table, pos, 0, True)
     dsa.rotary_embedding(x.transpose(0, 1), x.transpose(0, 1), pos, table, True)
     assert torch.equal(x.transpose(0, 1), want)
+
+
+def test_commit_gather_and_rotary_in_a_graph(dsa):
+    """Captured once, replayed with other lengths, paths, positions and contents."""
+    B, T, page = 3, 6, 16
+    cache = torch.zeros(40, page, 576, dtype=HF, device=DEV)
+    bt = torch.randperm(36, generator=gen(1), device=DEV).view(B, 12).int()
+    lens, drafts, cu = (torch.zeros(n, dtype=torch.int32, device=DEV) for n in (B, B, B + 1))
+    acc = torch.full((B, T), -1, dtype=torch.int32, device=DEV)
+    pos = torch.zeros(9, dtype=torch.int64, device=DEV)
+    table = dsa.rope.rope_cos_sin_cache(64, 50, device=DEV)
+    x = torch.zeros(9, 3, 64, dtype=BF, device=DEV)
+    out, turned = torch.zeros(200, 576, dtype=BF, device=DEV), torch.zeros_like(x)
+
+    def step():
+        dsa.commit_draft_rows([cache], bt, lens, acc, drafts)
+        dsa.gather_cache(out, cache, bt, cu)
+        dsa.rotary_embedding(turned, x, pos, table)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed, (n, d) in enumerate([([30, 6, 61], [6, 3, 1]), ([0, 64, 17], [2, 6, 6]), ([1, 1, 190], [1, 0, 6])]):
+        cache.copy_(torch.randn(cache.shape, generator=gen(seed), device=DEV))
+        x.copy_(torch.randn(x.shape, generator=gen(seed + 9), device=DEV))
+        pos.copy_(torch.randint(0, 50, pos.shape, generator=gen(seed), device=DEV))
+        lens.copy_(torch.tensor(n))
+        drafts.copy_(torch.tensor(d))
+        cu.copy_(torch.tensor([0, *np.cumsum(np.minimum(n, 66)).tolist()]))
+        acc.fill_(-1)
+        want = cache.clone().view(-1, 576)
+        row = lambda b, p: int(bt[b, p // page]) * page + p % page
+        for b in range(B):
+            path = [k for k in range(1, d[b], 2)]
+            acc[b, :len(path)] = torch.tensor(path, dtype=torch.int32)
+            old = want.clone()
+            for k, a in enumerate(path):
+                if n[b] - d[b] >= 0:
+                    want[row(b, n[b] - d[b] + k)] = old[row(b, n[b] - d[b] + a)]
+        out.fill_(3.0)
+        graph.replay()
+        assert torch.equal(cache.view(-1, 576), want)
+        rows = [row(b, p) for b in range(B) for p in range(min(n[b], 66))]
+        assert torch.equal(out[:len(rows)], want[rows].to(BF)) and bool((out[len(rows):] == 3.0).all())
+        assert torch.equal(turned, rope_f32(x, table, pos, 0, False))
