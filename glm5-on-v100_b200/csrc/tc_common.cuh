@@ -340,25 +340,23 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mbar) {
 }
 // Bounded wait in few instructions, for loops whose code has to fit the
 // instruction cache: one try and up to `more` others, each suspended for at most
-// about 2 us. False when they ran out; the caller records it.
-__device__ __forceinline__ bool mbar_wait_tries(uint32_t mbar, uint32_t parity, uint32_t more) {
-  uint32_t ok;
+// about 2 us. Sets `more` to 0 when they ran out; the caller records it.
+__device__ __forceinline__ void mbar_wait_sticky(uint32_t mbar, uint32_t parity, uint32_t& more) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       ".reg .u32 n;\n\t"
-      "mov.u32 n, %4;\n"
+      "mov.u32 n, %0;\n"
       "WAIT_%=:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "@p bra DONE_%=;\n\t"
       "setp.ne.u32 q, n, 0;\n\t"
       "sub.u32 n, n, 1;\n\t"
-      "@q bra WAIT_%=;\n"
-      "DONE_%=:\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(mbar), "r"(parity), "r"(2000u), "r"(more)
+      "@q bra WAIT_%=;\n\t"
+      "mov.u32 %0, 0;\n"
+      "DONE_%=:\n\t}"
+      : "+r"(more)
+      : "r"(mbar), "r"(parity), "r"(2000u)
       : "memory");
-  return ok != 0;
 }
 // Named barrier that also ORs a predicate over its threads.
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool pred) {

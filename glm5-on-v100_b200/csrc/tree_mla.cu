@@ -566,6 +566,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     __syncwarp();
     tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
   } else if (warp == kRowWarp) {
+    for (int i = lane; i < kRing * kKeys; i += 32) ring[i] = -1;
+    for (int i = lane; i < kSegs * (int)(sizeof(Segment) / 4); i += 32) reinterpret_cast<int*>(segs)[i] = 0;
+    __syncwarp();
     c = find_run(p, pair, lane);
     if (lane == 0) {
       *run_tiles = c.left;
@@ -580,17 +583,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
   const uint32_t tmem = *tmem_slot;
   const int total = uniform(*run_tiles);
 
-  uint32_t ok = 1;
-  // By a whole warp: `ok` stays uniform. The compiler is not to know that it is 0 after
-  // a wait that ran out: it would write the rest of the loop a second time for that.
-  auto wait = [&](uint32_t mbar, uint32_t parity) {
-    const bool got = __all_sync(0xffffffffu, mbar_wait_tries(mbar, parity, ok << 20));
-    if (!got && ok && lane == 0) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
-    ok = got ? ok : 0;
-    asm volatile("" : "+r"(ok));
+  // After a wait that ran out, `more` is 0: its thread's later waits return after one
+  // try, and it goes on through its role's barriers and arrivals with whatever is
+  // there. That is safe: rows in the ring and segment descriptors are valid from
+  // the start, and what a segment's loops go by is read only while no thread of the
+  // role has failed. The MMA and row warps stop instead (`ok`, uniform).
+  uint32_t more = 1u << 20;
+  auto wait = [&](uint32_t mbar, uint32_t parity) { mbar_wait_sticky(mbar, parity, more); };
+  auto wait_ok = [&](uint32_t mbar, uint32_t parity) {
+    mbar_wait_sticky(mbar, parity, more);
+    return __all_sync(0xffffffffu, more != 0);
   };
-  // After a wait that ran out (`ok` false) every thread of its warp still
-  // executes its role's barriers and arrivals, and later waits return at once.
   if (warp < kProducers) {
     // ------------------------------------------------------------- producers
     // K(t+1) is stored under PV(t-1), V(t) under QK(t+1); with two passes the first
@@ -608,13 +611,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     // the next segment's Q, through the K buffer
     auto enter = [&]() {
       const Segment& sg = segs[seg % kSegs];  // visible: the wait for this tile's rows
-      const bool live = !named_bar_or(2, kProducers * 32, !ok);  // all take the same number of barriers
+      const bool live = !named_bar_or(2, kProducers * 32, more == 0);  // all take the same number of barriers
       left = live ? uniform(sg.n) : 1 << 30;
       st = (st & ~(kTwo | kFine | kFull)) | (live ? uniform(sg.flags) : 0);
       if (live)
         load_q<FMT>(p, base, tmem, qe + 64 * (seg % kQeSegs), sg.b, sg.rt * kPairRows + kRows * rank, w, lane);
-      ok = live ? ok : 0;
-      asm volatile("" : "+r"(ok));
+      more = live ? more : 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(mb_q_full + 8 * (seg % kQeSegs));
       ++seg;
@@ -676,22 +678,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       };
       auto take = [&](int t) {
         wait(mb_raw_full, t & 1);
-        if (ok) {
-          const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
-          const uint32_t raw = base + SM_RAW + 4 * w * 656;
+        const uint32_t valid = raw_valid[w >> 3] >> (4 * w & 31);
+        const uint32_t raw = base + SM_RAW + 4 * w * 656;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) kd[x][h] = lds8(raw + 656 * x + 256 * h + 8 * lane);
+        ks = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
+        oc = *reinterpret_cast<const int4*>(ring + 4 * w);
+        os = ring[4 * w + ((lane >> 1) & 3)];
+        if ((valid & 15u) != 15u) {  // the others read as zeros
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) kd[x][h] = lds8(raw + 656 * x + 256 * h + 8 * lane);
-          ks = lds4(raw + 656 * ((lane >> 2) & 3) + 512 + 4 * (lane & 3));
-          oc = *reinterpret_cast<const int4*>(ring + 4 * w);
-          os = ring[4 * w + ((lane >> 1) & 3)];
-          if ((valid & 15u) != 15u) {  // the others read as zeros
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (!((valid >> x) & 1)) kd[x][0] = kd[x][1] = make_uint2(0, 0);
-            if (!((valid >> ((lane >> 2) & 3)) & 1)) ks = 1.f;
-          }
+            if (!((valid >> x) & 1)) kd[x][0] = kd[x][1] = make_uint2(0, 0);
+          if (!((valid >> ((lane >> 2) & 3)) & 1)) ks = 1.f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(mb_raw_free);
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         for (int s = 0; s < 2; ++s) {
           if (t < total && (s == 0 || (st & kTwo))) {
             wait_k();
-            if (ok) put_k(s == 0 && (st & kTwo));
+            put_k(s == 0 && (st & kTwo));
             fence_proxy_async();
             fence_before_sync();  // Q's tensor-memory stores
             __syncwarp();
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll 1
             for (int x = st & (kFine << kVShift) ? 0 : 1; x < 2; ++x) {
               wait_v();
-              if (ok) put_v(x == 0);
+              put_v(x == 0);
               fence_proxy_async();
               __syncwarp();
               if (lane == 0) mbar_arrive_cluster(v_full0);
@@ -774,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           for (int x = 0; x < 4; ++x) vd[x] = rank ? kd[x][1] : kd[x][0];
           vs = ks;
           st = (st & ~(7 << kVShift)) | (st & 7) << kVShift;
-          if (ok) load_others();
+          load_others();
         }
       }
     } else {
@@ -787,10 +787,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       auto store_k = [&](int t) {
         if (left <= 0 && t == 0) enter();
         wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
-        const int code = ok ? rows_of(t)[64 * rank + 4 * w + r4] : -1;
+        const int code = rows_of(t)[64 * rank + 4 * w + r4];
         wait_k();
         if (left <= 0) enter();
-        if (ok) {
+        {
           const uint8_t* row = p.kv + (int64_t)max(code, 0) * kRowBytes + 16 * l8;
 #pragma unroll
           for (int x = 0; x < 9; ++x)
@@ -810,11 +810,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         if (t + 1 < total) store_k(t + 1);
         if (t < 0) continue;
         int code[2];
-        code[0] = ok ? rows_of(t)[8 * w + r4] : -1;
-        code[1] = ok ? rows_of(t)[8 * w + r4 + 4] : -1;
+        code[0] = rows_of(t)[8 * w + r4];
+        code[1] = rows_of(t)[8 * w + r4 + 4];
         free_rows(t);
         if (t > 0) wait(mb_v_free, (t - 1) & 1);
-        if (ok) {
+        {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint8_t* row = p.kv + (int64_t)max(code[i], 0) * kRowBytes + 512 * rank + 16 * l8;
@@ -837,15 +837,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     // read, with the rows of the other CTA's keys beside it.
     uint64_t seen = 0;
     int seg = 0, t = 0;
+    bool ok = true;
 #pragma unroll 1
     for (; t < total; ++t) {
       if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
       int code[4];
       row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
       if constexpr (kFp8) {
-        if (t > 0) wait(mb_raw_free, (t - 1) & 1);
+        if (t > 0) ok = wait_ok(mb_raw_free, (t - 1) & 1);
       } else {
-        if (t >= kRing) wait(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
+        if (t >= kRing) ok = wait_ok(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
       }
       if (!ok) break;
       if (c.first && t > 0 && lane == 0) segs[seg % kSegs] = segment_of<kFp8>(c);
@@ -893,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
         wait(mb_raw_full, t & 1);
-        if (left == 0 && ok) {
+        if (left == 0) {
           left = uniform(segs[seg % kSegs].n);
           two = (uniform(segs[seg % kSegs].flags) & kTwo) != 0;
           ++seg;
@@ -905,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         for (int s = two ? 0 : 1; s < 2; ++s) {
           if (kc > 0) wait(mb_k_free, (kc - 1) & 1);
           // (Q passes through the K buffer's other blocks only)
-          if (ok) {
+          {
 #pragma unroll 2
             for (int x = 0; x < 8; ++x) {  // four rows on: half a swizzle atom, chunks flip bit 2
               uint4 d = lds16(raw + 4 * 656 * x);
@@ -928,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll 1
       for (int t = 0; t < total; ++t) {
         wait(mb_r_full + 8 * (t % kRing), (t / kRing) & 1);
-        const int code = ok ? ring[(t % kRing) * kKeys + 64 * rank + 32 * w + lane] : -1;
+        const int code = ring[(t % kRing) * kKeys + 64 * rank + 32 * w + lane];
         __syncwarp();
         if (lane == 0) mbar_arrive(mb_r_free + 8 * (t % kRing));
         if (code >= 0) prefetch_l2(p.kv + (int64_t)code * kRowBytes, kRowBytes);
@@ -942,6 +943,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       const uint64_t dq = sw128_desc(base + SM_Q, 16, 1024), dk = sw128_desc(base + SM_K, 16, 1024);
       const uint64_t dp = sw128_desc(base + SM_P, 16, 1024), dv = sw128_desc(base + SM_V, kVBlk, 1024);
       int kc = 0, gq = 0;
+      bool ok = true;
       int qseg = 0, qleft = 0;  // segment of the next QK
       bool two = false;
       int pseg = 0, pleft = 0, vc = 0;  // of the next PV
@@ -952,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll 1
         for (int s = 0; s < 2; ++s) {
           if (g + 1 < total && (s == 0 || two)) {
-            wait(mb_k_full, kc & 1);
+            ok = wait_ok(mb_k_full, kc & 1);
             if (!ok) break;
             if (s == 0) {
               if (qleft == 0) {  // its first tile is stored, so its descriptor is visible
@@ -961,7 +963,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
                 ++qseg;
               }
               --qleft;
-              if (gq > 0) wait(mb_s_free, (gq - 1) & 1);  // the softmax has read S(gq - 1)
+              if (gq > 0) ok = wait_ok(mb_s_free, (gq - 1) & 1);  // the softmax has read S(gq - 1)
               if (!ok) break;
               ++gq;
             }
@@ -983,17 +985,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           }
           if (s == 0 && g >= 0) {
             const bool first = pleft == 0;
-            wait(mb_p_full, g & 1);
+            ok = wait_ok(mb_p_full, g & 1);
+            if (!ok) break;
             if (first) {
               // the accumulator of the segment before has been read
-              if (pseg > 0) wait(mb_o_free, (pseg - 1) & 1);
-              if (ok) pleft = uniform(segs[pseg % kSegs].n);
-              if (ok) fine = (uniform(segs[pseg % kSegs].flags) & kFine) != 0;
+              if (pseg > 0) ok = wait_ok(mb_o_free, (pseg - 1) & 1);
+              if (!ok) break;
+              pleft = uniform(segs[pseg % kSegs].n);
+              fine = (uniform(segs[pseg % kSegs].flags) & kFine) != 0;
               ++pseg;
             }
 #pragma unroll 1
             for (int y = fine ? 0 : 1; y < 2; ++y) {
-              wait(mb_v_full, vc & 1);
+              ok = wait_ok(mb_v_full, vc & 1);
               if (!ok) break;
               fence_after_sync();
               const uint32_t keep = !first || (fine && y > 0);
@@ -1027,11 +1031,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     uint8_t* prow = sm + SM_P + (sp >> 1) * kBlk;
     // 16 scores of this thread's row, hidden keys as -inf
     auto read_s = [&](int col, uint32_t allow, uint32_t (&s)[16]) {
-      if (!ok) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = 0u;
-        return;
-      }
       tmem_ld16(t_sp + S_COL + 32 * hh + col, s);
       tmem_wait_ld();
       if ((allow & 0xffffu) != 0xffffu) {
@@ -1043,13 +1042,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
 #pragma unroll 1
     for (int seg = 0; g < total; ++seg) {
       wait(mb_q_full + 8 * (seg % kQeSegs), (seg / kQeSegs) & 1);
-      ok = named_bar_or(1, kSoftmaxWarps * 32, !ok) ? 0 : 1;  // all take the same number of barriers
-      asm volatile("" : "+r"(ok));
+      const bool live = !named_bar_or(1, kSoftmaxWarps * 32, more == 0);  // all take the same number of barriers
+      more = live ? more : 0;
       const Segment& sg = segs[seg % kSegs];
-      const int end = ok ? g + uniform(sg.n) : total;
+      const int end = live ? g + uniform(sg.n) : total;
       // positions before the drafts, from this thread's first key of the tile on
       int d = -64;
-      if (ok && (sg.rt * kPairRows + kRows * rank + row) / p.H < sg.nd) d = max(sg.pre - kofs, -64);
+      if (live && (sg.rt * kPairRows + kRows * rank + row) / p.H < sg.nd) d = max(sg.pre - kofs, -64);
       // not 0, so that a hidden key's -inf stays one
       const float rs = fmaxf(p.scale_log2 * __int_as_float((127 + (int)qe[64 * (seg % kQeSegs) + row]) << 23), FLT_MIN);
       float m = kNoMax, L = 0.f;
@@ -1059,7 +1058,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         // keys this thread's row sees, one bit each
         uint32_t allow = d >= 32 ? 0xffffffffu : d > 0 ? (1u << d) - 1 : 0u;
         if (d < 32 && d > -64) {  // drafts among the keys
-          uint64_t bits = (uint64_t)p.mask[(int64_t)sg.b * p.mask_stride + (sg.rt * kPairRows + kRows * rank + row) / p.H];
+          const int draft = min((sg.rt * kPairRows + kRows * rank + row) / p.H, p.T - 1);
+          uint64_t bits = (uint64_t)p.mask[(int64_t)sg.b * p.mask_stride + draft];
           if (sg.nd < 64) bits &= (1ull << sg.nd) - 1;
           allow |= (uint32_t)(d >= 0 ? bits << d : bits >> -d);
         }
@@ -1127,7 +1127,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         }
         // P's buffer and O are free once PV(t-1) has completed (the epilogue waited for a segment's last)
         if (!first) wait(mb_pv, (g - 1) & 1);
-        if (ok) {
+        {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) = pk[k];
@@ -1157,9 +1157,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       rowx[64 * q4 + row] = L;
       named_bar(1, kSoftmaxWarps * 32);
       L = (rowx[row] + rowx[64 + row]) + (rowx[128 + row] + rowx[192 + row]);
-      named_bar(1, kSoftmaxWarps * 32);
       wait(mb_pv, (g - 1) & 1);
-      if (ok) {
+      const bool good = !named_bar_or(1, kSoftmaxWarps * 32, more == 0);
+      if (good) {
         fence_after_sync();
         const bool mine = sg.rt * kPairRows + kRows * rank + row < p.T * p.H;
         const bool full = (sg.flags & kFull) != 0;
@@ -1213,6 +1213,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (lane == 0) mbar_arrive_cluster(o_free0);
     }
   }
+  if (more == 0) atomicExch(err, (int32_t)DSA_ERR_TIMEOUT);
   // every MMA has completed before TMEM is released, and no CTA leaves while the
   // other may still read its shared memory or arrive on its barriers
   __syncthreads();
