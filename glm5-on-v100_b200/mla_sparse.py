@@ -103,9 +103,11 @@ def forward_mqa_tree(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch
         q = q.reshape(B, T, q.shape[-2], q.shape[-1])
     if q.dtype not in (torch.float16, torch.bfloat16):
         q = q.to(torch.float16)
-    q = q.contiguous()
-    o = q.new_empty((*q.shape[:3], kv_lora_rank))
-    lse = q.new_empty(q.shape[:3], dtype=torch.float32)
+    if not q.is_contiguous():
+        q = q.contiguous()
+    B, T, H, _ = q.shape
+    o = q.new_empty((B, T, H, kv_lora_rank))
+    lse = torch.empty((B, T, H), dtype=torch.float32, device=q.device)
     ops.tree_mla_decode(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, float(scale), draft_lens)
     return (o, lse) if len(lead) == 3 else (o.view(*lead, kv_lora_rank), lse.view(lead))
 

@@ -522,13 +522,16 @@ def _vector(t, n, name, shape="[B]"):
 
 def _pages(block_table, B):
     """(pointer, row stride, blocks a row) of a block table of at least B rows."""
-    _int32(block_table, "block_table")
-    _rowmajor(block_table, "block_table")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise RuntimeError("block_table must be 2-D int32")
     n, width = block_table.shape
+    stride, inner = block_table.stride()
+    if inner != 1:
+        raise RuntimeError("block_table must have unit inner stride")
     if n < B:
         raise RuntimeError(f"block_table has fewer than {B} rows")
     _fits(B, width)
-    return block_table.data_ptr(), max(block_table.stride(0), width), width
+    return block_table.data_ptr(), max(stride, width), width
 
 
 def _latent_format(kv_cache):
@@ -542,39 +545,47 @@ def _latent_format(kv_cache):
     return _DTYPE[kv_cache.dtype], 576
 
 
+_HALF = frozenset((torch.float16, torch.bfloat16))
+
+
 def _tree_mla_decode_impl(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, draft_lens, scale):
     _check(q.is_cuda, "q must be a CUDA tensor")
     index = q.get_device()
     _same_device(index, "o lse kv_cache block_table seq_lens tree_mask draft_lens", o, lse, kv_cache, block_table,
                  seq_lens, tree_mask, draft_lens)
-    _check(q.dtype in (torch.float16, torch.bfloat16), "q must be fp16 or bf16")
-    _check(o.dtype in (torch.float16, torch.bfloat16), "o must be fp16 or bf16")
-    _check(lse.dtype == torch.float32, "lse must be fp32")
+    q_dtype, o_dtype = q.dtype, o.dtype
+    if q_dtype not in _HALF or o_dtype not in _HALF or lse.dtype != torch.float32:
+        raise RuntimeError("q and o must be fp16 or bf16, lse fp32")
     fmt, row = _latent_format(kv_cache)
-    _check(q.dim() == 4 and q.size(3) == 576, "q must be [B, T, n_head, 576]")
+    if q.dim() != 4 or q.size(3) != 576:
+        raise RuntimeError("q must be [B, T, n_head, 576]")
     B, T, H, _ = q.shape
-    _check(o.shape == (B, T, H, 512) and lse.shape == (B, T, H), "o/lse shape mismatch with q")
-    _check(q.is_contiguous() and o.is_contiguous() and lse.is_contiguous() and kv_cache.is_contiguous(),
-           "q, o, lse and kv_cache must be contiguous")
+    if o.shape != (B, T, H, 512) or lse.shape != (B, T, H):
+        raise RuntimeError("o/lse shape mismatch with q")
+    if not (q.is_contiguous() and o.is_contiguous() and lse.is_contiguous() and kv_cache.is_contiguous()):
+        raise RuntimeError("q, o, lse and kv_cache must be contiguous")
     pages = _pages(block_table, B)
     seq_lens = _vector(seq_lens, B, "seq_lens")
-    _check(tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.size(0) >= B and
-           tree_mask.size(1) == T and (T <= 1 or tree_mask.stride(1) == 1),
-           "tree_mask must be int64 [B, T] with unit inner stride")
     if draft_lens is not None:
         draft_lens = _vector(draft_lens, B, "draft_lens")
+    mask = tree_mask.shape
+    if tree_mask.dtype != torch.int64 or len(mask) != 2 or mask[0] < B or mask[1] != T:
+        raise RuntimeError("tree_mask must be int64 [B, T]")
+    mask_stride, inner = tree_mask.stride()
+    if T > 1 and inner != 1:
+        raise RuntimeError("tree_mask must have unit inner stride")
     page = kv_cache.size(-2)
     _check(page > 0, "kv_cache has no rows in a page")
     _fits(T, H, page)
     if torch.cuda.current_device() == index:
-        ws_bytes = int(L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H))
+        ws_bytes = L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H)
     else:
         with torch.cuda.device(index):
-            ws_bytes = int(L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H))
+            ws_bytes = L.lib().dsa_tree_mla_decode_workspace_bytes(B, T, H)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    _launch(index, "dsa_tree_mla_decode", o.data_ptr(), _DTYPE[o.dtype], lse.data_ptr(), q.data_ptr(), _DTYPE[q.dtype],
+    _launch(index, "dsa_tree_mla_decode", o.data_ptr(), _DTYPE[o_dtype], lse.data_ptr(), q.data_ptr(), _DTYPE[q_dtype],
             kv_cache.data_ptr(), fmt, kv_cache.numel() // row, page, *pages, seq_lens.data_ptr(), _ptr(draft_lens),
-            tree_mask.data_ptr(), max(tree_mask.stride(0), T), B, T, H, float(scale), _ptr(ws), ws_bytes)
+            tree_mask.data_ptr(), max(mask_stride, T), B, T, H, scale, _ptr(ws), ws_bytes)
 
 
 def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens):
