@@ -596,10 +596,10 @@ def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens)
     index = c0.get_device()
     _same_device(index, "block_table seq_lens accepted draft_lens", block_table, seq_lens, accepted, draft_lens)
     shape, dtype = c0.shape, c0.dtype
-    for i, c in enumerate(caches):
-        if c.shape != shape or c.dtype != dtype or c.get_device() != index or not c.is_contiguous():
-            raise RuntimeError(f"cache {i} must be contiguous with the shape, dtype and device of the first")
-    ptrs = [c.data_ptr() for c in caches]
+    if not (all(map(torch.Tensor.is_contiguous, caches)) and set(map(torch.Tensor.get_device, caches)) == {index} and
+            set(map(torch.Tensor.size, caches)) == {shape} and {c.dtype for c in caches} == {dtype}):
+        raise RuntimeError("caches must be contiguous with the shape, dtype and device of the first")
+    ptrs = list(map(torch.Tensor.data_ptr, caches))
     order, nbytes = sorted(ptrs), c0.numel() * c0.element_size()
     _check(nbytes == 0 or all(b - a >= nbytes for a, b in zip(order, order[1:])),
            "the same cache twice in the list, or caches that overlap")
