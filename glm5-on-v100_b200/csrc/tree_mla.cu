@@ -52,21 +52,22 @@
 // them): lse is within 3e-7. Up to 1024 positions the second product is the
 // rounding's own remainder, and V's is multiplied too (fewer keys average less).
 // Both sides, 8 heads x 16 drafts, 8 requests of 13,824 to 24,576 positions:
-// one product 80 us and 1.1e-6, two 106 us and 1.5e-7; 64 heads x 8 drafts, 4 x
-// 24,576: 142 us and 9.5e-7, 213 us and 1.7e-7. bf16 q is shifted by a power of
+// one product 74 us and 1.1e-6, two 102 us and 1.5e-7; 64 heads x 8 drafts, 4 x
+// 24,576: 133 us and 9.5e-7, 201 us and 1.7e-7. bf16 q is shifted by a power of
 // two per row into f16's range, which the row's scale undoes exactly. The running
 // maximum moves only when a score exceeds it by 2^8, so P <= 256 and O is rarely
 // rescaled.
 //
 // Measured (times with the merge): 32 drafts x 64 heads over 131,072 positions, fp8
-// 620 us = 940 TFLOP/s, 58% of the dense peak of a plain matrix product, 16-bit
-// cache 577 us. A tile takes a CTA 5300 cycles, the tensor cores 2700 of them: the
+// 608 us = 960 TFLOP/s, 59% of the rate of a plain matrix product, 16-bit
+// cache 607 us. A tile takes a CTA 5200 cycles, the tensor cores 2700 of them: the
 // bound is the producers' chain, K and V of a tile after one another, each store
 // (8 x 8 codes a lane) 1300 cycles of issue and latency and 700 of waits and fences.
-// With two products K is stored twice, 8600 cycles. The code of the loops counts: an
+// With two products K is stored twice, 8300 cycles. The code of the loops counts: an
 // SM's instruction cache misses go to a cache that several share, and took 76% of its
-// rate before the loops were cut (51% now), so the usual path has no calls and the
-// rare ones (scales out of f16's range, remainders) are rolled.
+// rate before the loops were cut (32 to 51% now), so the usual path has no calls,
+// the rare ones (scales out of f16's range, remainders) are rolled, and a wait is
+// three instructions.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
