@@ -1030,15 +1030,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
     const uint32_t p_full0 = cluster_map(mb_p_full, 0), o_free0 = cluster_map(mb_o_free, 0),
                    s_free0 = cluster_map(mb_s_free, 0);
     uint8_t* prow = sm + SM_P + (sp >> 1) * kBlk;
-    // 16 scores of this thread's row, hidden keys as -inf
-    auto read_s = [&](int col, uint32_t allow, uint32_t (&s)[16]) {
-      tmem_ld16(t_sp + S_COL + 32 * hh + col, s);
-      tmem_wait_ld();
-      if ((allow & 0xffffu) != 0xffffu) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;
-      }
-    };
     int g = 0;
 #pragma unroll 1
     for (int seg = 0; g < total; ++seg) {
@@ -1067,17 +1058,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         d = max(d - kKeys, -64);
         wait(mb_s_full, g & 1);
         fence_after_sync();
-        // twice through S, 16 columns at a time: the maximum, then the probabilities
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-          uint32_t s[16];
-          read_s(16 * x, allow >> (16 * x), s);
-          float y = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+        // this thread's scores, in registers from here on: S is free for the next tile
+        uint32_t s[32];
+        tmem_ld32(t_sp + S_COL + 32 * hh, s);
+        tmem_wait_ld();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(s_free0);
+        if (allow != 0xffffffffu) {
 #pragma unroll
-          for (int j = 2; j < 16; j += 2) y = max3(y, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-          mx = fmaxf(mx, y);
+          for (int j = 0; j < 32; ++j) s[j] = (allow >> j) & 1 ? s[j] : 0xff800000u;
         }
+        float mx = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+#pragma unroll
+        for (int j = 2; j < 32; j += 2) mx = max3(mx, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
         mx *= rs;  // rs >= 0
         float alpha = 1.f;
         const bool any = named_bar_or(1, kSoftmaxWarps * 32, mx > m + kRescale);
@@ -1091,36 +1085,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
             L *= alpha;
           }
         }
-        uint4 pk[4];
         const uint64_t rs2 = pack64(rs, rs), nm2 = pack64(-m, -m);
         uint64_t sum2 = 0;
-#pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-          uint32_t s[16];
-          read_s(16 * x, allow >> (16 * x), s);
-          pk[0] = pk[2];
-          pk[1] = pk[3];
-          uint32_t v[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float a, b;
-            unpack64(fma2(pack64(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), rs2, nm2), a, b);
-            a = ex2(a);
-            b = ex2(b);
-            sum2 = add2(sum2, pack64(a, b));
-            if (kBf16) {
-              const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-              v[j] = *reinterpret_cast<const uint32_t*>(&t);
-            } else {
-              v[j] = pack_half2(a, b);
-            }
+        for (int j = 0; j < 16; ++j) {  // the probabilities' pairs take the scores' places
+          float a, b;
+          unpack64(fma2(pack64(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), rs2, nm2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          sum2 = add2(sum2, pack64(a, b));
+          if (kBf16) {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+            s[j] = *reinterpret_cast<const uint32_t*>(&t);
+          } else {
+            s[j] = pack_half2(a, b);
           }
-          pk[2] = make_uint4(v[0], v[1], v[2], v[3]);
-          pk[3] = make_uint4(v[4], v[5], v[6], v[7]);
         }
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(s_free0);
         {
           float a, b;
           unpack64(sum2, a, b);
@@ -1131,7 +1111,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
         {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) = pk[k];
+            *reinterpret_cast<uint4*>(prow + sw128_off(row, 4 * hh + k)) =
+                make_uint4(s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]);
           if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
             fence_after_sync();
 #pragma unroll 1
