@@ -29,13 +29,14 @@
 // Roles (28 warps, 72 registers, no spills): the row warp walks the run, turns
 // positions into cache rows, and has this CTA's 64 rows of an fp8 tile copied as
 // they lie into one raw buffer (bulk copies; loads would go through the 28 KB that
-// L1 has left). Warps 0-15, four keys each, take the codes into registers, expand
+// L1 has left), prefetched into L2 while the buffer is still in use (8 heads ragged 100
+// -> 96 us from memory; 1 - 2% slower where the cache lies in L2 already). Warps 0-15, four keys each, take the codes into registers, expand
 // them and store K (keys x 576, K-major) and V (this CTA's 256 columns, MN-major):
 // its own keys' from the same registers, the other CTA's by loads a tile ahead,
 // which hit L2 (passing them between the CTAs' shared memory took 6600 cycles a
 // tile). Two tail warps copy the rotary part. 16-bit rows go to K and V by
 // cp.async. Warps 16-23 are the softmax, a thread a row and 32 keys (rows are TMEM
-// lanes: no shuffles). One warp of CTA 0 issues the MMAs, in uniform control flow
+// lanes: no shuffles), read into registers once, so that S is free at once. One warp of CTA 0 issues the MMAs, in uniform control flow
 // with one elected lane (80-130 cycles each otherwise, 45-64 now). Q lies in
 // tensor memory but for three of its nine 64-column blocks. QK(t+1) is issued
 // before PV(t), so K(t+1) is stored under PV(t-1), V(t) under QK(t+1), and the
@@ -52,20 +53,21 @@
 // them): lse is within 3e-7. Up to 1024 positions the second product is the
 // rounding's own remainder, and V's is multiplied too (fewer keys average less).
 // Both sides, 8 heads x 16 drafts, 8 requests of 13,824 to 24,576 positions:
-// one product 74 us and 1.1e-6, two 102 us and 1.5e-7; 64 heads x 8 drafts, 4 x
-// 24,576: 133 us and 9.5e-7, 201 us and 1.7e-7. bf16 q is shifted by a power of
+// one product 74 us and 1.1e-6, two 100 us and 1.5e-7; 64 heads x 8 drafts, 4 x
+// 24,576: 133 us and 9.5e-7, 188 us and 1.7e-7. bf16 q is shifted by a power of
 // two per row into f16's range, which the row's scale undoes exactly. The running
 // maximum moves only when a score exceeds it by 2^8, so P <= 256 and O is rarely
 // rescaled.
 //
 // Measured (times with the merge): 32 drafts x 64 heads over 131,072 positions, fp8
-// 608 us = 960 TFLOP/s, 59% of the rate of a plain matrix product, 16-bit
-// cache 607 us. A tile takes a CTA 5200 cycles, the tensor cores 2700 of them: the
+// 572 - 586 us = 1.0 PFLOP/s, 62% of the rate of a plain matrix product (690 in a long
+// loop, whose clocks the power limit lowers), 16-bit cache 544 us. A tile takes a CTA
+// 5000 cycles, the tensor cores 2700 of them: the
 // bound is the producers' chain, K and V of a tile after one another, each store
 // (8 x 8 codes a lane) 1300 cycles of issue and latency and 700 of waits and fences.
-// With two products K is stored twice, 8300 cycles. The code of the loops counts: an
+// With two products K is stored twice, 7800 cycles. The code of the loops counts: an
 // SM's instruction cache misses go to a cache that several share, and took 76% of its
-// rate before the loops were cut (32 to 51% now), so the usual path has no calls,
+// rate before the loops were cut (23% now), so the usual path has no calls,
 // the rare ones (scales out of f16's range, remainders) are rolled, and a wait is
 // three instructions.
 #include <algorithm>
@@ -844,7 +846,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (c.first) seen = seen_columns(p, c.b, c.r.nd, lane);
       int code[4];
       row_codes(p, c.b, c.r, seen, c.tile * kKeys, lane, code);
+      int mine[2];
+      bool run[2];  // 32 neighbouring rows are one copy
+      uint32_t valid[2];
       if constexpr (kFp8) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          mine[k] = rank ? code[2 + k] : code[k];
+          valid[k] = __ballot_sync(0xffffffffu, mine[k] >= 0);
+          const int head = __shfl_sync(0xffffffffu, mine[k], 0);
+          run[k] = __all_sync(0xffffffffu, mine[k] >= 0 && mine[k] == head + lane);
+          // the raw buffer is still in use: into L2
+          if (run[k] ? lane == 0 : mine[k] >= 0)
+            prefetch_l2(p.kv + (int64_t)mine[k] * kRowBytes, (run[k] ? 32 : 1) * kRowBytes);
+        }
         if (t > 0) ok = wait_ok(mb_raw_free, (t - 1) & 1);
       } else {
         if (t >= kRing) ok = wait_ok(mb_r_free + 8 * (t % kRing), (t / kRing - 1) & 1);
@@ -852,28 +867,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
       if (!ok) break;
       if (c.first && t > 0 && lane == 0) segs[seg % kSegs] = segment_of<kFp8>(c);
       if constexpr (kFp8) {
-        int mine[2];
-        uint32_t bytes = 0;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          mine[k] = rank ? code[2 + k] : code[k];
-          const uint32_t valid = __ballot_sync(0xffffffffu, mine[k] >= 0);
-          bytes += __popc(valid) * kRowBytes;
           ring[32 * k + lane] = rank ? code[k] : code[2 + k];  // the other CTA's keys
-          if (lane == 0) raw_valid[k] = valid;
+          if (lane == 0) raw_valid[k] = valid[k];
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(mb_raw_full, bytes);
+        if (lane == 0) mbar_arrive_expect_tx(mb_raw_full, (__popc(valid[0]) + __popc(valid[1])) * kRowBytes);
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          // 32 neighbouring rows are one copy
-          const int head = __shfl_sync(0xffffffffu, mine[k], 0);
-          const bool run = __all_sync(0xffffffffu, mine[k] >= 0 && mine[k] == head + lane);
-          if (run ? lane == 0 : mine[k] >= 0)
+        for (int k = 0; k < 2; ++k)
+          if (run[k] ? lane == 0 : mine[k] >= 0)
             bulk_load(base + SM_RAW + (32 * k + lane) * kRowBytes, p.kv + (int64_t)mine[k] * kRowBytes,
-                      (run ? 32 : 1) * kRowBytes, mb_raw_full);
-        }
+                      (run[k] ? 32 : 1) * kRowBytes, mb_raw_full);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) ring[(t % kRing) * kKeys + 32 * k + lane] = code[k];
