@@ -26,50 +26,51 @@
 // kernel, which is told where the runs start (no counters, nothing to reset, the
 // same bits in every run).
 //
-// Roles (28 warps, 72 registers, no spills): the row warp walks the run, turns
-// positions into cache rows, and has this CTA's 64 rows of an fp8 tile copied as
-// they lie into one raw buffer (bulk copies; loads would go through the 28 KB that
-// L1 has left), prefetched into L2 while the buffer is still in use (8 heads ragged 100
-// -> 96 us from memory; 1 - 2% slower where the cache lies in L2 already). Warps 0-15, four keys each, take the codes into registers, expand
-// them and store K (keys x 576, K-major) and V (this CTA's 256 columns, MN-major):
-// its own keys' from the same registers, the other CTA's by loads a tile ahead,
-// which hit L2 (passing them between the CTAs' shared memory took 6600 cycles a
-// tile). Two tail warps copy the rotary part. 16-bit rows go to K and V by
-// cp.async. Warps 16-23 are the softmax, a thread a row and 32 keys (rows are TMEM
-// lanes: no shuffles), read into registers once, so that S is free at once. One warp of CTA 0 issues the MMAs, in uniform control flow
-// with one elected lane (80-130 cycles each otherwise, 45-64 now). Q lies in
-// tensor memory but for three of its nine 64-column blocks. QK(t+1) is issued
-// before PV(t), so K(t+1) is stored under PV(t-1), V(t) under QK(t+1), and the
-// softmax of t runs under PV(t-1). The roles meet at mbarriers and run on through
-// the segments. Every wait is bounded.
+// Roles (28 warps, 72 registers): the row warp walks the run, turns positions into
+// cache rows, and has this CTA's 64 rows of an fp8 tile copied as they lie into one
+// raw buffer (bulk copies; loads would go through the 28 KB that L1 has left),
+// prefetched into L2 while the buffer is still in use (8 heads ragged 100 -> 96 us
+// from memory; 1 - 2% slower where the cache lies in L2 already). Warps 0-15, four
+// keys each, take the codes into registers, expand them and store K (keys x 576,
+// K-major) and V (this CTA's 256 columns, MN-major): its own keys' from the same
+// registers, the other CTA's by loads a tile ahead, which hit L2 (passing them
+// between the CTAs' shared memory took 6600 cycles a tile). Two tail warps copy the
+// rotary part. 16-bit rows go to K and V by cp.async. Warps 16-23 are the softmax,
+// a thread a row and 32 keys (rows are TMEM lanes: no shuffles), read into
+// registers once, so that S is free at once. One warp of CTA 0 issues the MMAs, in
+// uniform control flow with one elected lane (80-130 cycles each otherwise, 45-64
+// now). Q lies in tensor memory but for three of its nine 64-column blocks. QK(t+1)
+// is issued before PV(t), so K(t+1) is stored under PV(t-1), V(t) under QK(t+1),
+// and the softmax of t runs under PV(t-1). The roles meet at mbarriers and run on
+// through the segments. Every wait is bounded.
 //
-// Arithmetic: f16 operands (bf16 for a bf16 cache), f32 sums, maximum and state.
-// An fp8 value code * scale rounded once to f16 is off by half a step, 2^-11, which
-// puts 2e-4 on a score; lse averages that over the keys that weigh: 1e-6 of it
-// is left at 25,000 positions of N(0, 1) values, 6e-6 at 800. So a score takes one
+// Arithmetic: f16 operands (bf16 for a bf16 cache), f32 sums, maximum and state. An
+// fp8 value code * scale rounded once to f16 is off by half a step, 2^-11, which
+// puts 2e-4 on a score; lse averages that over the keys that weigh: 1e-6 of it is
+// left at 25,000 positions of N(0, 1) values, 6e-6 at 800. So a score takes one
 // product beyond 32768 positions. Up to there it takes two: the scale is cut into
 // hi (7 bits: code * hi is exact in f16) and lo, and K is stored and multiplied
 // with lo, then with hi, into the same S (the small products first: the sum keeps
-// them): lse is within 3e-7. Up to 1024 positions the second product is the
-// rounding's own remainder, and V's is multiplied too (fewer keys average less).
-// Both sides, 8 heads x 16 drafts, 8 requests of 13,824 to 24,576 positions:
-// one product 74 us and 1.1e-6, two 100 us and 1.5e-7; 64 heads x 8 drafts, 4 x
-// 24,576: 133 us and 9.5e-7, 188 us and 1.7e-7. bf16 q is shifted by a power of
-// two per row into f16's range, which the row's scale undoes exactly. The running
-// maximum moves only when a score exceeds it by 2^8, so P <= 256 and O is rarely
-// rescaled.
+// them): lse is within 7e-7, 2e-7 from 5,000 positions on. Up to 1024 positions the
+// second product is the rounding's own remainder, and V's is multiplied too (fewer
+// keys average less). Both sides, 8 heads x 16 drafts, 8 requests of 13,824 to
+// 24,576 positions: one product 74 us and 1.1e-6, two 100 us and 1.5e-7; 64 heads x
+// 8 drafts, 4 x 24,576: 133 us and 9.5e-7, 188 us and 1.7e-7. bf16 q is shifted by
+// a power of two per row into f16's range, which the row's scale undoes exactly.
+// The running maximum moves only when a score exceeds it by 2^8, so P <= 256 and O
+// is rarely rescaled.
 //
 // Measured (times with the merge): 32 drafts x 64 heads over 131,072 positions, fp8
-// 572 - 586 us = 1.0 PFLOP/s, 62% of the rate of a plain matrix product (690 in a long
-// loop, whose clocks the power limit lowers), 16-bit cache 544 us. A tile takes a CTA
-// 5000 cycles, the tensor cores 2700 of them: the
-// bound is the producers' chain, K and V of a tile after one another, each store
-// (8 x 8 codes a lane) 1300 cycles of issue and latency and 700 of waits and fences.
-// With two products K is stored twice, 7800 cycles. The code of the loops counts: an
-// SM's instruction cache misses go to a cache that several share, and took 76% of its
-// rate before the loops were cut (23% now), so the usual path has no calls,
-// the rare ones (scales out of f16's range, remainders) are rolled, and a wait is
-// three instructions.
+// 572 - 586 us = 1.0 PFLOP/s, 62% of the rate of a plain matrix product (690 in a
+// long loop, whose clocks the power limit lowers), 16-bit cache 544 us. A tile
+// takes a CTA 5000 cycles, the tensor cores 2700 of them: the bound is the
+// producers' chain, K and V of a tile after one another, each store (8 x 8 codes a
+// lane) 1300 cycles of issue and latency and 700 of waits and fences. With two
+// products K is stored twice, 7800 cycles. The code of the loops counts: an SM's
+// instruction cache misses go to a cache that several share, and took 76% of its
+// rate before the loops were cut (23% now), so the usual path has no calls, the
+// rare ones (scales out of f16's range, remainders) are rolled, and a wait is three
+// instructions.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
