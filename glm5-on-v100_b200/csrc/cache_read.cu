@@ -262,8 +262,8 @@ extern "C" int dsa_gather_cache(void* out, int out_dtype, int64_t out_stride, in
   const int need = cache_format == DSA_FP8_DS_MLA ? 576 : cache_format == DSA_FP8_IDXK ? 128 : width;
   DSA_REQUIRE(width == need && width > 0 && width % 8 == 0, DSA_ERR_INVALID,
               "gather_cache: rows of this cache hold %d values (a multiple of 8; got width %d)", need, width);
-  DSA_REQUIRE(n_out >= 0 && B >= 0 && n_rows >= 0 && page_size > 0 && max_blocks >= 0 && bt_stride >= max_blocks &&
-                  out_stride >= width,
+  DSA_REQUIRE(n_out >= 0 && B >= 0 && n_rows >= 0 && page_size > 0 && max_blocks >= 0 &&
+                  row_stride_ok(bt_stride, max_blocks) && out_stride >= width,
               DSA_ERR_INVALID, "gather_cache: bad sizes or strides");
   if (n_out == 0 || B == 0) return DSA_OK;
   DSA_REQUIRE(out && cu_seq_lens && (n_rows == 0 || cache) && (max_blocks == 0 || block_table), DSA_ERR_INVALID,
@@ -290,8 +290,11 @@ extern "C" int dsa_commit_draft_rows(void* const* caches, int n_caches, int64_t 
                                      const int32_t* accepted, int64_t acc_stride, int n_accept, int B, void* stream) {
   clear_error();
   DSA_REQUIRE(n_caches >= 0 && B >= 0 && n_accept >= 0 && n_drafts >= 0 && n_rows >= 0 && page_size > 0 &&
-                  max_blocks >= 0 && bt_stride >= max_blocks && acc_stride >= n_accept,
+                  max_blocks >= 0 && row_stride_ok(bt_stride, max_blocks) && row_stride_ok(acc_stride, n_accept),
               DSA_ERR_INVALID, "commit_draft_rows: bad sizes or strides");
+  // requests whose drafts are the same rows would move them under one another
+  DSA_REQUIRE(B <= 1 || max_blocks == 0 || bt_stride > 0, DSA_ERR_INVALID,
+              "commit_draft_rows: each request needs its own row of the block table");
   DSA_REQUIRE(n_drafts <= kMaxAccept && n_accept <= kMaxAccept, DSA_ERR_UNSUPPORTED,
               "commit_draft_rows: at most 64 drafts (got %d, %d accepted)", n_drafts, n_accept);
   const bool wide = row_bytes % 16 == 0;

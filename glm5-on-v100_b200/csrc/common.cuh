@@ -42,6 +42,10 @@ int check_launch(const char* what);
     }                                                                      \
   } while (0)
 
+// Row stride of a per-request input that is only read: rows do not overlap, or all
+// requests share one (0: an expanded tensor).
+inline bool row_stride_ok(int64_t stride, int64_t width) { return stride == 0 || stride >= width; }
+
 // Per-device one-time initialisation (function attributes are per device).
 constexpr int kMaxDevices = 64;
 int current_device();

@@ -1397,7 +1397,7 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
   DSA_REQUIRE(!(kv_format == DSA_BF16 && q_dtype == DSA_F16), DSA_ERR_UNSUPPORTED,
               "tree_mla_decode: a bf16 cache needs bf16 q");
   DSA_REQUIRE(page_size > 0 && max_blocks >= 0 && n_kv_rows >= 0 && n_kv_rows <= 0x7fffffff &&
-                  bt_stride >= max_blocks && mask_stride >= T,
+                  row_stride_ok(bt_stride, max_blocks) && row_stride_ok(mask_stride, T),
               DSA_ERR_INVALID, "tree_mla_decode: bad cache geometry or strides (page=%d max_blocks=%d rows=%lld)",
               page_size, max_blocks, (long long)n_kv_rows);
   DSA_REQUIRE(std::isfinite(scale), DSA_ERR_INVALID, "tree_mla_decode: scale must be finite");

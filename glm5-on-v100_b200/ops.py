@@ -520,18 +520,23 @@ def _vector(t, n, name, shape="[B]"):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _row_stride(t, rows):
+    """Elements from one of the `rows` used rows of a 2-D tensor to the next: 0 where
+    an expanded tensor repeats one row. A single row's stride may be anything."""
+    return t.stride(0) if rows > 1 else t.size(1)
+
+
 def _pages(block_table, B):
     """(pointer, row stride, blocks a row) of a block table of at least B rows."""
     if block_table.dtype != torch.int32 or block_table.dim() != 2:
         raise RuntimeError("block_table must be 2-D int32")
     n, width = block_table.shape
-    stride, inner = block_table.stride()
-    if inner != 1:
+    if block_table.stride(1) != 1:
         raise RuntimeError("block_table must have unit inner stride")
     if n < B:
         raise RuntimeError(f"block_table has fewer than {B} rows")
     _fits(B, width)
-    return block_table.data_ptr(), max(stride, width), width
+    return block_table.data_ptr(), _row_stride(block_table, B), width
 
 
 def _latent_format(kv_cache):
@@ -571,8 +576,7 @@ def _tree_mla_decode_impl(o, lse, q, kv_cache, block_table, seq_lens, tree_mask,
     mask = tree_mask.shape
     if tree_mask.dtype != torch.int64 or len(mask) != 2 or mask[0] < B or mask[1] != T:
         raise RuntimeError("tree_mask must be int64 [B, T]")
-    mask_stride, inner = tree_mask.stride()
-    if T > 1 and inner != 1:
+    if T > 1 and tree_mask.stride(1) != 1:
         raise RuntimeError("tree_mask must have unit inner stride")
     page = kv_cache.size(-2)
     _check(page > 0, "kv_cache has no rows in a page")
@@ -585,7 +589,7 @@ def _tree_mla_decode_impl(o, lse, q, kv_cache, block_table, seq_lens, tree_mask,
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     _launch(index, "dsa_tree_mla_decode", o.data_ptr(), _DTYPE[o_dtype], lse.data_ptr(), q.data_ptr(), _DTYPE[q_dtype],
             kv_cache.data_ptr(), fmt, kv_cache.numel() // row, page, *pages, seq_lens.data_ptr(), _ptr(draft_lens),
-            tree_mask.data_ptr(), max(mask_stride, T), B, T, H, scale, _ptr(ws), ws_bytes)
+            tree_mask.data_ptr(), _row_stride(tree_mask, B), B, T, H, scale, _ptr(ws), ws_bytes)
 
 
 def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens):
@@ -616,7 +620,7 @@ def _commit_draft_rows_impl(caches, block_table, seq_lens, accepted, draft_lens)
     _fits(shape[-2], width * c0.element_size(), A)
     _launch(index, "dsa_commit_draft_rows", (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), n // width, shape[-2],
             width * c0.element_size(), *pages, seq_lens.data_ptr(), draft_lens.data_ptr(), 64, accepted.data_ptr(),
-            max(accepted.stride(0), A), A, B)
+            _row_stride(accepted, B), A, B)
 
 
 def _gather_cache_impl(out, cache, block_table, cu_seq_lens, seq_starts):

@@ -416,7 +416,9 @@ int dsa_shard_exchange_merge(int32_t* out, int64_t out_stride,
  *
  * q      [B, T, n_head, 576] f16 or bf16, contiguous (bf16 with a bf16 cache)
  * kv     f16/bf16 [.., page, 576] or u8 [.., page, 656] (DSA_FP8_DS_MLA)
- * tree_mask int64 [B, T], row stride mask_stride; T <= 64
+ * tree_mask int64 [B, T], row stride mask_stride; T <= 64. A bt_stride or
+ *   mask_stride of 0 gives every request the first row (one tree for all, one
+ *   context read by all); otherwise they are at least max_blocks and T
  * o      [B, T, n_head, 512] f16 or bf16, contiguous; lse f32 [B, T, n_head]
  * workspace: at least dsa_tree_mla_decode_workspace_bytes(B, T, n_head) bytes
  *   of device memory, 16-byte aligned (may be NULL when that is 0); calls that
@@ -441,7 +443,9 @@ int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void* q,
  * before any is written. Entries below 0 or not below the request's draft
  * count, and rows outside the block table or the cache, are skipped.
  * row_bytes: a multiple of 16 up to 1152, or of 4 up to 132. n_drafts and
- * n_accept <= 64. */
+ * n_accept <= 64. An acc_stride of 0 gives every request the same path. The
+ * drafts of different requests must be different cache rows: with B > 1 a
+ * bt_stride of 0 is refused. */
 int dsa_commit_draft_rows(void* const* caches, int n_caches, int64_t n_rows,
                           int page_size, int row_bytes,
                           const int32_t* block_table, int64_t bt_stride,
@@ -459,7 +463,7 @@ int dsa_commit_draft_rows(void* const* caches, int n_caches, int64_t n_rows,
  * f16 rotary tail), DSA_FP8_IDXK (128 values), or DSA_F16 / DSA_BF16 rows of
  * `width` values (a multiple of 8). One rounding, to out's type.
  * out [n_out, width] f16/bf16, row stride out_stride (elements, multiple of 8);
- * cu_seq_lens int32 [B + 1] ascending. */
+ * cu_seq_lens int32 [B + 1] ascending; bt_stride 0: one table row for all. */
 int dsa_gather_cache(void* out, int out_dtype, int64_t out_stride, int n_out,
                      const void* cache, int cache_format, int64_t n_rows,
                      int page_size, int width, const int32_t* block_table,

@@ -806,3 +806,50 @@ def test_commit_gather_and_rotary_in_a_graph(dsa):
         rows = [row(b, p) for b in range(B) for p in range(min(n[b], 66))]
         assert torch.equal(out[:len(rows)], want[rows].to(BF)) and bool((out[len(rows):] == 3.0).all())
         assert torch.equal(turned, rope_f32(x, table, pos, 0, False))
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "bf16"])
+def test_one_tree_and_one_table_row_for_a_batch(dsa, oracle, fmt):
+    """Masks, tables and paths expanded over the batch give what their copies give."""
+    B, T, H, L = 5, 6, 8, 300
+    row, pages = tables([L], 64, 1)
+    cache = make_cache(fmt, pages, 64, 2, oracle)
+    q = torch.randn(B, T, H, 576, generator=gen(3), device=DEV).to(BF)
+    tree = random_masks(dsa, 1, T, 4)
+    lens = [300, 299, 64, 7, 130]
+    ln = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    outs = []
+    for share in (False, True):
+        mask, bt = tree.expand(B, T), row.expand(B, row.shape[1])
+        if not share:
+            mask, bt = mask.contiguous(), bt.contiguous()
+        o, lse = torch.empty(B, T, H, 512, dtype=BF, device=DEV), torch.empty(B, T, H, device=DEV)
+        dsa.tree_mla_decode(o, lse, q, cache, bt, ln, mask, SCALE)
+        back = torch.full((sum(lens), 576), 9.0, dtype=BF, device=DEV)
+        cu = torch.tensor([0, *np.cumsum(lens)], dtype=torch.int32, device=DEV)
+        dsa.gather_cache(back, cache, bt, cu)
+        outs.append((o, lse, back))
+    check_tree(outs[0][0], outs[0][1], tree64(q, cache, row.expand(B, -1), lens, tree.expand(B, T), None, SCALE), fmt)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    half = torch.as_strided(tree.expand(B, T).contiguous(), (B, T), (T - 1, 1))  # rows that overlap in part
+    with pytest.raises(RuntimeError):
+        dsa.tree_mla_decode(outs[0][0], outs[0][1], q, cache, row.expand(B, -1), ln, half, SCALE)
+
+
+def test_commit_of_one_path_for_a_batch(dsa):
+    B, T, page = 3, 8, 16
+    lens = [40, 20, 33]
+    bt, pages = tables(lens, page, 5)
+    pool = torch.randint(0, 255, (pages, page, 132), generator=gen(6), device=DEV, dtype=torch.int32).to(torch.uint8)
+    acc = torch.tensor([[1, 3, 4, 7, -1]], dtype=torch.int32, device=DEV)
+    ln, dl = torch.tensor(lens, dtype=torch.int32, device=DEV), torch.full((B,), T, dtype=torch.int32, device=DEV)
+    want = pool.clone()
+    dsa.commit_draft_rows([want], bt, ln, acc.expand(B, -1).contiguous(), dl)
+    assert not torch.equal(want, pool)
+    before = pool.clone()
+    with pytest.raises(RuntimeError, match="row of the block table"):
+        dsa.commit_draft_rows([pool], bt[:1].expand(B, -1), ln, acc.expand(B, -1), dl)
+    assert torch.equal(pool, before)
+    dsa.commit_draft_rows([pool], bt, ln, acc.expand(B, -1), dl)
+    assert torch.equal(pool, want)

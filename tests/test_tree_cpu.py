@@ -193,3 +193,38 @@ def test_new_ops_registered(dsa):
         "o", "lse", "q", "kv_cache", "block_table", "seq_lens", "tree_mask", "draft_lens", "scale"]
     for name in ("tree_mla_decode", "commit_draft_rows", "gather_cache", "rotary_embedding"):
         assert hasattr(ns, name) and callable(getattr(dsa, name))
+
+
+def test_expanded_rows_keep_their_stride(dsa):
+    """One tree, path or table row shared by a batch (expand) has a row stride of 0:
+    the entry points get that, not the width, which would take them past its storage."""
+    ops, L, lib = _ops(dsa), dsa._lib, dsa._lib.lib()
+    one = torch.arange(3, dtype=torch.int32)[None]
+    assert ops._pages(one.expand(4, 3), 4)[1:] == (0, 3)
+    assert ops._pages(one, 1)[1:] == (3, 3)
+    assert ops._pages(torch.as_strided(one, (1, 3), (1, 1)), 1)[1:] == (3, 3)  # one row: any stride
+    assert ops._pages(torch.zeros(4, 9, dtype=torch.int32)[:, 2:5], 4)[1:] == (9, 3)
+    assert ops._pages(torch.as_strided(torch.zeros(9, dtype=torch.int32), (4, 3), (2, 1)), 4)[1:] == (2, 3)
+    # the entries take 0 and what rows that do not overlap have, nothing between
+    P = ctypes.c_void_p
+    for stride, code in [(0, L.DSA_OK), (4, L.DSA_OK), (9, L.DSA_OK), (1, L.DSA_ERR_INVALID), (3, L.DSA_ERR_INVALID),
+                         (-4, L.DSA_ERR_INVALID)]:
+        assert _tree(lib, B=0, bts=stride) == code, stride
+        assert _tree(lib, B=0, T=4, ms=stride) == code, stride
+        assert lib.dsa_gather_cache(P(1024), 1, 576, 4, P(1024), 3, 640, 64, 576, P(1024), stride, 4, P(1024), None, 0,
+                                    None) == code, stride
+        caches = (ctypes.c_void_p * 1)(1024)
+        assert lib.dsa_commit_draft_rows(caches, 1, 640, 64, 656, P(1024), 4, 4, P(1024), P(1024), 64, P(1024), stride, 4, 0,
+                                         None) == code, stride
+
+
+def test_commit_entry_refuses_one_table_row_for_several_requests(dsa):
+    L, lib = dsa._lib, dsa._lib.lib()
+    P = ctypes.c_void_p
+
+    def call(B, bts, rows=0):
+        return lib.dsa_commit_draft_rows((ctypes.c_void_p * 1)(1024), 1, rows, 64, 656, P(1024), bts, 4, P(1024), P(1024),
+                                         64, P(1024), 8, 8, B, None)
+
+    assert call(2, 0, rows=640) == L.DSA_ERR_INVALID
+    assert call(1, 0) == L.DSA_OK and call(2, 4) == L.DSA_OK  # (a cache without rows: nothing to move)
