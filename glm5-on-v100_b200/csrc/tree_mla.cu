@@ -57,8 +57,12 @@
 // 24,576 positions: one product 74 us and 1.1e-6, two 100 us and 1.5e-7; 64 heads x
 // 8 drafts, 4 x 24,576: 133 us and 9.5e-7, 188 us and 1.7e-7. bf16 q is shifted by
 // a power of two per row into f16's range, which the row's scale undoes exactly.
-// The running maximum moves only when a score exceeds it by 2^8, so P <= 256 and O
-// is rarely rescaled.
+// Probabilities are 2^(z - m) with m 7 below the running maximum, in log2 units, and
+// m moves only when a score exceeds it by 15: P <= 2^15 uses f16's range at both ends,
+// and O is rarely rescaled. Without the 7 the faint keys of a long context became zeros
+// in P while the sum kept them: one key 17.5 nats above 131,071 others of value 1, its
+// own 1/2, gave o = 0.4983 for 0.5016; 0.5005 now. What is left is the tensor cores'
+// f32 accumulator, which cuts a product two bits below its own last place.
 //
 // Measured (times with the merge): 32 drafts x 64 heads over 131,072 positions, fp8
 // 572 - 586 us = 1.0 PFLOP/s, 62% of the rate of a plain matrix product (690 in a
@@ -113,7 +117,8 @@ constexpr uint32_t TMEM_COLS = 512;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kNoMax = -1e30f;
 constexpr int kMaxSeq = 0x7fffff00;   // tile ends stay in 32 bits
-constexpr float kRescale = 8.0f;       // log2 units
+constexpr float kHead = 7.0f;          // log2 units: a new maximum's probability is 2^kHead
+constexpr float kRescale = 15.0f;      // and none is above 2^kRescale, inside f16
 constexpr int kTwoPassKeys = 32768;    // fp8: two products to a score up to here
 constexpr int kFineKeys = 1024;        // and up to here the second is the rounding's remainder
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -1087,8 +1092,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_mla_kernel(const TreeArgs p,
           named_bar(1, kSoftmaxWarps * 32);
           const float rm = fmaxf(fmaxf(rowx[row], rowx[64 + row]), fmaxf(rowx[128 + row], rowx[192 + row]));
           if (rm > m + kRescale) {
-            alpha = ex2(m - rm);
-            m = rm;
+            alpha = ex2(m - (rm - kHead));
+            m = rm - kHead;
             L *= alpha;
           }
         }

@@ -853,3 +853,45 @@ def test_commit_of_one_path_for_a_batch(dsa):
     assert torch.equal(pool, before)
     dsa.commit_draft_rows([pool], bt, ln, acc.expand(B, -1), dl)
     assert torch.equal(pool, want)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("fp8", HF), ("f16", HF), ("bf16", BF)])
+@pytest.mark.parametrize("at", [0, 70_000, 131_071])
+def test_tree_many_faint_keys_beside_a_strong_one(dsa, oracle, fmt, dtype, at):
+    """One key 17.5 nats above 131,071 others, whose weights of e^-17.5 = 1.7 * 2^-26
+    add up to 0.0033 of the row. As many requests as there are CTA pairs, so that a
+    pair's run is a whole context. All values are 1 but the strong key's, 1/2, so o
+    = (1/2 + n w) / (1 + n w). Off are: a faint probability, by at most half a step of
+    the 16-bit type (2^-11, bf16 2^-8) or 2^-25 of a scale of 2^7; its product, once the
+    accumulator holds the strong one (2^6: last place 2^-17), by less than a quarter of
+    that place, 2^-19 / 2^7 of o; the sum, by half a step at each of its 1024 tiles; o,
+    by its own half step. (Faint probabilities that became zeros made 0.0033.)"""
+    n, B, page = 131_072, torch.cuda.get_device_properties(0).multi_processor_count // 2, 64
+    pages = n // page
+    x = torch.zeros(n, 576, device=DEV)
+    x[:, :512] = 1.0
+    x[at, :512] = 0.5
+    x[at, 575] = 1.0  # only the rotary part of q is set: the scores
+    if fmt == "fp8":
+        cache = torch.zeros(n, 656, dtype=torch.uint8, device=DEV)
+        cache[:, :512] = x[:, :512].to(torch.float8_e4m3fn).view(torch.uint8)
+        cache[:, 512:528] = torch.ones(n, 4, device=DEV).view(torch.uint8)
+        cache[:, 528:] = x[:, 512:].half().contiguous().view(torch.uint8)
+        cache = cache.view(pages, page, 656)
+    else:
+        cache = x.to(HF if fmt == "f16" else BF).view(pages, page, 576)
+    q = torch.zeros(B, 1, 2, 576, dtype=dtype, device=DEV)
+    q[..., 575] = 17.5
+    bt = torch.arange(pages, dtype=torch.int32, device=DEV)[None].expand(B, -1).contiguous()
+    ln = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    mask = torch.ones(B, 1, dtype=torch.int64, device=DEV)
+    o, lse = torch.empty(B, 1, 2, 512, dtype=dtype, device=DEV), torch.empty(B, 1, 2, device=DEV)
+    dsa.tree_mla_decode(o, lse, q, cache, bt, ln, mask, 1.0)
+    w = (n - 1) * np.exp(-17.5)
+    half = 2.0 ** -8 if dtype == BF else 2.0 ** -11
+    want = (0.5 + w) / (1 + w)
+    total = (n // 128 + 128) * 2.0 ** -24  # of the sum: tiles, and the additions inside one and of the quarters
+    tol = w * half + n * 2.0 ** -32 + (n - at) * 2.0 ** -26 + want * total + half * want
+    err = float((o.double() - want).abs().max())
+    assert err <= tol, (err, tol)
+    assert float((lse.double() - (17.5 + np.log1p(w))).abs().max()) <= total + 2.0 ** -20 + 2.0 ** -22 * 17.5
