@@ -86,6 +86,10 @@ def draft_tree_masks(parents: torch.Tensor):
     return mask, depth
 
 
+def _as_int32(t):
+    return t if t is None or t.dtype == torch.int32 or t.is_floating_point() else t.to(torch.int32)
+
+
 def forward_mqa_tree(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                      tree_mask: torch.Tensor, scale: float, draft_lens: torch.Tensor | None = None,
                      kv_lora_rank: int = 512):
@@ -94,17 +98,21 @@ def forward_mqa_tree(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch
     (where expand_spec_rows turns a line of drafts into independent rows).
 
     q [B, T, H, 576], or the step's tokens [B * T, H, 576] with tree_mask [B,
-    T]; seq_lens counts the drafts. Returns (o in q's dtype and leading shape,
-    [.., H, 512], lse f32 [.., H]).
+    T]; f16 or bf16 (bf16 with a bf16 cache). Other types are rounded to bf16
+    for a bf16 cache and else to f16, where values beyond 65504 are infinite
+    (bf16 q of any magnitude is served by every cache). seq_lens counts the drafts; lengths and table
+    of any integer type. Returns (o in the 16-bit type that q came in or was
+    rounded to, in q's leading shape, [.., H, 512], lse f32 [.., H]).
     """
     B, T = tree_mask.shape
     lead = q.shape[:-1]
     if q.dim() != 4:
         q = q.reshape(B, T, q.shape[-2], q.shape[-1])
     if q.dtype not in (torch.float16, torch.bfloat16):
-        q = q.to(torch.float16)
+        q = q.to(torch.bfloat16 if kv_cache.dtype == torch.bfloat16 else torch.float16)
     if not q.is_contiguous():
         q = q.contiguous()
+    block_table, seq_lens, draft_lens = map(_as_int32, (block_table, seq_lens, draft_lens))
     B, T, H, _ = q.shape
     o = q.new_empty((B, T, H, kv_lora_rank))
     lse = torch.empty((B, T, H), dtype=torch.float32, device=q.device)

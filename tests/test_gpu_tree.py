@@ -895,3 +895,24 @@ def test_tree_many_faint_keys_beside_a_strong_one(dsa, oracle, fmt, dtype, at):
     err = float((o.double() - want).abs().max())
     assert err <= tol, (err, tol)
     assert float((lse.double() - (17.5 + np.log1p(w))).abs().max()) <= total + 2.0 ** -20 + 2.0 ** -22 * 17.5
+
+
+@pytest.mark.parametrize("fmt,served", [("fp8", HF), ("f16", HF), ("bf16", BF)])
+def test_forward_mqa_tree_takes_f32_queries_and_64_bit_integers(dsa, oracle, fmt, served):
+    """f32 q is rounded to the type that the cache's products take; o comes in it."""
+    B, T, H, lens, drafts = 2, 3, 8, [300, 70], [3, 2]
+    bt, pages = tables(lens, 64, 1)
+    cache = make_cache(fmt, pages, 64, 2, oracle)
+    q = torch.randn(B, T, H, 576, generator=gen(3), device=DEV)
+    mask = random_masks(dsa, B, T, 4)
+    ln, dl = torch.tensor(lens, dtype=torch.int32, device=DEV), torch.tensor(drafts, dtype=torch.int32, device=DEV)
+    o, lse = dsa.mla_sparse.forward_mqa_tree(q, cache, bt, ln, mask, SCALE, draft_lens=dl)
+    assert o.dtype == served and o.shape == (B, T, H, 512) and lse.dtype == F32
+    check_tree(o, lse, tree64(q.to(served), cache, bt, lens, mask, drafts, SCALE), fmt)
+    for k in range(4):
+        o2, lse2 = dsa.mla_sparse.forward_mqa_tree(q.to(served).view(B * T, H, 576) if k == 3 else q, cache,
+                                                   bt.long() if k != 1 else bt, ln.long() if k != 2 else ln, mask, SCALE,
+                                                   draft_lens=dl.long() if k else dl)
+        assert torch.equal(o2.view_as(o), o) and torch.equal(lse2.view_as(lse), lse)
+    with pytest.raises(RuntimeError):
+        dsa.mla_sparse.forward_mqa_tree(q, cache, bt, ln.float(), mask, SCALE)

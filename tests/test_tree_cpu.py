@@ -228,3 +228,19 @@ def test_commit_entry_refuses_one_table_row_for_several_requests(dsa):
 
     assert call(2, 0, rows=640) == L.DSA_ERR_INVALID
     assert call(1, 0) == L.DSA_OK and call(2, 4) == L.DSA_OK  # (a cache without rows: nothing to move)
+
+
+def test_tree_wrapper_rounds_queries_to_the_cache_type(dsa, monkeypatch):
+    """What forward_mqa_tree hands to the operator, for each type of q and cache."""
+    seen = {}
+    monkeypatch.setattr(dsa.ops, "tree_mla_decode", lambda o, lse, q, kv, bt, ln, mask, scale, dl: seen.update(
+        o=o.dtype, q=q.dtype, bt=bt.dtype, ln=ln.dtype, dl=None if dl is None else dl.dtype))
+    bf, hf, f32, i32, i64 = torch.bfloat16, torch.float16, torch.float32, torch.int32, torch.int64
+    for q, kv, want in [(f32, bf, bf), (f32, hf, hf), (f32, torch.uint8, hf), (torch.float64, bf, bf), (bf, hf, bf),
+                        (hf, torch.uint8, hf), (bf, torch.uint8, bf)]:
+        for lens in (None, torch.ones(1, dtype=i64), torch.ones(1, dtype=i32)):
+            o, lse = dsa.mla_sparse.forward_mqa_tree(torch.zeros(1, 2, 3, 576, dtype=q), torch.zeros(1, 64, 576).to(kv),
+                                                     torch.zeros(1, 1, dtype=i64), torch.ones(1, dtype=i64),
+                                                     torch.ones(1, 2, dtype=i64), 1.0, draft_lens=lens)
+            assert seen == dict(o=want, q=want, bt=i32, ln=i32, dl=None if lens is None else i32)
+            assert o.dtype == want and o.shape == (1, 2, 3, 512) and lse.shape == (1, 2, 3)
