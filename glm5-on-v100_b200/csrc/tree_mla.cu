@@ -45,18 +45,25 @@
 // through the segments. Every wait is bounded.
 //
 // Arithmetic: f16 operands (bf16 for a bf16 cache), f32 sums, maximum and state. An
-// fp8 value code * scale rounded once to f16 is off by half a step, 2^-11, which
-// puts 2e-4 on a score; lse averages that over the keys that weigh: 1e-6 of it is
-// left at 25,000 positions of N(0, 1) values, 6e-6 at 800. So a score takes one
-// product beyond 32768 positions. Up to there it takes two: the scale is cut into
-// hi (7 bits: code * hi is exact in f16) and lo, and K is stored and multiplied
-// with lo, then with hi, into the same S (the small products first: the sum keeps
-// them): lse is within 7e-7, 2e-7 from 5,000 positions on. Up to 1024 positions the
-// second product is the rounding's own remainder, and V's is multiplied too (fewer
-// keys average less). Both sides, 8 heads x 16 drafts, 8 requests of 13,824 to
-// 24,576 positions: one product 74 us and 1.1e-6, two 100 us and 1.5e-7; 64 heads x
-// 8 drafts, 4 x 24,576: 133 us and 9.5e-7, 188 us and 1.7e-7. bf16 q is shifted by
-// a power of two per row into f16's range, which the row's scale undoes exactly.
+// fp8 value code * scale rounded once to f16 is off by up to half a step, 2^-11, which
+// puts up to 2^-11 * scale * sum_d |q_d kv_d| on a score, 2e-4 for N(0, 1) rows and
+// queries. Rows that weigh many keys average it (lse 1e-6 at 25,000 positions); where
+// one key carries the row, lse and the weights keep it: with queries 4 times as large
+// lse is off by 9e-4 (rms) and f16 o by 7e-4 of its norm at 32,769 positions, by 3e-5
+// and 3e-4 at 32,768; bf16 o by 1.8e-3 and 1.7e-3. Beyond 32768 positions a score
+// takes that one product all the same, because the second costs half as much
+// again there (131,072 positions x 32 x 64: 584 us, 870 with two). Up to 32768 it takes
+// two: the scale is cut into hi (7 bits: code * hi is exact in f16) and lo, and K is
+// stored and multiplied with lo, then with hi, into the same S (the small products
+// first: the sum keeps them): 2^-16 of a value, 2^-15 where scales are below 2^-8.
+// Up to 1024 positions the second product is the rounding's own remainder, and V's is
+// multiplied too (fewer keys average less). N(0, 1) rows, 8 heads x 16 drafts, 8
+// requests of 13,824 to 24,576 positions: one product 74 us and lse within 1.1e-6, two
+// 100 us and 1.5e-7; 64 heads x 8 drafts, 4 x 24,576: 133 us and 9.5e-7, 188 us and
+// 1.7e-7. V's values are rounded to f16 once beyond 1024 positions (o 14% farther from
+// 64 bits than with exact ones, f16 o), a bf16 cache's probabilities to bf16, as both
+// operands of a product have one type (o 14% too). bf16 q is shifted by a power of two
+// per row into f16's range, which the row's scale undoes exactly.
 // Probabilities are 2^(z - m) with m 7 below the running maximum, in log2 units, and
 // m moves only when a score exceeds it by 15: P <= 2^15 uses f16's range at both ends,
 // and O is rarely rescaled. Without the 7 the faint keys of a long context became zeros

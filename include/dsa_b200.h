@@ -412,7 +412,14 @@ int dsa_shard_exchange_merge(int32_t* out, int64_t out_stride,
  * cache row outside [0, n_kv_rows), or past the block table, reads as zeros.
  * A position that some rows see must hold finite values: its NaN or infinity
  * reaches the other rows of the request too. Values of an fp8 cache enter the
- * products as f16, so one beyond 65504 counts as infinite.
+ * products as f16, so one beyond 65504 counts as infinite, and none is held
+ * finer than 2^-24.
+ * Roundings ahead of the f32 sums, relative to the value: scores of a 16-bit
+ * cache none, an fp8 key's values 2^-16 (5 * 2^-17 where their scale is 2^-10
+ * to 2^-8) in requests of up to 32768 positions and 2^-11 in longer ones, for
+ * speed: there a score may be off by 2^-11 * scale * sum_d |q_d kv_d|, and lse
+ * with it where one key carries a row. Probabilities 2^-11 (bf16 cache: 2^-8);
+ * fp8 values under them 2^-22 up to 1024 positions, 2^-11 beyond.
  *
  * q      [B, T, n_head, 576] f16 or bf16, contiguous (bf16 with a bf16 cache)
  * kv     f16/bf16 [.., page, 576] or u8 [.., page, 656] (DSA_FP8_DS_MLA)

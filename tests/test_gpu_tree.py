@@ -916,3 +916,32 @@ def test_forward_mqa_tree_takes_f32_queries_and_64_bit_integers(dsa, oracle, fmt
         assert torch.equal(o2.view_as(o), o) and torch.equal(lse2.view_as(lse), lse)
     with pytest.raises(RuntimeError):
         dsa.mla_sparse.forward_mqa_tree(q, cache, bt, ln.float(), mask, SCALE)
+
+
+@pytest.mark.parametrize("lens,amp,step", [([32768, 32000], 1.0, 2.0 ** -16), ([32769, 33000], 1.0, 2.0 ** -11),
+                                           ([1500, 9001], 0.25, 5 * 2.0 ** -17), ([1024, 700], 0.25, 2.0 ** -22)])
+def test_tree_lse_of_peaked_rows(dsa, oracle, lens, amp, step):
+    """Queries so large that a key or two carry each row, so that lse keeps the error
+    of their scores. An fp8 key's value is held to `step` of itself: two products to a
+    score up to 32768 positions, one beyond, scales of 2^-10 to 2^-8 (amp 1/4: N(0, 1)
+    rows have 2^-7.9 to 2^-6.6) cut less finely, up to 1024 positions the first
+    product's own remainder. In the 2-norm that leaves step / sqrt 3 of the latent
+    part's terms. The f32 accumulator cuts each of the up to 1152 products below a
+    quarter of its last place, 2^-25 of a partial sum, and those are taken as no larger
+    than twice the score; each of the 72 instructions rounds the sum once, 2^-23."""
+    B, T, H = len(lens), 2, 16
+    bt, pages = tables(lens, 64, 41)
+    cache = make_cache("fp8", pages, 64, 42, oracle)
+    rows = cache.view(-1, 656)
+    rows[:, 512:528] = (rows[:, 512:528].contiguous().view(F32) * amp).view(torch.uint8)
+    q = (torch.randn(B, T, H, 576, generator=gen(43), device=DEV) * 16.0).to(BF)
+    mask = random_masks(dsa, B, T, 44)
+    o, lse = torch.empty(B, T, H, 512, dtype=BF, device=DEV), torch.empty(B, T, H, device=DEV)
+    dsa.tree_mla_decode(o, lse, q, cache, bt, torch.tensor(lens, dtype=torch.int32, device=DEV), mask, SCALE)
+    ref = tree64(q, cache, bt, lens, mask, None, SCALE)
+    check_tree(o, lse, ref, "fp8")
+    k2 = values64(cache)[:, :512].square().mean(0)
+    norm = (q[..., :512].double().square() @ k2).sqrt().max() * SCALE
+    rms = (lse.double() - ref[1]).square().mean().sqrt()
+    tol = float(step / 3 ** 0.5 * norm) + float(ref[1].abs().max()) * 2 * (1152 * 2.0 ** -25 + 72 * 2.0 ** -23)
+    assert float(rms) <= tol, (float(rms), tol)
