@@ -327,8 +327,10 @@ __device__ __forceinline__ uint4 dequant8(uint2 v, uint32_t cut) {
   return *reinterpret_cast<const uint4*>(x);
 }
 
-// With one of the two parts, as f16 (hi: exact): the two products' sum keeps the scale
-// to 2^-18, or to 2^-25 of the largest value where f16 runs out of exponents.
+// With one of the two parts, as f16 (hi: exact). lo has at most 2^-6 of the scale, so as
+// f16 it keeps the scale to 2^-18, and its product with a code is rounded by 2^-17 of
+// the value; a lo below 2^-14 (scales below 2^-7) is off by up to 2^-25, which is 2^-17
+// of a scale of 2^-8 and 2^-15 of the smallest, 2^-10, alike for the group's 128 values.
 __device__ __forceinline__ uint4 dequant8_part(uint2 v, __half part) {
   __half2 x[4];
   e4m3x4_to_half2x2(v.x, x[0], x[1]);
