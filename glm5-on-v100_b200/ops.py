@@ -649,7 +649,7 @@ def _gather_cache_impl(out, cache, block_table, cu_seq_lens, seq_starts):
         return
     _fits(n + 64, cache.size(-2), width)
     _launch(index, "dsa_gather_cache", out.data_ptr(), _DTYPE[out.dtype],
-            max(out.stride(0), width) if n == 1 else out.stride(0), n, cache.data_ptr(), fmt, cache.numel() // elems,
+            _row_stride(out, n), n, cache.data_ptr(), fmt, cache.numel() // elems,
             cache.size(-2), width, *pages, cu_seq_lens.data_ptr(), _ptr(seq_starts), B)
 
 

@@ -945,3 +945,13 @@ def test_tree_lse_of_peaked_rows(dsa, oracle, lens, amp, step):
     rms = (lse.double() - ref[1]).square().mean().sqrt()
     tol = float(step / 3 ** 0.5 * norm) + float(ref[1].abs().max()) * 2 * (1152 * 2.0 ** -25 + 72 * 2.0 ** -23)
     assert float(rms) <= tol, (float(rms), tol)
+
+
+@pytest.mark.parametrize("wide", [576, 580, 2000])
+def test_gather_into_one_row_of_any_stride(dsa, oracle, wide):
+    """A single output row's stride says nothing of its alignment."""
+    cache = make_cache("fp8", 2, 64, 2, oracle)
+    bt = torch.tensor([[1]], dtype=torch.int32, device=DEV)
+    buf = torch.full((1, wide), 9.0, dtype=BF, device=DEV)
+    dsa.gather_cache(buf[:, :576], cache, bt, torch.tensor([0, 1], dtype=torch.int32, device=DEV))
+    assert torch.equal(buf[:, :576], plain_rows(cache, BF)[64:65]) and bool((buf[:, 576:] == 9).all())
