@@ -1414,7 +1414,8 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
                   row_stride_ok(bt_stride, max_blocks) && row_stride_ok(mask_stride, T),
               DSA_ERR_INVALID, "tree_mla_decode: bad cache geometry or strides (page=%d max_blocks=%d rows=%lld)",
               page_size, max_blocks, (long long)n_kv_rows);
-  DSA_REQUIRE(std::isfinite(scale), DSA_ERR_INVALID, "tree_mla_decode: scale must be finite");
+  const float scale_log2 = (float)(std::fabs(scale) * 1.4426950408889634);
+  DSA_REQUIRE(std::isfinite(scale_log2), DSA_ERR_INVALID, "tree_mla_decode: scale must be finite, in f32 too");
   if (B == 0 || T == 0 || n_head == 0) return DSA_OK;
   DSA_REQUIRE(n_head <= 1024 && B <= 65535, DSA_ERR_UNSUPPORTED, "tree_mla_decode: at most 65535 requests of 1024 heads");
   DSA_REQUIRE(o && lse && q && seq_lens && tree_mask && (n_kv_rows == 0 || kv_cache) && (max_blocks == 0 || block_table),
@@ -1451,7 +1452,7 @@ extern "C" int dsa_tree_mla_decode(void* o, int o_dtype, float* lse, const void*
   p.q_bf16 = q_dtype == DSA_BF16;
   p.o_bf16 = o_dtype == DSA_BF16;
   p.q_sign = scale < 0 ? 0x80008000u : 0u;
-  p.scale_log2 = (float)(std::fabs(scale) * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   const size_t need = tree_workspace(T, n_head, p.pairs);
   DSA_REQUIRE(workspace != nullptr && workspace_bytes >= need, DSA_ERR_WORKSPACE,
               "tree_mla_decode: workspace needs %zu bytes, got %zu", need, workspace_bytes);

@@ -244,3 +244,12 @@ def test_tree_wrapper_rounds_queries_to_the_cache_type(dsa, monkeypatch):
                                                      torch.ones(1, 2, dtype=i64), 1.0, draft_lens=lens)
             assert seen == dict(o=want, q=want, bt=i32, ln=i32, dl=None if lens is None else i32)
             assert o.dtype == want and o.shape == (1, 2, 3, 512) and lse.shape == (1, 2, 3)
+
+
+def test_tree_entry_refuses_scales_that_f32_cannot_hold(dsa):
+    """A finite double beyond f32 would make every score infinite or NaN."""
+    L, lib = dsa._lib, dsa._lib.lib()
+    for scale in (1e39, -1e300, 3e38, math.inf, -math.inf, math.nan):  # 3e38 log2(e) is past f32's 3.4e38
+        assert _tree(lib, B=0, scale=scale) == L.DSA_ERR_INVALID, scale
+    for scale in (0.0, -1.0, 1e-320, 1e30):
+        assert _tree(lib, B=0, scale=scale) == L.DSA_OK, scale
