@@ -23,6 +23,7 @@
 // (3.9 TB/s); 16 tokens: the call, 12 us of host time and 4 of the kernel.
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 
 #include "common.cuh"
 
@@ -190,7 +191,6 @@ extern "C" int dsa_rotary_embedding(void* out, int64_t out_tok_stride, int64_t o
   DSA_REQUIRE(width <= 2048, DSA_ERR_UNSUPPORTED, "rotary_embedding: heads are at most 2048 wide (got %d)", width);
   DSA_REQUIRE(n_tok <= (1 << 28) && n_head <= 65535, DSA_ERR_UNSUPPORTED, "rotary_embedding: too many tokens or heads");
   if (n_tok == 0 || n_head == 0) return DSA_OK;
-  DSA_REQUIRE(out && x && positions && cos_sin && max_pos > 0, DSA_ERR_INVALID, "rotary_embedding: null pointer");
   // no two of out's heads share an element: the nearer of its strides spans a head,
   // the other all the heads at the nearer one
   const int64_t st = n_tok > 1 ? out_tok_stride : INT64_MAX, sh = n_head > 1 ? out_head_stride : INT64_MAX;
@@ -200,6 +200,21 @@ extern "C" int dsa_rotary_embedding(void* out, int64_t out_tok_stride, int64_t o
               (long long)out_head_stride);
   const int item = dtype == DSA_F32 ? 4 : 2;
   const int e = 16 / item;
+  // x moved against out by `d` elements, with out's strides: a head of one meets a head
+  // of the other when d lies within a width of a distance between two heads
+  if ((n_tok == 1 || out_tok_stride == x_tok_stride) && (n_head == 1 || out_head_stride == x_head_stride)) {
+    const int64_t d = ((int64_t)reinterpret_cast<uintptr_t>(out) - (int64_t)reinterpret_cast<uintptr_t>(x)) / item;
+    const int64_t n_far = st <= sh ? n_head : n_tok;
+    bool meet = false;
+    for (int64_t f = d / far - 1; d != 0 && f <= d / far + 1; ++f) {
+      if (std::abs(f) >= n_far) continue;
+      const int64_t r = d - (f == 0 ? 0 : f * far);
+      for (int64_t k = r / near - 1; k <= r / near + 1; ++k)
+        meet |= std::abs(k) < n_near && std::abs(r - (k == 0 ? 0 : k * near)) < width;
+    }
+    DSA_REQUIRE(!meet, DSA_ERR_INVALID, "rotary_embedding: out overlaps x without being x");
+  }
+  DSA_REQUIRE(out && x && positions && cos_sin && max_pos > 0, DSA_ERR_INVALID, "rotary_embedding: null pointer");
   auto is16 = [&](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = is16(out) && is16(x) && is16(cos_sin) && out_tok_stride % e == 0 && out_head_stride % e == 0 &&
                    x_tok_stride % e == 0 && x_head_stride % e == 0 && width % e == 0 && rope_offset % e == 0 &&

@@ -484,7 +484,8 @@ int dsa_gather_cache(void* out, int out_dtype, int64_t out_stride, int n_out,
  * (i, i + rotary_dim/2) with rope_neox; the rest of the head is copied. x and
  * out [n_tok, n_head, width] in dtype (f16, bf16 or f32), unit inner stride,
  * token and head strides in elements. out may be x itself (same strides) or
- * must not overlap it. Same arithmetic as the cache writers. width <= 2048. */
+ * must not overlap it (refused when the strides are the same). Same arithmetic
+ * as the cache writers. width <= 2048. */
 int dsa_rotary_embedding(void* out, int64_t out_tok_stride,
                          int64_t out_head_stride, const void* x,
                          int64_t x_tok_stride, int64_t x_head_stride,

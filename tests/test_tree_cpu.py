@@ -253,3 +253,21 @@ def test_tree_entry_refuses_scales_that_f32_cannot_hold(dsa):
         assert _tree(lib, B=0, scale=scale) == L.DSA_ERR_INVALID, scale
     for scale in (0.0, -1.0, 1e-320, 1e30):
         assert _tree(lib, B=0, scale=scale) == L.DSA_OK, scale
+
+
+def test_rotary_entry_refuses_an_out_that_overlaps_x(dsa):
+    """Every shift of x against out, with strides in both orders, against sets of
+    elements. Calls that are to be served have no table, which is refused later on."""
+    L, lib = dsa._lib, dsa._lib.lib()
+    P = ctypes.c_void_p
+
+    def refused(n, h, st, sh, w, shift):
+        lib.dsa_rotary_embedding(P(1 << 20), st, sh, P((1 << 20) - 2 * shift), st, sh, 1, P(1024), P(1024), 0, 4, 0, 0, n, h, w,
+                                 None)
+        return b"overlaps x" in lib.dsa_last_error()
+
+    for n, h, st, sh, w in [(3, 4, 40, 9, 8), (3, 4, 9, 30, 8), (1, 3, 5, 16, 4), (4, 1, 6, 77, 6), (1, 1, 0, 0, 8), (2, 2, 64, 32, 8)]:
+        heads = {t * (st if n > 1 else 0) + k * (sh if h > 1 else 0) + e for t in range(n) for k in range(h) for e in range(w)}
+        for shift in range(-170, 171):
+            meet = shift != 0 and any(p - shift in heads for p in heads)
+            assert refused(n, h, st, sh, w, shift) == meet, (n, h, st, sh, w, shift)
