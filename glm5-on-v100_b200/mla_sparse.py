@@ -97,6 +97,11 @@ def forward_mqa_tree(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch
     context and its own ancestors in one pass over the paged latent cache
     (where expand_spec_rows turns a line of drafts into independent rows).
 
+    The attention is dense: every position of the context is attended, not the
+    top-k that the indexer picks. It equals forward_mqa_sparse over a line of
+    drafts only in contexts of up to top-k positions; beyond, a model decoded
+    with the sparse attention is verified against another distribution.
+
     q [B, T, H, 576], or the step's tokens [B * T, H, 576] with tree_mask [B,
     T]; f16 or bf16 (bf16 with a bf16 cache). Other types are rounded to bf16
     for a bf16 cache and else to f16, where values beyond 65504 are infinite

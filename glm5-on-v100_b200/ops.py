@@ -821,11 +821,11 @@ def indexer_qk_store(q_out, weights_out, kv_cache, q, kw, slot_mapping, ln_weigh
 
 
 def tree_mla_decode(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, scale: float, draft_lens=None) -> None:
-    """Attention of a tree of drafts over the whole latent cache: q [B, T, H,
-    576] -> o [B, T, H, 512], lse [B, T, H] f32. seq_lens counts the drafts
-    (the last draft_lens[b], default T, positions of a request); bit j of
-    tree_mask[b, i] (int64, T <= 64) lets draft i see draft j, the positions
-    before the drafts are seen by all. Rows that see nothing and rows past
+    """Dense attention of a tree of drafts over the whole latent cache (no top-k
+    selection, unlike sm70_sparse_mla_decode): q [B, T, H, 576] -> o [B, T, H,
+    512], lse [B, T, H] f32. seq_lens counts the drafts (the last draft_lens[b],
+    default T, positions of a request); bit j of tree_mask[b, i] (int64, T <=
+    64) lets draft i see draft j, the positions before the drafts are seen by all. Rows that see nothing and rows past
     draft_lens[b] become o = 0, lse = -inf."""
     _op("tree_mla_decode")(o, lse, q, kv_cache, block_table, seq_lens, tree_mask, draft_lens, float(scale))
 
@@ -834,7 +834,9 @@ def commit_draft_rows(caches, block_table, seq_lens, accepted, draft_lens) -> No
     """After verification: in every cache of the list (latent or indexer-K, one
     geometry and block table; one launch for up to 128 layers) the k-th
     accepted draft's row moves from position pre + accepted[b, k] to pre + k,
-    pre = seq_lens[b] - draft_lens[b]. accepted int32 [B, n <= 64], -1 padded."""
+    pre = seq_lens[b] - draft_lens[b]. accepted int32 [B, n <= 64], -1 padded;
+    draft_lens as in the attention, none above its T. The requests' drafts lie
+    in cache rows of their own."""
     _op("commit_draft_rows")(caches, block_table, seq_lens, accepted, draft_lens)
 
 
