@@ -60,9 +60,9 @@
 // multiplied too (fewer keys average less). N(0, 1) rows, 8 heads x 16 drafts, 8
 // requests of 13,824 to 24,576 positions: one product 74 us and lse within 1.1e-6, two
 // 100 us and 1.5e-7; 64 heads x 8 drafts, 4 x 24,576: 133 us and 9.5e-7, 188 us and
-// 1.7e-7. V's values are rounded to f16 once beyond 1024 positions (o 14% farther from
-// 64 bits than with exact ones, f16 o), a bf16 cache's probabilities to bf16, as both
-// operands of a product have one type (o 14% too). bf16 q is shifted by a power of two
+// 1.7e-7. V's values are rounded to f16 once beyond 1024 positions (f16 o 14 - 45%
+// farther from 64 bits than the plain form's), a bf16 cache's probabilities to bf16, as both
+// operands of a product have one type (o 14 - 25% farther). bf16 q is shifted by a power of two
 // per row into f16's range, which the row's scale undoes exactly.
 // Probabilities are 2^(z - m) with m 7 below the running maximum, in log2 units, and
 // m moves only when a score exceeds it by 15: P <= 2^15 uses f16's range at both ends,
@@ -72,16 +72,19 @@
 // f32 accumulator, which cuts a product two bits below its own last place.
 //
 // Measured (times with the merge): 32 drafts x 64 heads over 131,072 positions, fp8
-// 572 - 586 us = 1.0 PFLOP/s, 62% of the rate of a plain matrix product (690 in a
-// long loop, whose clocks the power limit lowers), 16-bit cache 544 us. A tile
+// 584 - 598 us = 1.0 PFLOP/s, 61% of the rate of a plain matrix product (686 in a
+// long loop, whose clocks the power limit lowers), 16-bit cache 584 - 608 us. A tile
 // takes a CTA 5000 cycles, the tensor cores 2700 of them: the bound is the
 // producers' chain, K and V of a tile after one another, each store (8 x 8 codes a
 // lane) 1300 cycles of issue and latency and 700 of waits and fences. With two
 // products K is stored twice, 7800 cycles. The code of the loops counts: an SM's
 // instruction cache misses go to a cache that several share, and took 76% of its
 // rate before the loops were cut (23% now), so the usual path has no calls, the
-// rare ones (scales out of f16's range, remainders) are rolled, and a wait is three
-// instructions.
+// others (remainders, scales below 2^-10 or above 128) are rolled, and a wait is three
+// instructions. A producer warp with one such scale among its tile's takes the rolled
+// path. N(0, 1) rows have none; rows a tenth as large, or with one of the four groups so
+// quiet, have them in every tile: 8 heads ragged 98 -> 182 us, 64 heads 189 -> 401,
+// long context 598 -> 1450; with 1% of the rows all zero 130, 276 and 813.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -303,8 +306,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // How codes are expanded to f16: the product code * scale rounded once, by f16
-// arithmetic where the scale's parts and the products stay in f16's range, by f32
-// elsewhere.
+// arithmetic where the scale's parts and the products stay in f16's range (groups whose
+// largest value lies between 0.44 and 57344), by f32 elsewhere: twice the time, figures
+// above.
 __device__ __forceinline__ bool fast_scale(float sc) { return sc >= 0x1p-10f && sc <= 128.0f; }
 
 // A scale cut in two f16 parts, hi (low half word) with 7 significant bits and lo the
@@ -365,7 +369,7 @@ __device__ __forceinline__ uint4 rest8(uint2 v, uint32_t cut, uint32_t small) {
 }
 
 // The same for any scale, or with `rest` what that rounding left, itself rounded.
-// Rare: kept out of the loops' code, which has to fit the instruction cache.
+// Kept out of the loops' code, which has to fit the instruction cache.
 __device__ __noinline__ uint4 dequant8_any(uint2 v, float sc, bool rest, bool fast) {
   if (fast) return rest8(v, cut_scale(sc), cut_rest(sc));
   __half2 x[4];
